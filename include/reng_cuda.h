@@ -293,6 +293,104 @@ int reng_model_time_kernels_rows(reng_model *m, int rows, int iters, float *ms_o
 int reng_gemm_bf16(const uint16_t *w, int rows, int K, const uint16_t *x, int M, float *y, int splits,
                    int iters, float *ms_out, int mem);
 
+/* ============================================ 8-bit block operators ===
+ * The operators of an 8-bit (W8A8) path: FP8 codes with one f32 scale per
+ * block of 128, the product of two such matrices, and the step between two
+ * decoder blocks that writes them.  No counterpart in the reference, whose
+ * FP8 is per-row and weight-only (crates/reng-fp8).
+ *
+ * All pointers are device pointers on the current device; the calls are
+ * asynchronous on `stream`, allocate nothing and may be captured into a CUDA
+ * graph.  Matrices are row-major with their own row pitch (ld*, in elements)
+ * of at least a row.  No output may overlap an input or another output,
+ * except where a call says so.  0 rows: nothing is written.
+ */
+#define RENG_TYPE_BF16 0 /* bf16 bit patterns */
+#define RENG_TYPE_F32 1
+
+/*
+ * Quantize x [rows, cols] (`type`) to codes [rows, cols] with one scale per
+ * block: block_rows 1: per 1 x 128 group of a row (activations), scales
+ * [rows, ceil(cols / 128)]; block_rows 128: per 128 x 128 block (weights),
+ * scales [ceil(rows / 128), ceil(cols / 128)].  A block's scale is its absmax
+ * / max_finite (1.0 for a block of zeros, never below the smallest normal
+ * f32; NaN is never the absmax) and its codes encode(x / scale) by the rules of reng_fp8_quantize: an infinity
+ * makes its own block's scale infinite, and itself and NaN code to NaN.  Any
+ * cols, pitch and element alignment; 16-byte aligned rows are read wide.
+ */
+int reng_fp8_quantize_blocks(const void *x, int type, int64_t rows, int64_t cols, int64_t ldx,
+                             int block_rows, int fmt, uint8_t *codes, int64_t ldc, float *scales,
+                             int64_t lds, void *stream);
+
+/*
+ * The same, in 1 x 128 groups, of h = gate / (1 + exp(-gate)) * up, computed
+ * in f32 and rounded once, to the codes: the input of a down projection.
+ * gate and up are [rows, cols] with one row pitch ldx (the two halves of a
+ * gate/up projection's output rows: up = gate + cols, ldx = 2 cols).
+ */
+int reng_fp8_swiglu_quantize(const void *gate, const void *up, int type, int64_t rows, int64_t cols,
+                             int64_t ldx, int fmt, uint8_t *codes, int64_t ldc, float *scales,
+                             int64_t lds, void *stream);
+
+/*
+ * y[m][n] = sum_b x_scales[m][b] * w_scales[n / 128][b] * sum_{k in block b} x[m][k] * w[n][k]
+ *
+ * x codes [M, K] with 1 x 128 scales, w codes [N, K] with 128 x 128 scales,
+ * y [M, N] in y_type.  Products and sums in f32, scales applied to each
+ * block's sum in f32, one rounding to y_type.  Codes must start on a 16-byte
+ * boundary and have a pitch that is a multiple of 16 (RENG_E_INVAL); M, N and
+ * K are otherwise free up to 2^30.  The formats of x and w are independent.
+ * E4M3 codes are read with the tensor core's table: the codes this library's
+ * encoders write, and NaN, mean what reng_fp8_decode says, but 0x78..0x7e
+ * (reserved there, never written) read as 256..448.
+ * Deterministic: the order of the sums does not depend on timing.
+ */
+int reng_gemm_fp8_blocks(const uint8_t *x, int64_t ldx, const float *x_scales, int64_t ldsx, int x_fmt,
+                         const uint8_t *w, int64_t ldw, const float *w_scales, int64_t ldsw, int w_fmt,
+                         int64_t M, int64_t N, int64_t K, void *y, int y_type, int64_t ldy,
+                         void *stream);
+
+/* Whether a product of reng_gemm_fp8_blocks on the current device gave up on
+ * a bounded device wait since the last call of this function: RENG_E_TIMEOUT
+ * (its results are invalid), else RENG_OK.  Synchronises with the device. */
+int reng_gemm_fp8_blocks_status(void);
+
+/* What h is written as. */
+#define RENG_NORM_NONE 0 /* y only */
+#define RENG_NORM_BF16 1
+#define RENG_NORM_F32 2
+#define RENG_NORM_E4M3 3 /* codes + 1 x 128 scales */
+#define RENG_NORM_E5M2 4
+
+/* The step between two decoder blocks (reng_block_norm). */
+typedef struct reng_block_norm_desc {
+    const void *branch;     /* [rows, cols] the block's output; NULL: y is residual, unwritten */
+    const void *residual;   /* [rows, cols] the residual stream */
+    const void *gate;       /* [rows, cols] multiplier of the branch, or [cols] with ld_gate 0; NULL: 1 */
+    const float *post_gain; /* [cols] gain of the norm after the block; NULL: no such norm */
+    const float *pre_gain;  /* [cols] gain of the norm before the next block; NULL: 1 */
+    void *y;                /* [rows, cols] new residual stream, residual_type; may be `residual` itself */
+    void *h;                /* [rows, cols] the next block's input (unused with RENG_NORM_NONE) */
+    float *h_scales;        /* [rows, ceil(cols / 128)] with RENG_NORM_E4M3 / E5M2 */
+    int64_t rows, cols;
+    int64_t ld_branch, ld_residual, ld_gate, ld_y, ld_h, ld_scales;
+    int32_t branch_type, residual_type, gate_type; /* RENG_TYPE_* */
+    int32_t out;            /* RENG_NORM_* */
+    float scale;            /* the branch's residual scale */
+    float eps;              /* of both norms */
+} reng_block_norm_desc;
+
+/*
+ * Per row, with r(v) = 1 / sqrt(mean(v^2) + eps):
+ *   u = branch;  u = u * r(u) * post_gain  (with post_gain);  u = u * gate  (with gate)
+ *   y = round(residual + scale * u)        to residual_type
+ *   h = y * r(y) * pre_gain                from y as rounded
+ * computed in f32; h is rounded once, to its type or to FP8 codes of
+ * 1 x 128 groups (as reng_fp8_quantize_blocks).  Without a branch only h is
+ * written, from residual.  A desc with neither branch nor h is refused.
+ */
+int reng_block_norm(const reng_block_norm_desc *desc, void *stream);
+
 /* ============================================== tensor parallelism ===
  * Replaces hccl::Rank::join's unique-id exchange (hccl.rs:580-637): rank 0
  * creates the id, the caller ships it to the other ranks (a file, a store),

@@ -11,6 +11,13 @@ pub const RENG_FP8_E5M2: c_int = 1;
 pub const RENG_SCALING_PCS: c_int = 0;
 pub const RENG_SCALING_HW: c_int = 1;
 pub const RENG_SCALING_UNIT: c_int = 2;
+pub const RENG_TYPE_BF16: c_int = 0;
+pub const RENG_TYPE_F32: c_int = 1;
+pub const RENG_NORM_NONE: i32 = 0;
+pub const RENG_NORM_BF16: i32 = 1;
+pub const RENG_NORM_F32: i32 = 2;
+pub const RENG_NORM_E4M3: i32 = 3;
+pub const RENG_NORM_E5M2: i32 = 4;
 
 #[repr(C)]
 pub struct reng_model { _private: [u8; 0] }
@@ -43,6 +50,17 @@ pub struct reng_step_times {
 pub struct reng_device_info {
     pub ordinal: i32, pub name: [c_char; 96], pub pci_bus_id: [c_char; 32],
     pub total_bytes: u64, pub sm_count: i32, pub cc_major: i32, pub cc_minor: i32,
+}
+
+#[repr(C)]
+pub struct reng_block_norm_desc {
+    pub branch: *const c_void, pub residual: *const c_void, pub gate: *const c_void,
+    pub post_gain: *const f32, pub pre_gain: *const f32,
+    pub y: *mut c_void, pub h: *mut c_void, pub h_scales: *mut f32,
+    pub rows: i64, pub cols: i64, pub ld_branch: i64, pub ld_residual: i64,
+    pub ld_gate: i64, pub ld_y: i64, pub ld_h: i64, pub ld_scales: i64,
+    pub branch_type: i32, pub residual_type: i32, pub gate_type: i32,
+    pub out: i32, pub scale: f32, pub eps: f32,
 }
 
 #[link(name = "reng_cuda")]
@@ -86,4 +104,16 @@ extern "C" {
     pub fn reng_model_tp_exchange(m: *mut reng_model, kind: *mut c_int) -> c_int;
     pub fn reng_model_time_exchange(m: *mut reng_model, iters: c_int, ms_out: *mut f32) -> c_int;
     pub fn reng_tp_peer_wait_check(device: c_int) -> c_int;
+    pub fn reng_fp8_quantize_blocks(x: *const c_void, ty: c_int, rows: i64, cols: i64, ldx: i64,
+                                    block_rows: c_int, fmt: c_int, codes: *mut u8, ldc: i64,
+                                    scales: *mut f32, lds: i64, stream: *mut c_void) -> c_int;
+    pub fn reng_fp8_swiglu_quantize(gate: *const c_void, up: *const c_void, ty: c_int, rows: i64, cols: i64,
+                                    ldx: i64, fmt: c_int, codes: *mut u8, ldc: i64, scales: *mut f32,
+                                    lds: i64, stream: *mut c_void) -> c_int;
+    pub fn reng_gemm_fp8_blocks(x: *const u8, ldx: i64, x_scales: *const f32, ldsx: i64, x_fmt: c_int,
+                                w: *const u8, ldw: i64, w_scales: *const f32, ldsw: i64, w_fmt: c_int,
+                                m: i64, n: i64, k: i64, y: *mut c_void, y_type: c_int, ldy: i64,
+                                stream: *mut c_void) -> c_int;
+    pub fn reng_gemm_fp8_blocks_status() -> c_int;
+    pub fn reng_block_norm(desc: *const reng_block_norm_desc, stream: *mut c_void) -> c_int;
 }

@@ -30,45 +30,10 @@
 #include <vector>
 
 #include "common.cuh"
+#include "fp8_encode.cuh"
 #include "fp8_product.h"
 
 namespace reng {
-
-// Two f32 -> two E4M3 codes (first argument in the low byte).
-__device__ __forceinline__ uint32_t cvt_e4m3x2(float lo, float hi) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-__device__ __forceinline__ uint32_t cvt_e5m2x2(float lo, float hi) {
-    uint16_t r;
-    asm("cvt.rn.satfinite.e5m2x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
-template <int FMT>
-__device__ __forceinline__ uint32_t encode2(float a, float b) {
-    uint32_t c;
-    if (FMT == RENG_FP8_E4M3) {
-        c = cvt_e4m3x2(fminf(fmaxf(a, -240.0f), 240.0f), fminf(fmaxf(b, -240.0f), 240.0f));
-    } else {
-        c = cvt_e5m2x2(a, b);
-    }
-    if (isnan(a)) c = (c & 0xff00u) | ((__float_as_uint(a) >> 24) & 0x80u) | 0x7fu;
-    if (isnan(b)) c = (c & 0x00ffu) | ((((__float_as_uint(b) >> 24) & 0x80u) | 0x7fu) << 8);
-    return c;
-}
-
-// x / s as the reference's host computes it: IEEE division; a NaN weight
-// comes through as itself, sign included (x86 returns the NaN operand; GPU
-// arithmetic would return its canonical positive NaN), and a NaN generated
-// by the division is x86's default NaN, whose sign bit is set.
-__device__ __forceinline__ float div_host(float x, float s) {
-    if (isnan(x)) return x;
-    float q = __fdiv_rn(x, s);
-    if (isnan(q)) q = __uint_as_float(0xffc00000u);
-    return q;
-}
 
 // The same quotient without the division (fp8_product.h: Markstein's
 // correction of x * RN(1 / s)), for rows fp8_product_ok admits.

@@ -1,0 +1,48 @@
+// What the standalone operators share (fp8_blocks.cu, block_norm.cu,
+// gemm_fp8.cu): argument rules and the launch.
+#pragma once
+#include "common.cuh"
+
+namespace reng {
+
+inline int64_t ops_groups(int64_t cols) { return (cols + 127) / 128; }
+
+// A row pitch that holds its row, in a matrix whose extent (and that of any
+// index formed from it) stays far inside 64 bits.
+inline bool ops_pitch_ok(int64_t rows, int64_t cols, int64_t ld) {
+    constexpr int64_t kMax = (int64_t)1 << 40;
+    return rows <= kMax && cols <= kMax && ld >= cols && ld <= kMax && (rows == 0 || ld <= kMax / rows);
+}
+
+// Whether a base and a byte pitch keep every row on an n-byte boundary.
+inline bool ops_aligned(const void* p, int64_t pitch_bytes, int n) {
+    return (uintptr_t)p % (uintptr_t)n == 0 && pitch_bytes % n == 0;
+}
+
+// SMs of the current device.
+inline cudaError_t current_sms(int* sms) {
+    int dev = 0;
+    const cudaError_t e = cudaGetDevice(&dev);
+    *sms = e == cudaSuccess ? num_sms(dev) : 0;
+    return e;
+}
+
+// Launch with the programmatic-serialization attribute: the kernel may start
+// while its predecessor drains, and waits for it (pdl_wait) before it touches
+// memory.
+template <typename... P, typename... A>
+cudaError_t launch_ops(void (*k)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, A... args) {
+    cudaLaunchConfig_t cfg = {};
+    cudaLaunchAttribute attr[1];
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, k, args...);
+}
+
+}  // namespace reng

@@ -27,6 +27,14 @@ RENG_SCALING_PCS = 0
 RENG_SCALING_HW = 1
 RENG_SCALING_UNIT = 2
 
+RENG_TYPE_BF16 = 0
+RENG_TYPE_F32 = 1
+RENG_NORM_NONE = 0
+RENG_NORM_BF16 = 1
+RENG_NORM_F32 = 2
+RENG_NORM_E4M3 = 3
+RENG_NORM_E5M2 = 4
+
 RENG_WEIGHTS_BF16 = 0
 RENG_WEIGHTS_FP8_E4M3 = 1
 
@@ -69,6 +77,15 @@ class DeviceInfo(C.Structure):
                 ("cc_minor", C.c_int32)]
 
 
+class BlockNormDesc(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in
+                ("branch", "residual", "gate", "post_gain", "pre_gain", "y", "h", "h_scales")] + \
+               [(n, C.c_int64) for n in
+                ("rows", "cols", "ld_branch", "ld_residual", "ld_gate", "ld_y", "ld_h", "ld_scales")] + \
+               [(n, C.c_int32) for n in ("branch_type", "residual_type", "gate_type", "out")] + \
+               [("scale", C.c_float), ("eps", C.c_float)]
+
+
 # Every exported symbol with its argument types (restype int unless noted).
 _P = C.c_void_p
 SIGNATURES = {
@@ -97,6 +114,14 @@ SIGNATURES = {
     "reng_model_time_kernels": ([_P, C.c_int, _P], C.c_int),
     "reng_model_time_kernels_rows": ([_P, C.c_int, C.c_int, _P], C.c_int),
     "reng_model_time_exchange": ([_P, C.c_int, _P], C.c_int),
+    "reng_fp8_quantize_blocks": ([_P, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int, C.c_int, _P, C.c_int64,
+                                  _P, C.c_int64, _P], C.c_int),
+    "reng_fp8_swiglu_quantize": ([_P, _P, C.c_int, C.c_int64, C.c_int64, C.c_int64, C.c_int, _P, C.c_int64, _P,
+                                  C.c_int64, _P], C.c_int),
+    "reng_gemm_fp8_blocks": ([_P, C.c_int64, _P, C.c_int64, C.c_int, _P, C.c_int64, _P, C.c_int64, C.c_int,
+                              C.c_int64, C.c_int64, C.c_int64, _P, C.c_int, C.c_int64, _P], C.c_int),
+    "reng_gemm_fp8_blocks_status": ([], C.c_int),
+    "reng_block_norm": ([_P, _P], C.c_int),
     "reng_tp_unique_id": ([_P], C.c_int),
     "reng_gemm_bf16": ([_P, C.c_int, C.c_int, _P, C.c_int, _P, C.c_int, C.c_int, _P, C.c_int], C.c_int),
 }

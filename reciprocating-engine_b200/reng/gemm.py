@@ -5,6 +5,13 @@ patterns (the projection kernel of steps with more than 8 rows).
 
 w_bits: uint16 [rows][K] bf16 bits, x_bits: uint16 [M][K] (1 <= M <= 1024,
 N-tiles of 256 rows beyond 256; K % 8 == 0).  iters > 0 also times the kernel alone (mean ms per launch).
+
+And the block-scaled FP8 product on torch CUDA tensors:
+
+    y = gemm_fp8_blocks(x, x_scales, w, w_scales)
+
+with x from fp8.quantize_blocks(.., 1) / fp8.swiglu_quantize /
+norm.block_norm_fp8 and w from fp8.quantize_blocks(.., 128).
 """
 import ctypes as C
 
@@ -25,3 +32,32 @@ def gemm_bf16(w_bits, x_bits, splits=0, iters=0):
     _lib.call("reng_gemm_bf16", w.ctypes.data, rows, K, x.ctypes.data, M, y.ctypes.data, splits, iters,
               C.byref(ms), _lib.RENG_MEM_HOST)
     return y, float(ms.value)
+
+
+def gemm_fp8_blocks(x, x_scales, w, w_scales, out=None, dtype=None, x_fmt=_lib.RENG_FP8_E4M3,
+                    w_fmt=_lib.RENG_FP8_E4M3, stream=None):
+    """y[m][n] = sum_b x_scales[m][b] w_scales[n / 128][b] sum_{k in b} x[m][k] w[n][k].
+
+    x uint8 codes [M, K] with scales [M, ceil(K / 128)], w uint8 codes [N, K]
+    with scales [ceil(N / 128), ceil(K / 128)]; rows start on 16 bytes
+    (fp8.quantize_blocks lays them out so).  y [M, N] is `out`, or a new
+    tensor of `dtype` (bf16 by default, or f32)."""
+    import torch
+    from ._tensors import TYPES, call, groups, matrix
+    dev = x.device
+    u8, f32 = (torch.uint8,), (torch.float32,)
+    ldx = matrix(x, "x", u8, dev)
+    M, K = x.shape
+    N = w.shape[0] if w.dim() == 2 else 0
+    ldw = matrix(w, "w", u8, dev, (N, K))
+    kb = groups(K)
+    ldsx = matrix(x_scales, "x_scales", f32, dev, (M, kb))
+    ldsw = matrix(w_scales, "w_scales", f32, dev, (groups(N), kb))
+    if out is None:
+        out = torch.empty((M, N), dtype=dtype or torch.bfloat16, device=dev)
+    elif dtype is not None and out.dtype != dtype:
+        raise ValueError("out is %s, not %s" % (out.dtype, dtype))
+    ldy = matrix(out, "out", TYPES, dev, (M, N))
+    call(dev, stream, "reng_gemm_fp8_blocks", x.data_ptr(), ldx, x_scales.data_ptr(), ldsx, x_fmt, w.data_ptr(), ldw,
+         w_scales.data_ptr(), ldsw, w_fmt, M, N, K, out.data_ptr(), TYPES[out.dtype], ldy)
+    return out
