@@ -14,6 +14,7 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 #include "fp8_encode.cuh"
 #include "ops.cuh"
@@ -34,262 +35,288 @@ struct NormArgs {
     float scale, eps;
 };
 
-__device__ __forceinline__ int esize(int type) { return type == RENG_TYPE_BF16 ? 2 : 4; }
-
-// 8 values of a row whose type is known at run time (the branch is uniform).
-// Plain loads: y may be written over residual.
-template <bool VEC>
-__device__ __forceinline__ void load8t(const void* base, int type, int64_t elem, int64_t c, int64_t cols,
-                                       float (&v)[8]) {
-    if (VEC) {
-        if (type == RENG_TYPE_BF16) {
-            const uint4 u = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(base) + elem + c);
-            v[0] = bf16lo(u.x), v[1] = bf16hi(u.x), v[2] = bf16lo(u.y), v[3] = bf16hi(u.y);
-            v[4] = bf16lo(u.z), v[5] = bf16hi(u.z), v[6] = bf16lo(u.w), v[7] = bf16hi(u.w);
-        } else {
-            const float4* p = reinterpret_cast<const float4*>(static_cast<const float*>(base) + elem + c);
-            const float4 a = p[0], b = p[1];
-            v[0] = a.x, v[1] = a.y, v[2] = a.z, v[3] = a.w, v[4] = b.x, v[5] = b.y, v[6] = b.z, v[7] = b.w;
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        v[i] = 0.f;
-        if (c + i < cols)
-            v[i] = type == RENG_TYPE_BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(base)[elem + c + i])
-                                          : static_cast<const float*>(base)[elem + c + i];
-    }
-}
-
-template <bool VEC>
-__device__ __forceinline__ void store8t(void* base, int type, int64_t elem, int64_t c, int64_t cols,
-                                        const float (&v)[8]) {
-    if (VEC) {
-        if (type == RENG_TYPE_BF16) {
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + elem + c) =
-                make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                           pack_bf16x2(v[6], v[7]));
-        } else {
-            float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + elem + c);
-            p[0] = make_float4(v[0], v[1], v[2], v[3]);
-            p[1] = make_float4(v[4], v[5], v[6], v[7]);
-        }
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (c + i < cols) {
-            if (type == RENG_TYPE_BF16)
-                static_cast<uint16_t*>(base)[elem + c + i] = f32_to_bf16_bits(v[i]);
-            else
-                static_cast<float*>(base)[elem + c + i] = v[i];
-        }
-}
-
 // Sum over the CTA, the same bits on every thread (warps added in order).
-__device__ __forceinline__ float cta_sum(float v, float* red) {
+// `red` alternates between two buffers, so one barrier is enough: a buffer is
+// written again only after the barrier of the other's sum.
+__device__ __forceinline__ float cta_sum(float v, float (&red)[2][32], int& turn) {
     v = warp_sum(v);
     const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    if ((threadIdx.x & 31) == 0) red[warp] = v;
+    float* r = red[turn];
+    turn ^= 1;
+    if ((threadIdx.x & 31) == 0) r[warp] = v;
     __syncthreads();
     float s = 0.f;
-    for (int w = 0; w < nw; w++) s += red[w];
-    __syncthreads();
+    for (int w = 0; w < nw; w++) s += r[w];
     return s;
 }
 
 __device__ __forceinline__ float inv_rms(float sum, float n, float eps) { return 1.0f / sqrtf(sum / n + eps); }
 
-// h of 8 columns; every lane of the warp calls it (the FP8 groups shuffle).
+// The 4 groups of a warp tile of one row: the first column of the lane's
+// values in each (VEC: in its own).
 template <bool VEC>
-__device__ __forceinline__ void emit(const NormArgs& a, int64_t row, int64_t c, bool live, float inv,
-                                     const float (&y)[8]) {
-    float h[8];
-    float m = 0.f;
+struct Tile {
+    static constexpr int G = VEC ? 1 : kTileGroups;
+    int64_t c[G];
+    bool live[G];
+    __device__ __forceinline__ Tile(int64_t tile, int64_t cols) {
+        const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < 8; i++) h[i] = 0.f;
-    if (live) {
-        if (a.pre) {
-            load8t<VEC>(a.pre, RENG_TYPE_F32, 0, c, a.cols, h);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 8; i++) h[i] = 1.f;
+        for (int g = 0; g < G; g++) {
+            c[g] = tile * (kTileGroups * kFp8Group) + (VEC ? lane * 16 : g * kFp8Group);
+            live[g] = c[g] < cols;
         }
-#pragma unroll
-        for (int i = 0; i < 8; i++) h[i] = c + i < a.cols ? y[i] * inv * h[i] : 0.f;
     }
-    if (a.out == OUT_BF16 || a.out == OUT_F32) {
-        if (live) store8t<VEC>(a.h, a.out == OUT_BF16 ? RENG_TYPE_BF16 : RENG_TYPE_F32, row * a.ldh, c, a.cols, h);
-        return;
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) m = fp8_absmax(m, h[i]);
-    m = half_warp_max(m);
-    if (!live) return;
-    uint8_t* codes = static_cast<uint8_t*>(a.h) + row * a.ldh;
-    float s;
-    uint2 q;
-    if (a.out == OUT_E4M3) {
-        s = fp8_block_scale<RENG_FP8_E4M3>(m);
-        q = fp8_encode8<RENG_FP8_E4M3>(h, s, m);
+};
+
+template <bool KEEP, int TYPE, bool VEC>
+__device__ __forceinline__ void tile_load(const void* base, int64_t at, const Tile<VEC>& t, int64_t cols,
+                                          Raw16<TYPE, VEC>& r) {
+    const char* row = static_cast<const char*>(base) + at * (TYPE == RENG_TYPE_BF16 ? 2 : 4);
+    raw_zero(r);
+    if constexpr (VEC) {
+        if (t.live[0]) raw_load<TYPE, KEEP>(row + t.c[0] * (TYPE == RENG_TYPE_BF16 ? 2 : 4), r);
     } else {
-        s = fp8_block_scale<RENG_FP8_E5M2>(m);
-        q = fp8_encode8<RENG_FP8_E5M2>(h, s, m);
-    }
-    if ((c & (kFp8Group - 1)) == 0) a.scales[row * a.lds + c / kFp8Group] = s;
-    store_codes8<VEC>(codes, c, a.cols, q);
-}
-
-// y of 8 columns from the branch values u (already normed and gained).
-template <bool VEC>
-__device__ __forceinline__ void residual8(const NormArgs& a, int64_t row, int64_t c, float (&u)[8], float (&y)[8]) {
-    if (a.gate) {
-        float g[8];
-        load8t<VEC>(a.gate, a.tg, row * a.ldg, c, a.cols, g);
 #pragma unroll
-        for (int i = 0; i < 8; i++) u[i] *= g[i];
-    }
-#pragma unroll
-    for (int i = 0; i < 8; i++) {
-        y[i] = fmaf(a.scale, u[i], y[i]);
-        if (a.tr == RENG_TYPE_BF16) y[i] = round_bf16(y[i]);
+        for (int g = 0; g < kTileGroups; g++)
+            if (t.live[g]) raw_load<TYPE, KEEP>(row, t.c[g], cols, g, r);
     }
 }
 
-// One CTA per row, the row in registers: C chunks of 8 columns per thread.
-template <int C>
-__global__ void __launch_bounds__(1024) k_block_norm(NormArgs a) {
-    __shared__ float red[32];
-    pdl_wait();
-    pdl_launch();
-    const int T = blockDim.x;
-    const float n = (float)a.cols;
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        float y[C][8], u[C][8];
+// The same as floats, of a type known at run time (uniform).
+template <bool KEEP, bool VEC>
+__device__ __forceinline__ void tile_floats(const void* base, int type, int64_t at, const Tile<VEC>& t, int64_t cols,
+                                            float (&v)[16]) {
+    if (type == RENG_TYPE_BF16) {
+        Raw16<RENG_TYPE_BF16, VEC> r;
+        tile_load<KEEP>(base, at, t, cols, r);
+        raw_floats(r, v);
+    } else {
+        Raw16<RENG_TYPE_F32, VEC> r;
+        tile_load<KEEP>(base, at, t, cols, r);
+        raw_floats(r, v);
+    }
+}
+
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void tile_store(void* base, int64_t at, const Tile<VEC>& t, int64_t cols,
+                                           const float (&v)[16]) {
+    if constexpr (VEC) {
+        if (!t.live[0]) return;
+        if (TYPE == RENG_TYPE_BF16) {
+            uint4* p = reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at + t.c[0]);
 #pragma unroll
-        for (int k = 0; k < C; k++) {
-            const int64_t c = ((int64_t)k * T + threadIdx.x) * 8;
+            for (int i = 0; i < 2; i++)
+                p[i] = make_uint4(bf16x2(v[8 * i], v[8 * i + 1]), bf16x2(v[8 * i + 2], v[8 * i + 3]),
+                                  bf16x2(v[8 * i + 4], v[8 * i + 5]), bf16x2(v[8 * i + 6], v[8 * i + 7]));
+        } else {
+            float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + at + t.c[0]);
 #pragma unroll
-            for (int i = 0; i < 8; i++) y[k][i] = 0.f, u[k][i] = 0.f;
-            if (c < a.cols) {
-                load8t<true>(a.residual, a.tr, row * a.ldr, c, a.cols, y[k]);
-                if (a.branch) load8t<true>(a.branch, a.tb, row * a.ldb, c, a.cols, u[k]);
+            for (int i = 0; i < 4; i++) p[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        }
+    } else {
+        const int lane = threadIdx.x & 31;
+#pragma unroll
+        for (int e = 0; e < 16; e++) {
+            const int64_t c = t.c[e >> 2] + 32 * (e & 3) + lane;
+            if (c < cols) {
+                if (TYPE == RENG_TYPE_BF16)
+                    static_cast<uint16_t*>(base)[at + c] = __bfloat16_as_ushort(__float2bfloat16_rn(v[e]));
+                else static_cast<float*>(base)[at + c] = v[e];
             }
         }
+    }
+}
+
+// u of a tile becomes the branch's share of y: normed, gained, gated; then
+// y += scale * u, rounded to y's type.
+template <int TR, bool VEC>
+__device__ __forceinline__ void tile_residual(const NormArgs& a, int64_t row, const Tile<VEC>& t, float inv,
+                                              float (&u)[16], float (&y)[16]) {
+    float g[16];
+    if (a.post) {
+        tile_floats<true, VEC>(a.post, RENG_TYPE_F32, 0, t, a.cols, g);
+#pragma unroll
+        for (int i = 0; i < 16; i++) u[i] = u[i] * inv * g[i];
+    }
+    if (a.gate) {
+        tile_floats<true, VEC>(a.gate, a.tg, row * a.ldg, t, a.cols, g);
+#pragma unroll
+        for (int i = 0; i < 16; i++) u[i] *= g[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 16; i++) y[i] = fmaf(a.scale, u[i], y[i]);
+    if (TR == RENG_TYPE_BF16) {
+#pragma unroll
+        for (int i = 0; i < 16; i += 2) {
+            const uint32_t p = bf16x2(y[i], y[i + 1]);
+            y[i] = bf16lo(p), y[i + 1] = bf16hi(p);
+        }
+    }
+}
+
+template <int FMT, bool VEC>
+__device__ __forceinline__ void tile_emit_fp8(const NormArgs& a, int64_t row, const Tile<VEC>& t,
+                                              const float (&h)[16]) {
+    constexpr int G = Tile<VEC>::G;
+    const int lane = threadIdx.x & 31;
+    uint32_t m[G];
+    bool odd;
+    tile_absmax<VEC>(h, m, odd);
+    group_max<VEC>(m);
+    float s[G];
+#pragma unroll
+    for (int g = 0; g < G; g++) s[g] = fp8_block_scale<FMT>(__uint_as_float(m[g]));
+    const uint4 q = tile_codes<FMT, VEC>(h, s, odd);
+    uint8_t* dst = static_cast<uint8_t*>(a.h) + row * a.ldh;
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        if (!t.live[g]) continue;
+        if ((lane & (VEC ? 7 : 31)) == 0) a.scales[row * a.lds + t.c[g] / kFp8Group] = s[g];
+        if constexpr (VEC) *reinterpret_cast<uint4*>(dst + t.c[g]) = q;
+        else store_codes(dst, t.c[g], a.cols, g == 0 ? q.x : g == 1 ? q.y : g == 2 ? q.z : q.w);
+    }
+}
+
+// h of a tile (whole warps: the FP8 groups shuffle).
+template <bool VEC>
+__device__ __forceinline__ void tile_emit(const NormArgs& a, int64_t row, const Tile<VEC>& t, float inv,
+                                          const float (&y)[16]) {
+    float h[16];
+    if (a.pre) {
+        tile_floats<true, VEC>(a.pre, RENG_TYPE_F32, 0, t, a.cols, h);
+#pragma unroll
+        for (int i = 0; i < 16; i++) h[i] = y[i] * inv * h[i];
+    } else {
+#pragma unroll
+        for (int i = 0; i < 16; i++) h[i] = y[i] * inv;
+    }
+    if (a.out == OUT_BF16) tile_store<RENG_TYPE_BF16, VEC>(a.h, row * a.ldh, t, a.cols, h);
+    else if (a.out == OUT_F32) tile_store<RENG_TYPE_F32, VEC>(a.h, row * a.ldh, t, a.cols, h);
+    else if (a.out == OUT_E4M3) tile_emit_fp8<RENG_FP8_E4M3, VEC>(a, row, t, h);
+    else tile_emit_fp8<RENG_FP8_E5M2, VEC>(a, row, t, h);
+}
+
+__device__ __forceinline__ float square_sum(const float (&v)[16], float s) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) s = fmaf(v[i], v[i], s);
+    return s;
+}
+
+// One CTA per row, the row in registers: C warp tiles per warp.
+template <int TB, int TR, bool VEC, int C>
+__global__ void __launch_bounds__(512) k_block_norm(NormArgs a) {
+    __shared__ float red[2][32];
+    int turn = 0;
+    const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    const float n = (float)a.cols;
+    pdl_wait();
+    pdl_launch();
+    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        float y[C][16], u[C][16];
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            const Tile<VEC> t(k * nw + warp, a.cols);
+            Raw16<TR, VEC> r;
+            Raw16<TB, VEC> b;
+            tile_load<false>(a.residual, row * a.ldr, t, a.cols, r);
+            if (a.branch) tile_load<false>(a.branch, row * a.ldb, t, a.cols, b);
+            raw_floats(r, y[k]);
+            if (a.branch) raw_floats(b, u[k]);
+        }
         if (a.branch) {
+            float inv = 1.f;
             if (a.post) {
                 float s = 0.f;
 #pragma unroll
-                for (int k = 0; k < C; k++)
-#pragma unroll
-                    for (int i = 0; i < 8; i++) s = fmaf(u[k][i], u[k][i], s);
-                const float inv = inv_rms(cta_sum(s, red), n, a.eps);
-#pragma unroll
-                for (int k = 0; k < C; k++) {
-                    const int64_t c = ((int64_t)k * T + threadIdx.x) * 8;
-                    if (c < a.cols) {
-                        float g[8];
-                        load8t<true>(a.post, RENG_TYPE_F32, 0, c, a.cols, g);
-#pragma unroll
-                        for (int i = 0; i < 8; i++) u[k][i] = u[k][i] * inv * g[i];
-                    }
-                }
+                for (int k = 0; k < C; k++) s = square_sum(u[k], s);
+                inv = inv_rms(cta_sum(s, red, turn), n, a.eps);
             }
 #pragma unroll
             for (int k = 0; k < C; k++) {
-                const int64_t c = ((int64_t)k * T + threadIdx.x) * 8;
-                if (c < a.cols) {
-                    residual8<true>(a, row, c, u[k], y[k]);
-                    store8t<true>(a.y, a.tr, row * a.ldy, c, a.cols, y[k]);
-                }
+                const Tile<VEC> t(k * nw + warp, a.cols);
+                tile_residual<TR, VEC>(a, row, t, inv, u[k], y[k]);
+                tile_store<TR, VEC>(a.y, row * a.ldy, t, a.cols, y[k]);
             }
         }
         if (a.out == OUT_NONE) continue;
         float s = 0.f;
 #pragma unroll
-        for (int k = 0; k < C; k++)
+        for (int k = 0; k < C; k++) s = square_sum(y[k], s);
+        const float inv = inv_rms(cta_sum(s, red, turn), n, a.eps);
 #pragma unroll
-            for (int i = 0; i < 8; i++) s = fmaf(y[k][i], y[k][i], s);
-        const float inv = inv_rms(cta_sum(s, red), n, a.eps);
-#pragma unroll
-        for (int k = 0; k < C; k++) {
-            const int64_t c = ((int64_t)k * T + threadIdx.x) * 8;
-            emit<true>(a, row, c, c < a.cols, inv, y[k]);
-        }
+        for (int k = 0; k < C; k++) tile_emit<VEC>(a, row, Tile<VEC>(k * nw + warp, a.cols), inv, y[k]);
     }
 }
 
-// Any width, pitch and alignment: the row in three passes over its columns
-// (each thread reads back only what it wrote itself).
-__global__ void __launch_bounds__(1024) k_block_norm_any(NormArgs a) {
-    __shared__ float red[32];
+// Rows too long for the registers: three passes over the columns, each warp
+// reading back only what it wrote itself.
+template <int TB, int TR, bool VEC>
+__global__ void __launch_bounds__(512) k_block_norm_long(NormArgs a) {
+    __shared__ float red[2][32];
+    int turn = 0;
+    const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
+    const float n = (float)a.cols;
+    const int64_t tiles = (a.cols + kTileGroups * kFp8Group - 1) / (kTileGroups * kFp8Group);
     pdl_wait();
     pdl_launch();
-    const float n = (float)a.cols;
-    const int64_t stride = (int64_t)blockDim.x * 8;
-    const int64_t end = (a.cols + 127) / 128 * 128;  // whole groups: a group's lanes stay together
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         float inv = 1.f;
         if (a.branch && a.post) {
             float s = 0.f;
-            for (int64_t c = threadIdx.x * 8; c < a.cols; c += stride) {
-                float u[8];
-                load8t<false>(a.branch, a.tb, row * a.ldb, c, a.cols, u);
-#pragma unroll
-                for (int i = 0; i < 8; i++) s = fmaf(u[i], u[i], s);
+            for (int64_t i = warp; i < tiles; i += nw) {
+                float u[16];
+                tile_floats<false, VEC>(a.branch, TB, row * a.ldb, Tile<VEC>(i, a.cols), a.cols, u);
+                s = square_sum(u, s);
             }
-            inv = inv_rms(cta_sum(s, red), n, a.eps);
+            inv = inv_rms(cta_sum(s, red, turn), n, a.eps);
         }
-        const void* src = a.branch ? a.y : a.residual;
-        const int64_t lds = a.branch ? a.ldy : a.ldr;
         float s = 0.f;
-        for (int64_t c = threadIdx.x * 8; c < a.cols; c += stride) {
-            float y[8];
-            load8t<false>(a.residual, a.tr, row * a.ldr, c, a.cols, y);
+        for (int64_t i = warp; i < tiles; i += nw) {
+            const Tile<VEC> t(i, a.cols);
+            float y[16];
+            tile_floats<false, VEC>(a.residual, TR, row * a.ldr, t, a.cols, y);
             if (a.branch) {
-                float u[8];
-                load8t<false>(a.branch, a.tb, row * a.ldb, c, a.cols, u);
-                if (a.post) {
-                    float g[8];
-                    load8t<false>(a.post, RENG_TYPE_F32, 0, c, a.cols, g);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) u[i] = u[i] * inv * g[i];
-                }
-                residual8<false>(a, row, c, u, y);
-                store8t<false>(a.y, a.tr, row * a.ldy, c, a.cols, y);
+                float u[16];
+                tile_floats<false, VEC>(a.branch, TB, row * a.ldb, t, a.cols, u);
+                tile_residual<TR, VEC>(a, row, t, inv, u, y);
+                tile_store<TR, VEC>(a.y, row * a.ldy, t, a.cols, y);
             }
-#pragma unroll
-            for (int i = 0; i < 8; i++) s = fmaf(y[i], y[i], s);
+            s = square_sum(y, s);
         }
         if (a.out == OUT_NONE) continue;
-        inv = inv_rms(cta_sum(s, red), n, a.eps);
-        for (int64_t c0 = 0; c0 < end; c0 += stride) {
-            const int64_t c = c0 + threadIdx.x * 8;
-            float y[8];
-            load8t<false>(src, a.tr, row * lds, c, a.cols, y);
-            emit<false>(a, row, c, c < a.cols, inv, y);
+        inv = inv_rms(cta_sum(s, red, turn), n, a.eps);
+        for (int64_t i = warp; i < tiles; i += nw) {
+            const Tile<VEC> t(i, a.cols);
+            float y[16];
+            if (a.branch) tile_floats<false, VEC>(a.y, TR, row * a.ldy, t, a.cols, y);
+            else tile_floats<false, VEC>(a.residual, TR, row * a.ldr, t, a.cols, y);
+            tile_emit<VEC>(a, row, t, inv, y);
         }
     }
+}
+
+template <int TB, int TR, bool VEC>
+cudaError_t launch_row(const NormArgs& a, int sms, cudaStream_t st) {
+    constexpr int kTile = kTileGroups * kFp8Group;
+    const int64_t tiles = (a.cols + kTile - 1) / kTile;
+    const dim3 grid((unsigned)std::min<int64_t>(a.rows, (int64_t)1 << 30));
+    if (tiles <= 16) return launch_ops(k_block_norm<TB, TR, VEC, 1>, grid, dim3(32 * (unsigned)tiles), 0, st, a);
+    if (tiles <= 32)
+        return launch_ops(k_block_norm<TB, TR, VEC, 2>, grid, dim3(32 * (unsigned)((tiles + 1) / 2)), 0, st, a);
+    return launch_ops(k_block_norm_long<TB, TR, VEC>, grid, dim3(512), 0, st, a);
 }
 
 int launch(const NormArgs& a, bool vec, cudaStream_t st) {
     int sms = 0;
     RENG_CUDA_TRY(current_sms(&sms));
-    const int64_t chunks = a.cols / 8;
-    const unsigned grid = (unsigned)std::min<int64_t>(a.rows, (int64_t)1 << 20);
-    auto threads = [](int64_t n) { return (unsigned)((n + 31) / 32 * 32); };
-    cudaError_t e;
-    if (!vec || chunks > 4096) {
-        const unsigned t = std::min<unsigned>(1024u, threads((a.cols + 7) / 8));
-        e = launch_ops(k_block_norm_any, dim3(grid), dim3(t), 0, st, a);
-    } else if (chunks <= 1024) {
-        e = launch_ops(k_block_norm<1>, dim3(grid), dim3(threads(chunks)), 0, st, a);
-    } else if (chunks <= 2048) {
-        e = launch_ops(k_block_norm<2>, dim3(grid), dim3(threads((chunks + 1) / 2)), 0, st, a);
-    } else {
-        e = launch_ops(k_block_norm<4>, dim3(grid), dim3(threads((chunks + 3) / 4)), 0, st, a);
-    }
+    constexpr int B = RENG_TYPE_BF16, F = RENG_TYPE_F32;
+    auto pick = [&](auto v) {
+        constexpr bool V = decltype(v)::value;
+        if (a.tr == B) return a.tb == B ? launch_row<B, B, V>(a, sms, st) : launch_row<F, B, V>(a, sms, st);
+        return a.tb == B ? launch_row<B, F, V>(a, sms, st) : launch_row<F, F, V>(a, sms, st);
+    };
+    const cudaError_t e = vec ? pick(std::true_type()) : pick(std::false_type());
     if (e != cudaSuccess) return fail(RENG_E_CUDA, std::string("reng_block_norm: ") + cudaGetErrorString(e));
     return RENG_OK;
 }
@@ -342,7 +369,7 @@ extern "C" int reng_block_norm(const reng_block_norm_desc *d, void *stream) {
     a.ldy = d->ld_y;
     a.ldh = d->ld_h;
     a.lds = d->ld_scales;
-    a.tb = d->branch_type;
+    a.tb = d->branch ? d->branch_type : d->residual_type;
     a.tr = d->residual_type;
     a.tg = d->gate_type;
     a.out = d->out;
@@ -358,8 +385,8 @@ extern "C" int reng_block_norm(const reng_block_norm_desc *d, void *stream) {
                        aligned(a.post, 0, 4, 4) && aligned(a.pre, 0, 4, 4) &&
                        (!fp8 || aligned(a.scales, a.lds, 4, 4)),
                    f + "a buffer is not aligned to its element");
-    const bool vec = a.cols % 8 == 0 && aligned(a.branch, a.ldb, eb, 16) && aligned(a.residual, a.ldr, er, 16) &&
+    const bool vec = a.cols % 16 == 0 && aligned(a.branch, a.ldb, eb, 16) && aligned(a.residual, a.ldr, er, 16) &&
                      aligned(a.gate, a.ldg, eg, 16) && aligned(y, a.ldy, er, 16) &&
-                     aligned(h, a.ldh, eh, fp8 ? 8 : 16) && aligned(a.post, 0, 4, 16) && aligned(a.pre, 0, 4, 16);
+                     aligned(h, a.ldh, eh, 16) && aligned(a.post, 0, 4, 16) && aligned(a.pre, 0, 4, 16);
     return launch(a, vec, (cudaStream_t)stream);
 }

@@ -50,12 +50,6 @@ __device__ __forceinline__ float fp8_max_finite() {
     return FMT == RENG_FP8_E4M3 ? 240.0f : 57344.0f;
 }
 
-// The running absmax of |x|: '>' against it, so a NaN is never taken.
-__device__ __forceinline__ float fp8_absmax(float m, float x) {
-    const float a = fabsf(x);
-    return a > m ? a : m;
-}
-
 // absmax / max_finite, 1 for a block of zeros.  No lower than the smallest
 // normal f32: a quotient that underflowed to 0 would make the block's zeros
 // 0 / 0, and a subnormal one has too few bits to divide by.
@@ -64,71 +58,167 @@ __device__ __forceinline__ float fp8_block_scale(float absmax) {
     return absmax > 0.0f ? fmaxf(__fdiv_rn(absmax, fp8_max_finite<FMT>()), 1.17549435e-38f) : 1.0f;
 }
 
-// encode(v[i] / s) of 8 values whose magnitudes are at most absmax, the
-// quotients by fp8_product.h's correction where it admits the scale and by
-// the division elsewhere.  fp_quotient keeps a NaN's sign; an infinity makes
-// s infinite, so its block takes the division.
-template <int FMT>
-__device__ __forceinline__ uint2 fp8_encode8(const float (&v)[8], float s, float absmax) {
-    uint32_t c[4];
-    const float r = __frcp_rn(s);
-    if (fp8_product_ok(s, r, absmax)) {
-#pragma unroll
-        for (int i = 0; i < 4; i++) c[i] = encode2<FMT>(fp_quotient(v[2 * i], s, r), fp_quotient(v[2 * i + 1], s, r));
-    } else {
-#pragma unroll
-        for (int i = 0; i < 4; i++) c[i] = encode2<FMT>(div_host(v[2 * i], s), div_host(v[2 * i + 1], s));
-    }
-    return make_uint2(c[0] | (c[1] << 16), c[2] | (c[3] << 16));
-}
+// ------------------------------------------------------------ warp tiles --
+// The block operators work on a warp tile: 4 groups of 128 values, 16 values
+// per lane.  Two ways to lay a tile over the lanes:
+//   VEC      lane l holds columns 16 (l % 8) .. + 15 of group l / 8: wide
+//            loads and stores; needs rows on 16 bytes and whole 16-column
+//            chunks;
+//   not VEC  value e of lane l is column 32 (e % 4) + l of group e / 4: one
+//            element per access, consecutive lanes on consecutive elements,
+//            for any pitch, alignment and width.
+// A group's (row pointer, first column) is the caller's; columns at or past
+// `cols` read as 0, which no absmax or sum notices, and are not written.
+constexpr int kTileGroups = 4;
 
-// Maximum over the 16 lanes of a half-warp (one 128-value group).
-__device__ __forceinline__ float half_warp_max(float v) {
-#pragma unroll
-    for (int o = 8; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
-    return v;
-}
-
-// -------------------------------------------------- 8 consecutive values --
-// Loads and stores of 8 consecutive elements at column c of a row of `cols`.
-// VEC: rows and base are 16-byte aligned (8 for codes) and the 8 elements
-// take one or two wide accesses where they all exist; the row's last partial
-// chunk, and every chunk without VEC, goes element by element.  Columns past
-// the end read as 0, which no absmax or sum notices, and are not written.
+// The raw elements of a lane's 16 values.
 template <int TYPE, bool VEC>
-__device__ __forceinline__ void load8(const void* row, int64_t c, int64_t cols, float (&v)[8]) {
-    if (VEC && c + 8 <= cols) {
-        if (TYPE == RENG_TYPE_BF16) {
-            const uint4 u = ldg_stream(static_cast<const uint16_t*>(row) + c);
-            v[0] = bf16lo(u.x), v[1] = bf16hi(u.x), v[2] = bf16lo(u.y), v[3] = bf16hi(u.y);
-            v[4] = bf16lo(u.z), v[5] = bf16hi(u.z), v[6] = bf16lo(u.w), v[7] = bf16hi(u.w);
-        } else {
-            const uint4 a = ldg_stream(static_cast<const float*>(row) + c);
-            const uint4 b = ldg_stream(static_cast<const float*>(row) + c + 4);
-            v[0] = __uint_as_float(a.x), v[1] = __uint_as_float(a.y), v[2] = __uint_as_float(a.z);
-            v[3] = __uint_as_float(a.w), v[4] = __uint_as_float(b.x), v[5] = __uint_as_float(b.y);
-            v[6] = __uint_as_float(b.z), v[7] = __uint_as_float(b.w);
-        }
-        return;
-    }
+struct Raw16 {
+    static constexpr int N = TYPE == RENG_TYPE_BF16 && VEC ? 8 : 16;
+    uint32_t w[N];
+};
+
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void raw_zero(Raw16<TYPE, VEC>& r) {
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        v[i] = 0.f;
-        if (c + i < cols)
-            v[i] = TYPE == RENG_TYPE_BF16 ? bf16_bits_to_f32(static_cast<const uint16_t*>(row)[c + i])
-                                          : static_cast<const float*>(row)[c + i];
+    for (int i = 0; i < Raw16<TYPE, VEC>::N; i++) r.w[i] = 0u;
+}
+
+// Loads go past L1 (each element is read once) unless KEEP, for the vectors
+// that every row reads again.
+template <bool KEEP, typename T>
+__device__ __forceinline__ T ld_elem(const T* p) {
+    return KEEP ? *p : __ldcg(p);
+}
+
+// VEC: 16 elements from p (16-byte aligned).
+template <int TYPE, bool KEEP = false>
+__device__ __forceinline__ void raw_load(const void* p, Raw16<TYPE, true>& r) {
+#pragma unroll
+    for (int i = 0; i < Raw16<TYPE, true>::N / 4; i++) {
+        const uint4 q = ld_elem<KEEP>(static_cast<const uint4*>(p) + i);
+        r.w[4 * i] = q.x, r.w[4 * i + 1] = q.y, r.w[4 * i + 2] = q.z, r.w[4 * i + 3] = q.w;
     }
 }
 
-template <bool VEC>
-__device__ __forceinline__ void store_codes8(uint8_t* row, int64_t c, int64_t cols, uint2 q) {
-    if (VEC && c + 8 <= cols) {
-        *reinterpret_cast<uint2*>(row + c) = q;
-        return;
-    }
+// not VEC: group g's 4 values of this lane, from column c0 of `row`.
+template <int TYPE, bool KEEP = false>
+__device__ __forceinline__ void raw_load(const void* row, int64_t c0, int64_t cols, int g, Raw16<TYPE, false>& r) {
+    const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < 8; i++)
-        if (c + i < cols) row[c + i] = (uint8_t)((i < 4 ? q.x : q.y) >> (8 * (i & 3)));
+    for (int i = 0; i < 4; i++) {
+        const int64_t c = c0 + 32 * i + lane;
+        if (c < cols)
+            r.w[4 * g + i] = TYPE == RENG_TYPE_BF16 ? (uint32_t)ld_elem<KEEP>(static_cast<const uint16_t*>(row) + c)
+                                                    : ld_elem<KEEP>(static_cast<const uint32_t*>(row) + c);
+    }
+}
+
+template <int TYPE, bool VEC>
+__device__ __forceinline__ void raw_floats(const Raw16<TYPE, VEC>& r, float (&v)[16]) {
+#pragma unroll
+    for (int i = 0; i < 16; i++) {
+        if (TYPE == RENG_TYPE_F32) v[i] = __uint_as_float(r.w[i]);
+        else if (VEC) v[i] = (i & 1) ? bf16hi(r.w[i / 2]) : bf16lo(r.w[i / 2]);
+        else v[i] = bf16lo(r.w[i]);
+    }
+}
+
+// Two floats rounded to bf16 (nearest even), the first in the low half.
+__device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
+
+// Maximum over a group's lanes of each group's value: VEC has one value per
+// lane (8 lanes a group), else 4 values per lane (all lanes).
+template <bool VEC>
+__device__ __forceinline__ void group_max(uint32_t (&m)[VEC ? 1 : kTileGroups]) {
+#pragma unroll
+    for (int o = VEC ? 4 : 16; o > 0; o >>= 1)
+#pragma unroll
+        for (int g = 0; g < (VEC ? 1 : kTileGroups); g++) m[g] = max(m[g], __shfl_xor_sync(0xffffffffu, m[g], o));
+}
+
+// The absmax bits of a tile's groups.  Bits of magnitudes order as their
+// values do, with NaN above infinity, so one integer maximum also tells
+// whether a value is not finite; `odd` says so for the whole warp, and then
+// the maximum is taken again without the NaNs.
+template <bool VEC>
+__device__ __forceinline__ void tile_absmax(const float (&v)[16], uint32_t (&m)[VEC ? 1 : kTileGroups], bool& odd) {
+#pragma unroll
+    for (int g = 0; g < (VEC ? 1 : kTileGroups); g++) {
+        m[g] = 0u;
+#pragma unroll
+        for (int i = 0; i < (VEC ? 16 : 4); i++) m[g] = max(m[g], abs_bits(v[4 * g + i]));
+    }
+    uint32_t top = m[0];
+#pragma unroll
+    for (int g = 1; g < (VEC ? 1 : kTileGroups); g++) top = max(top, m[g]);
+    odd = __any_sync(0xffffffffu, top >= 0x7f800000u);
+    if (odd) {
+#pragma unroll
+        for (int g = 0; g < (VEC ? 1 : kTileGroups); g++) {
+            m[g] = 0u;
+#pragma unroll
+            for (int i = 0; i < (VEC ? 16 : 4); i++) {
+                const uint32_t a = abs_bits(v[4 * g + i]);
+                if (a <= 0x7f800000u) m[g] = max(m[g], a);
+            }
+        }
+    }
+}
+
+// Codes of two finite values whose scale holds their block's absmax: the
+// quotients are at most max_finite and a rounding, which the converter
+// brings back to max_finite, so nothing is clamped and no NaN is looked for.
+// r = RN(1 / s); s of at least 2^-60 takes fp8_product.h's correction (the
+// correctly rounded quotient), a smaller one the division.
+template <int FMT>
+__device__ __forceinline__ uint32_t fp8_codes2(float a, float b, float s, float r) {
+    const bool product = s >= 8.6736174e-19f;
+    const float qa = product ? fp_quotient(a, s, r) : __fdiv_rn(a, s);
+    const float qb = product ? fp_quotient(b, s, r) : __fdiv_rn(b, s);
+    return FMT == RENG_FP8_E4M3 ? cvt_e4m3x2(qa, qb) : cvt_e5m2x2(qa, qb);
+}
+
+// The codes of a lane's 16 values, 4 to a word in order, given the scale of
+// each of its groups.
+template <int FMT, bool VEC>
+__device__ __forceinline__ uint4 tile_codes(const float (&v)[16], const float (&s)[VEC ? 1 : kTileGroups], bool odd) {
+    uint32_t w[4];
+    if (odd) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float sc = s[VEC ? 0 : i];
+            w[i] = encode2<FMT>(div_host(v[4 * i], sc), div_host(v[4 * i + 1], sc)) |
+                   encode2<FMT>(div_host(v[4 * i + 2], sc), div_host(v[4 * i + 3], sc)) << 16;
+        }
+    } else {
+        float r[VEC ? 1 : kTileGroups];
+#pragma unroll
+        for (int g = 0; g < (VEC ? 1 : kTileGroups); g++) r[g] = __frcp_rn(s[g]);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float sc = s[VEC ? 0 : i], rc = r[VEC ? 0 : i];
+            w[i] = fp8_codes2<FMT>(v[4 * i], v[4 * i + 1], sc, rc) |
+                   fp8_codes2<FMT>(v[4 * i + 2], v[4 * i + 3], sc, rc) << 16;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// not VEC: group g's 4 codes of this lane.
+__device__ __forceinline__ void store_codes(uint8_t* row, int64_t c0, int64_t cols, uint32_t codes) {
+    const int lane = threadIdx.x & 31;
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const int64_t c = c0 + 32 * i + lane;
+        if (c < cols) row[c] = (uint8_t)(codes >> (8 * i));
+    }
 }
 
 }  // namespace reng

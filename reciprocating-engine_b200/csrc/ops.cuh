@@ -19,6 +19,21 @@ inline bool ops_aligned(const void* p, int64_t pitch_bytes, int n) {
     return (uintptr_t)p % (uintptr_t)n == 0 && pitch_bytes % n == 0;
 }
 
+// t / d for t below 2^31 by a multiplication (Granlund and Montgomery,
+// "Division by invariant integers using multiplication", 1994): with
+// l = ceil(log2 d) and mul = floor(2^32 (2^l - d) / d) + 1, the quotient is
+// (umulhi(t, mul) + t) >> l.
+struct FastDiv {
+    uint32_t d, mul, shift;
+    explicit FastDiv(uint32_t div = 1) : d(div), shift(0) {
+        while (((uint64_t)1 << shift) < d) shift++;
+        mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1);
+    }
+#ifdef __CUDACC__
+    __device__ __forceinline__ uint32_t div(uint32_t t) const { return (__umulhi(t, mul) + t) >> shift; }
+#endif
+};
+
 // SMs of the current device.
 inline cudaError_t current_sms(int* sms) {
     int dev = 0;

@@ -280,45 +280,20 @@ def quantize_blocks(x, block_rows=1, fmt=Fp8Format.E4M3, codes=None, scales=None
     [ceil(rows / block_rows), ceil(cols / 128)]), the operands of
     gemm.gemm_fp8_blocks.  A block's scale is absmax / max_finite (1 for
     zeros) and its codes encode(x / scale) by the rules of quantize_with."""
-    import torch
-    from ._tensors import TYPES, call, codes_empty, groups, matrix
-    dev = x.device
-    ldx = matrix(x, "x", TYPES, dev)
-    rows, cols = x.shape
-    if block_rows not in (1, 128):
-        raise ValueError("block_rows must be 1 or 128")
-    shape = (-(-rows // block_rows), groups(cols))
-    if codes is None:
-        codes = codes_empty(rows, cols, dev)
-    if scales is None:
-        scales = torch.empty(shape, dtype=torch.float32, device=dev)
-    call(dev, stream, "reng_fp8_quantize_blocks", x.data_ptr(), TYPES[x.dtype], rows, cols, ldx, block_rows, fmt,
-         codes.data_ptr(), matrix(codes, "codes", (torch.uint8,), dev, (rows, cols)),
-         scales.data_ptr(), matrix(scales, "scales", (torch.float32,), dev, shape))
-    return codes, scales
+    from ._tensors import on_stream, quantize_blocks as run
+    if stream is not None:
+        return on_stream(stream, x, run, x, block_rows, fmt, codes, scales)
+    return run(x, block_rows, fmt, codes, scales)
 
 
 def swiglu_quantize(gate_up, fmt=Fp8Format.E4M3, codes=None, scales=None, stream=None):
     """quantize_blocks of h = silu(gate) * up in 1 x 128 groups, h in f32:
     gate_up [rows, 2 * cols] (bf16 or f32) holds the gate columns, then the
     up columns.  Returns (codes uint8 [rows, cols], scales)."""
-    import torch
-    from ._tensors import TYPES, call, codes_empty, groups, matrix
-    dev = gate_up.device
-    ldx = matrix(gate_up, "gate_up", TYPES, dev)
-    rows, both = gate_up.shape
-    if both % 2:
-        raise ValueError("gate_up has %d columns: not a gate and an up half" % both)
-    cols = both // 2
-    if codes is None:
-        codes = codes_empty(rows, cols, dev)
-    if scales is None:
-        scales = torch.empty((rows, groups(cols)), dtype=torch.float32, device=dev)
-    p = gate_up.data_ptr()
-    call(dev, stream, "reng_fp8_swiglu_quantize", p, p + cols * gate_up.element_size(), TYPES[gate_up.dtype], rows,
-         cols, ldx, fmt, codes.data_ptr(), matrix(codes, "codes", (torch.uint8,), dev, (rows, cols)),
-         scales.data_ptr(), matrix(scales, "scales", (torch.float32,), dev, (rows, groups(cols))))
-    return codes, scales
+    from ._tensors import on_stream, swiglu_quantize as run
+    if stream is not None:
+        return on_stream(stream, gate_up, run, gate_up, fmt, codes, scales)
+    return run(gate_up, fmt, codes, scales)
 
 
 # Rows per matrix the model-level pass measures its error on (FP8_ERROR_ROWS,

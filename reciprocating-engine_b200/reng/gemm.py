@@ -42,22 +42,7 @@ def gemm_fp8_blocks(x, x_scales, w, w_scales, out=None, dtype=None, x_fmt=_lib.R
     with scales [ceil(N / 128), ceil(K / 128)]; rows start on 16 bytes
     (fp8.quantize_blocks lays them out so).  y [M, N] is `out`, or a new
     tensor of `dtype` (bf16 by default, or f32)."""
-    import torch
-    from ._tensors import TYPES, call, groups, matrix
-    dev = x.device
-    u8, f32 = (torch.uint8,), (torch.float32,)
-    ldx = matrix(x, "x", u8, dev)
-    M, K = x.shape
-    N = w.shape[0] if w.dim() == 2 else 0
-    ldw = matrix(w, "w", u8, dev, (N, K))
-    kb = groups(K)
-    ldsx = matrix(x_scales, "x_scales", f32, dev, (M, kb))
-    ldsw = matrix(w_scales, "w_scales", f32, dev, (groups(N), kb))
-    if out is None:
-        out = torch.empty((M, N), dtype=dtype or torch.bfloat16, device=dev)
-    elif dtype is not None and out.dtype != dtype:
-        raise ValueError("out is %s, not %s" % (out.dtype, dtype))
-    ldy = matrix(out, "out", TYPES, dev, (M, N))
-    call(dev, stream, "reng_gemm_fp8_blocks", x.data_ptr(), ldx, x_scales.data_ptr(), ldsx, x_fmt, w.data_ptr(), ldw,
-         w_scales.data_ptr(), ldsw, w_fmt, M, N, K, out.data_ptr(), TYPES[out.dtype], ldy)
-    return out
+    from ._tensors import gemm_fp8_blocks as run, on_stream
+    if stream is not None:
+        return on_stream(stream, x, run, x, x_scales, w, w_scales, out, dtype, x_fmt, w_fmt)
+    return run(x, x_scales, w, w_scales, out, dtype, x_fmt, w_fmt)

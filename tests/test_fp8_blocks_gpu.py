@@ -203,6 +203,9 @@ def test_product_of_no_rows():
 
 
 # ----------------------------------------------------------------- SwiGLU --
+SWIGLU_REL = 12 * U32
+
+
 def check_groups(codes, scales, h, fmt, rel):
     """codes, scales of values known to `rel` relative: the scale to rel and a
     rounding, every code within half a step of its value over the scale given."""
@@ -224,11 +227,11 @@ def test_swiglu_quantize(rows, cols, dtype, fmt):
     both[0, 0] = -100.0  # exp(100) overflows f32: the product is zero there
     codes, scales = fp8.swiglu_quantize(both, fmt)
     g, u = both[:, :cols].double(), both[:, cols:].double()
-    # exp to 2 steps, the sum, the quotient and the product one rounding each, and the
-    # argument's own exponential error is none: at most 8 roundings in all
+    # 2^hi to 2^-22 (4 roundings), its correction, the sum and the two products one each,
+    # the reciprocal to 2^-23 (2): at most SWIGLU_REL of 12 roundings
     h = g / (1 + torch.exp(-g)) * u
     h = torch.where(h.abs() < 1e-35, torch.zeros_like(h), h)
-    check_groups(codes, scales, h, fmt, 8 * U32)
+    check_groups(codes, scales, h, fmt, SWIGLU_REL)
 
 
 # ------------------------------------------------------------------- norm --
@@ -366,7 +369,7 @@ def test_a_run_of_them_together(m):
     check_groups(xc, xs, want_h(y, g, 1e-5), 0, NORM_REL)
     check_product(gu, xc, xs, *wgu)
     gate, up = gu[:, :1536].double(), gu[:, 1536:].double()
-    check_groups(hc, hs, gate / (1 + torch.exp(-gate)) * up, 0, 8 * U32)
+    check_groups(hc, hs, gate / (1 + torch.exp(-gate)) * up, 0, SWIGLU_REL)
     check_product(out, hc, hs, *wd)
 
 
