@@ -29,294 +29,356 @@ struct NormArgs {
     void *y, *h;
     float* scales;
     const float *post, *pre;
-    int64_t rows, cols, ldb, ldr, ldg, ldy, ldh, lds;
-    int tb, tr, tg;  // element types (RENG_TYPE_*); y has tr
+    int64_t rows, ldb, ldr, ldg, ldy, ldh, lds;
+    int cols;
+    int tg;  // the gate's element type (RENG_TYPE_*)
     int out;
-    float scale, eps;
+    float scale, eps, inv_n;
 };
 
-// Sum over the CTA, the same bits on every thread (warps added in order).
-// `red` alternates between two buffers, so one barrier is enough: a buffer is
-// written again only after the barrier of the other's sum.
-__device__ __forceinline__ float cta_sum(float v, float (&red)[2][32], int& turn) {
-    v = warp_sum(v);
-    const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    float* r = red[turn];
-    turn ^= 1;
-    if ((threadIdx.x & 31) == 0) r[warp] = v;
-    __syncthreads();
-    float s = 0.f;
-    for (int w = 0; w < nw; w++) s += r[w];
-    return s;
+template <int TYPE>
+constexpr int kBytes = TYPE == RENG_TYPE_BF16 ? 2 : 4;
+
+template <int TYPE, typename P>
+__device__ __forceinline__ P* row_at(P* base, int64_t elems) {
+    return reinterpret_cast<P*>((uintptr_t)base + elems * kBytes<TYPE>);
 }
 
-__device__ __forceinline__ float inv_rms(float sum, float n, float eps) { return 1.0f / sqrtf(sum / n + eps); }
+// The warps that share a row: a CTA holds blockDim / (32 nw) such teams, each
+// on a row of its own.
+struct Team {
+    int nw, warp, id;  // warps of a team, this warp in it, the team in its CTA
+    int turn;
+    __device__ __forceinline__ explicit Team(int warps) : nw(warps), turn(0) {
+        const int w = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0);
+        id = w / nw;
+        warp = w - id * nw;
+    }
+    // Sum over the team, the same bits on every thread (warps added in order).
+    // `red` alternates between two rows, so one barrier is enough: a row is
+    // written again only after the barrier of the other's sum.
+    __device__ __forceinline__ float sum(float v, float (&red)[2][16]) {
+        v = warp_sum(v);
+        if (nw == 1) return v;
+        float* r = red[turn] + id * nw;
+        turn ^= 1;
+        if ((threadIdx.x & 31) == 0) r[warp] = v;
+        asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(32 * nw) : "memory");
+        float s = 0.f;
+        for (int w = 0; w < nw; w++) s += r[w];
+        return s;
+    }
+};
+
+// 1 / sqrt(sum / n + eps): the hardware's root is within 2 steps.
+__device__ __forceinline__ float inv_rms(float sum, const NormArgs& a) { return rsqrtf(fmaf(sum, a.inv_n, a.eps)); }
 
 // The 4 groups of a warp tile of one row: the first column of the lane's
-// values in each (VEC: in its own).
-template <bool VEC>
+// values in each of its groups.
+template <int G>
 struct Tile {
-    static constexpr int G = VEC ? 1 : kTileGroups;
-    int64_t c[G];
+    int c[G];
     bool live[G];
-    __device__ __forceinline__ Tile(int64_t tile, int64_t cols) {
-        const int lane = threadIdx.x & 31;
+    __device__ __forceinline__ Tile(int tile, int cols) {
 #pragma unroll
         for (int g = 0; g < G; g++) {
-            c[g] = tile * (kTileGroups * kFp8Group) + (VEC ? lane * 16 : g * kFp8Group);
+            c[g] = (tile * kTileGroups + lane_group<G>(g)) * kFp8Group + lane_col<G>();
             live[g] = c[g] < cols;
         }
     }
 };
 
-template <bool KEEP, int TYPE, bool VEC>
-__device__ __forceinline__ void tile_load(const void* base, int64_t at, const Tile<VEC>& t, int64_t cols,
-                                          Raw16<TYPE, VEC>& r) {
-    const char* row = static_cast<const char*>(base) + at * (TYPE == RENG_TYPE_BF16 ? 2 : 4);
+template <bool KEEP, int TYPE, int G>
+__device__ __forceinline__ void tile_load(const void* row, const Tile<G>& t, int cols, Raw16<TYPE, G>& r) {
     raw_zero(r);
-    if constexpr (VEC) {
-        if (t.live[0]) raw_load<TYPE, KEEP>(row + t.c[0] * (TYPE == RENG_TYPE_BF16 ? 2 : 4), r);
-    } else {
 #pragma unroll
-        for (int g = 0; g < kTileGroups; g++)
-            if (t.live[g]) raw_load<TYPE, KEEP>(row, t.c[g], cols, g, r);
+    for (int g = 0; g < G; g++) {
+        if (!t.live[g]) continue;
+        if constexpr (G < 4) raw_load<TYPE, KEEP>(static_cast<const char*>(row) + (uint32_t)(t.c[g] * kBytes<TYPE>), g, r);
+        else raw_load<TYPE, KEEP>(row, t.c[g], cols, g, r);
     }
 }
 
-// The same as floats, of a type known at run time (uniform).
-template <bool KEEP, bool VEC>
-__device__ __forceinline__ void tile_floats(const void* base, int type, int64_t at, const Tile<VEC>& t, int64_t cols,
-                                            float (&v)[16]) {
-    if (type == RENG_TYPE_BF16) {
-        Raw16<RENG_TYPE_BF16, VEC> r;
-        tile_load<KEEP>(base, at, t, cols, r);
-        raw_floats(r, v);
-    } else {
-        Raw16<RENG_TYPE_F32, VEC> r;
-        tile_load<KEEP>(base, at, t, cols, r);
-        raw_floats(r, v);
-    }
+// v *= the row's elements at the tile.
+template <int TYPE, int G>
+__device__ __forceinline__ void tile_mul(const void* row, const Tile<G>& t, int cols, f2 (&v)[8]) {
+    Raw16<TYPE, G> r;
+    f2 w[8];
+    tile_load<true>(row, t, cols, r);
+    raw_floats(r, w);
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = mul_f2(v[i], w[i]);
 }
 
-template <int TYPE, bool VEC>
-__device__ __forceinline__ void tile_store(void* base, int64_t at, const Tile<VEC>& t, int64_t cols,
-                                           const float (&v)[16]) {
-    if constexpr (VEC) {
-        if (!t.live[0]) return;
-        if (TYPE == RENG_TYPE_BF16) {
-            uint4* p = reinterpret_cast<uint4*>(static_cast<uint16_t*>(base) + at + t.c[0]);
+// y's raw form from its values, rounded to TYPE.
+template <int TYPE, int G>
+__device__ __forceinline__ void raw_round(const f2 (&v)[8], Raw16<TYPE, G>& r) {
 #pragma unroll
-            for (int i = 0; i < 2; i++)
-                p[i] = make_uint4(bf16x2(v[8 * i], v[8 * i + 1]), bf16x2(v[8 * i + 2], v[8 * i + 3]),
-                                  bf16x2(v[8 * i + 4], v[8 * i + 5]), bf16x2(v[8 * i + 6], v[8 * i + 7]));
+    for (int i = 0; i < 8; i++) {
+        float lo, hi;
+        split_f2(v[i], lo, hi);
+        if (TYPE == RENG_TYPE_F32) {
+            r.w[2 * i] = __float_as_uint(lo), r.w[2 * i + 1] = __float_as_uint(hi);
         } else {
-            float4* p = reinterpret_cast<float4*>(static_cast<float*>(base) + at + t.c[0]);
+            const uint32_t p = bf16x2(lo, hi);
+            if (G < 4) r.w[i] = p;
+            else r.w[2 * i] = p & 0xffffu, r.w[2 * i + 1] = p >> 16;
+        }
+    }
+}
+
+template <int TYPE, int G>
+__device__ __forceinline__ void tile_store(void* row, const Tile<G>& t, int cols, const Raw16<TYPE, G>& r) {
+    if constexpr (G < 4) {
+        constexpr int n = Raw16<TYPE, G>::N / (4 * G);
 #pragma unroll
-            for (int i = 0; i < 4; i++) p[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+        for (int g = 0; g < G; g++) {
+            if (!t.live[g]) continue;
+            uint4* p = reinterpret_cast<uint4*>(static_cast<char*>(row) + (uint32_t)(t.c[g] * kBytes<TYPE>));
+#pragma unroll
+            for (int i = 0; i < n; i++) {
+                const int k = 4 * (n * g + i);
+                p[i] = make_uint4(r.w[k], r.w[k + 1], r.w[k + 2], r.w[k + 3]);
+            }
         }
     } else {
         const int lane = threadIdx.x & 31;
 #pragma unroll
         for (int e = 0; e < 16; e++) {
-            const int64_t c = t.c[e >> 2] + 32 * (e & 3) + lane;
+            const int c = t.c[e >> 2] + 32 * (e & 3) + lane;
             if (c < cols) {
-                if (TYPE == RENG_TYPE_BF16)
-                    static_cast<uint16_t*>(base)[at + c] = __bfloat16_as_ushort(__float2bfloat16_rn(v[e]));
-                else static_cast<float*>(base)[at + c] = v[e];
+                if (TYPE == RENG_TYPE_BF16) static_cast<uint16_t*>(row)[c] = (uint16_t)r.w[e];
+                else static_cast<uint32_t*>(row)[c] = r.w[e];
             }
         }
     }
 }
 
-// u of a tile becomes the branch's share of y: normed, gained, gated; then
-// y += scale * u, rounded to y's type.
-template <int TR, bool VEC>
-__device__ __forceinline__ void tile_residual(const NormArgs& a, int64_t row, const Tile<VEC>& t, float inv,
-                                              float (&u)[16], float (&y)[16]) {
-    float g[16];
+// y of a tile, rounded, from the branch u and the residual y: norm, gain and
+// gate of the branch, then y + scale u.
+template <int TB, int TR, int G>
+__device__ __forceinline__ void tile_residual(const NormArgs& a, int64_t row, const Tile<G>& t, float inv,
+                                              const Raw16<TB, G>& u, Raw16<TR, G>& y) {
+    f2 v[8], w[8];
+    raw_floats(u, v);
     if (a.post) {
-        tile_floats<true, VEC>(a.post, RENG_TYPE_F32, 0, t, a.cols, g);
+        const f2 n = make_f2(inv);
 #pragma unroll
-        for (int i = 0; i < 16; i++) u[i] = u[i] * inv * g[i];
+        for (int i = 0; i < 8; i++) v[i] = mul_f2(v[i], n);
+        tile_mul<RENG_TYPE_F32>(a.post, t, a.cols, v);
     }
     if (a.gate) {
-        tile_floats<true, VEC>(a.gate, a.tg, row * a.ldg, t, a.cols, g);
-#pragma unroll
-        for (int i = 0; i < 16; i++) u[i] *= g[i];
+        if (a.tg == RENG_TYPE_BF16) tile_mul<RENG_TYPE_BF16>(row_at<RENG_TYPE_BF16>(a.gate, row * a.ldg), t, a.cols, v);
+        else tile_mul<RENG_TYPE_F32>(row_at<RENG_TYPE_F32>(a.gate, row * a.ldg), t, a.cols, v);
     }
+    raw_floats(y, w);
+    const f2 s = make_f2(a.scale);
 #pragma unroll
-    for (int i = 0; i < 16; i++) y[i] = fmaf(a.scale, u[i], y[i]);
-    if (TR == RENG_TYPE_BF16) {
-#pragma unroll
-        for (int i = 0; i < 16; i += 2) {
-            const uint32_t p = bf16x2(y[i], y[i + 1]);
-            y[i] = bf16lo(p), y[i + 1] = bf16hi(p);
-        }
-    }
+    for (int i = 0; i < 8; i++) w[i] = fma_f2(s, v[i], w[i]);
+    raw_round(w, y);
 }
 
-template <int FMT, bool VEC>
-__device__ __forceinline__ void tile_emit_fp8(const NormArgs& a, int64_t row, const Tile<VEC>& t,
-                                              const float (&h)[16]) {
-    constexpr int G = Tile<VEC>::G;
-    const int lane = threadIdx.x & 31;
-    uint32_t m[G];
+template <int FMT, int G>
+__device__ __forceinline__ void tile_emit_fp8(const NormArgs& a, int64_t row, const Tile<G>& t, const f2 (&h)[8]) {
+    float m[G], s[G], r[G];
     bool odd;
-    tile_absmax<VEC>(h, m, odd);
-    group_max<VEC>(m);
-    float s[G];
-#pragma unroll
-    for (int g = 0; g < G; g++) s[g] = fp8_block_scale<FMT>(__uint_as_float(m[g]));
-    const uint4 q = tile_codes<FMT, VEC>(h, s, odd);
+    tile_absmax(h, m, odd);
+    group_max(m);
+    tile_scales<FMT>(m, s, r);
+    uint32_t w[4];
+    tile_codes<FMT>(h, s, r, odd, w);
     uint8_t* dst = static_cast<uint8_t*>(a.h) + row * a.ldh;
+    float* scales = a.scales + row * a.lds;
 #pragma unroll
     for (int g = 0; g < G; g++) {
         if (!t.live[g]) continue;
-        if ((lane & (VEC ? 7 : 31)) == 0) a.scales[row * a.lds + t.c[g] / kFp8Group] = s[g];
-        if constexpr (VEC) *reinterpret_cast<uint4*>(dst + t.c[g]) = q;
-        else store_codes(dst, t.c[g], a.cols, g == 0 ? q.x : g == 1 ? q.y : g == 2 ? q.z : q.w);
+        if (lane_first<G>()) scales[t.c[g] / kFp8Group] = s[g];
+        tile_store_codes<G>(dst, t.c[g], a.cols, g, w);
     }
 }
 
 // h of a tile (whole warps: the FP8 groups shuffle).
-template <bool VEC>
-__device__ __forceinline__ void tile_emit(const NormArgs& a, int64_t row, const Tile<VEC>& t, float inv,
-                                          const float (&y)[16]) {
-    float h[16];
-    if (a.pre) {
-        tile_floats<true, VEC>(a.pre, RENG_TYPE_F32, 0, t, a.cols, h);
+template <int TR, int G>
+__device__ __forceinline__ void tile_emit(const NormArgs& a, int64_t row, const Tile<G>& t, float inv,
+                                          const Raw16<TR, G>& y) {
+    f2 h[8];
+    raw_floats(y, h);
+    const f2 n = make_f2(inv);
 #pragma unroll
-        for (int i = 0; i < 16; i++) h[i] = y[i] * inv * h[i];
+    for (int i = 0; i < 8; i++) h[i] = mul_f2(h[i], n);
+    if (a.pre) tile_mul<RENG_TYPE_F32>(a.pre, t, a.cols, h);
+    if (a.out == OUT_E4M3) {
+        tile_emit_fp8<RENG_FP8_E4M3, G>(a, row, t, h);
+    } else if (a.out == OUT_E5M2) {
+        tile_emit_fp8<RENG_FP8_E5M2, G>(a, row, t, h);
+    } else if (a.out == OUT_BF16) {
+        Raw16<RENG_TYPE_BF16, G> r;
+        raw_round(h, r);
+        tile_store(row_at<RENG_TYPE_BF16>(a.h, row * a.ldh), t, a.cols, r);
     } else {
-#pragma unroll
-        for (int i = 0; i < 16; i++) h[i] = y[i] * inv;
+        Raw16<RENG_TYPE_F32, G> r;
+        raw_round(h, r);
+        tile_store(row_at<RENG_TYPE_F32>(a.h, row * a.ldh), t, a.cols, r);
     }
-    if (a.out == OUT_BF16) tile_store<RENG_TYPE_BF16, VEC>(a.h, row * a.ldh, t, a.cols, h);
-    else if (a.out == OUT_F32) tile_store<RENG_TYPE_F32, VEC>(a.h, row * a.ldh, t, a.cols, h);
-    else if (a.out == OUT_E4M3) tile_emit_fp8<RENG_FP8_E4M3, VEC>(a, row, t, h);
-    else tile_emit_fp8<RENG_FP8_E5M2, VEC>(a, row, t, h);
 }
 
-__device__ __forceinline__ float square_sum(const float (&v)[16], float s) {
+template <int TYPE, int G>
+__device__ __forceinline__ f2 square_sum(const Raw16<TYPE, G>& r, f2 s) {
+    f2 v[8];
+    raw_floats(r, v);
 #pragma unroll
-    for (int i = 0; i < 16; i++) s = fmaf(v[i], v[i], s);
+    for (int i = 0; i < 8; i++) s = fma_f2(v[i], v[i], s);
     return s;
 }
+__device__ __forceinline__ float f2_sum(f2 s) {
+    float lo, hi;
+    split_f2(s, lo, hi);
+    return lo + hi;
+}
+// Raw words stay raw between the passes over them: as floats they would take
+// twice the registers, which here are loads in flight.
+template <int TYPE, int G>
+__device__ __forceinline__ void keep_raw(Raw16<TYPE, G>& r) {
+#pragma unroll
+    for (int i = 0; i < Raw16<TYPE, G>::N; i++) asm volatile("" : "+r"(r.w[i]));
+}
 
-// One CTA per row, the row in registers: C warp tiles per warp.
-template <int TB, int TR, bool VEC, int C>
-__global__ void __launch_bounds__(512) k_block_norm(NormArgs a) {
-    __shared__ float red[2][32];
-    int turn = 0;
-    const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    const float n = (float)a.cols;
+// A team per row, the row in registers: C warp tiles per warp.  The next
+// row's residual and branch are loaded before this row's two sums are formed,
+// so the memory is busy while the team waits for itself.
+template <int TB, int TR, int G, int C>
+__global__ void __launch_bounds__(C == 1 ? 256 : 512, C == 1 ? 3 : 1) k_block_norm(const NormArgs a, int nw) {
+    __shared__ float red[2][16];
+    Team team(nw);
+    const int teams = blockDim.x / (32 * nw);
+    const int64_t step = (int64_t)gridDim.x * teams;
+    int64_t row = (int64_t)blockIdx.x * teams + team.id;
     pdl_wait();
     pdl_launch();
-    for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
-        float y[C][16], u[C][16];
+    Raw16<TR, G> r[C];
+    Raw16<TB, G> b[C];
+    auto load = [&](int64_t at) {
 #pragma unroll
         for (int k = 0; k < C; k++) {
-            const Tile<VEC> t(k * nw + warp, a.cols);
-            Raw16<TR, VEC> r;
-            Raw16<TB, VEC> b;
-            tile_load<false>(a.residual, row * a.ldr, t, a.cols, r);
-            if (a.branch) tile_load<false>(a.branch, row * a.ldb, t, a.cols, b);
-            raw_floats(r, y[k]);
-            if (a.branch) raw_floats(b, u[k]);
+            const Tile<G> t(k * nw + team.warp, a.cols);
+            tile_load<false>(row_at<TR>(a.residual, at * a.ldr), t, a.cols, r[k]);
+            if (a.branch) tile_load<false>(row_at<TB>(a.branch, at * a.ldb), t, a.cols, b[k]);
         }
+    };
+    if (row < a.rows) load(row);
+    for (; row < a.rows; row += step) {
+        Raw16<TR, G> y[C];
+        Raw16<TB, G> u[C];
+#pragma unroll
+        for (int k = 0; k < C; k++) {
+            y[k] = r[k];
+            if (a.branch) u[k] = b[k];
+        }
+        if (row + step < a.rows) load(row + step);
         if (a.branch) {
             float inv = 1.f;
             if (a.post) {
-                float s = 0.f;
+                f2 s = 0ull;
 #pragma unroll
-                for (int k = 0; k < C; k++) s = square_sum(u[k], s);
-                inv = inv_rms(cta_sum(s, red, turn), n, a.eps);
+                for (int k = 0; k < C; k++) {
+                    s = square_sum(u[k], s);
+                    keep_raw(u[k]);
+                }
+                inv = inv_rms(team.sum(f2_sum(s), red), a);
             }
 #pragma unroll
             for (int k = 0; k < C; k++) {
-                const Tile<VEC> t(k * nw + warp, a.cols);
-                tile_residual<TR, VEC>(a, row, t, inv, u[k], y[k]);
-                tile_store<TR, VEC>(a.y, row * a.ldy, t, a.cols, y[k]);
+                const Tile<G> t(k * nw + team.warp, a.cols);
+                tile_residual(a, row, t, inv, u[k], y[k]);
+                tile_store(row_at<TR>(a.y, row * a.ldy), t, a.cols, y[k]);
             }
         }
         if (a.out == OUT_NONE) continue;
-        float s = 0.f;
+        f2 s = 0ull;
 #pragma unroll
-        for (int k = 0; k < C; k++) s = square_sum(y[k], s);
-        const float inv = inv_rms(cta_sum(s, red, turn), n, a.eps);
+        for (int k = 0; k < C; k++) {
+            s = square_sum(y[k], s);
+            keep_raw(y[k]);
+        }
+        const float inv = inv_rms(team.sum(f2_sum(s), red), a);
 #pragma unroll
-        for (int k = 0; k < C; k++) tile_emit<VEC>(a, row, Tile<VEC>(k * nw + warp, a.cols), inv, y[k]);
+        for (int k = 0; k < C; k++) tile_emit(a, row, Tile<G>(k * nw + team.warp, a.cols), inv, y[k]);
     }
 }
 
 // Rows too long for the registers: three passes over the columns, each warp
 // reading back only what it wrote itself.
-template <int TB, int TR, bool VEC>
-__global__ void __launch_bounds__(512) k_block_norm_long(NormArgs a) {
-    __shared__ float red[2][32];
-    int turn = 0;
-    const int warp = threadIdx.x >> 5, nw = blockDim.x >> 5;
-    const float n = (float)a.cols;
-    const int64_t tiles = (a.cols + kTileGroups * kFp8Group - 1) / (kTileGroups * kFp8Group);
+template <int TB, int TR, int G>
+__global__ void __launch_bounds__(512) k_block_norm_long(const NormArgs a) {
+    __shared__ float red[2][16];
+    Team team(16);
+    const int tiles = (a.cols + kTileGroups * kFp8Group - 1) / (kTileGroups * kFp8Group);
     pdl_wait();
     pdl_launch();
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
+        const void *branch = row_at<TB>(a.branch, row * a.ldb), *residual = row_at<TR>(a.residual, row * a.ldr);
+        void* out = row_at<TR>(a.y, row * a.ldy);
         float inv = 1.f;
         if (a.branch && a.post) {
-            float s = 0.f;
-            for (int64_t i = warp; i < tiles; i += nw) {
-                float u[16];
-                tile_floats<false, VEC>(a.branch, TB, row * a.ldb, Tile<VEC>(i, a.cols), a.cols, u);
+            f2 s = 0ull;
+            for (int i = team.warp; i < tiles; i += team.nw) {
+                Raw16<TB, G> u;
+                tile_load<false>(branch, Tile<G>(i, a.cols), a.cols, u);
                 s = square_sum(u, s);
             }
-            inv = inv_rms(cta_sum(s, red, turn), n, a.eps);
+            inv = inv_rms(team.sum(f2_sum(s), red), a);
         }
-        float s = 0.f;
-        for (int64_t i = warp; i < tiles; i += nw) {
-            const Tile<VEC> t(i, a.cols);
-            float y[16];
-            tile_floats<false, VEC>(a.residual, TR, row * a.ldr, t, a.cols, y);
+        f2 s = 0ull;
+        for (int i = team.warp; i < tiles; i += team.nw) {
+            const Tile<G> t(i, a.cols);
+            Raw16<TR, G> y;
+            tile_load<false>(residual, t, a.cols, y);
             if (a.branch) {
-                float u[16];
-                tile_floats<false, VEC>(a.branch, TB, row * a.ldb, t, a.cols, u);
-                tile_residual<TR, VEC>(a, row, t, inv, u, y);
-                tile_store<TR, VEC>(a.y, row * a.ldy, t, a.cols, y);
+                Raw16<TB, G> u;
+                tile_load<false>(branch, t, a.cols, u);
+                tile_residual(a, row, t, inv, u, y);
+                tile_store(out, t, a.cols, y);
             }
             s = square_sum(y, s);
         }
         if (a.out == OUT_NONE) continue;
-        inv = inv_rms(cta_sum(s, red, turn), n, a.eps);
-        for (int64_t i = warp; i < tiles; i += nw) {
-            const Tile<VEC> t(i, a.cols);
-            float y[16];
-            if (a.branch) tile_floats<false, VEC>(a.y, TR, row * a.ldy, t, a.cols, y);
-            else tile_floats<false, VEC>(a.residual, TR, row * a.ldr, t, a.cols, y);
-            tile_emit<VEC>(a, row, t, inv, y);
+        inv = inv_rms(team.sum(f2_sum(s), red), a);
+        for (int i = team.warp; i < tiles; i += team.nw) {
+            const Tile<G> t(i, a.cols);
+            Raw16<TR, G> y;
+            tile_load<false>(a.branch ? out : residual, t, a.cols, y);
+            tile_emit(a, row, t, inv, y);
         }
     }
 }
 
-template <int TB, int TR, bool VEC>
+template <int TB, int TR, int G>
 cudaError_t launch_row(const NormArgs& a, int sms, cudaStream_t st) {
     constexpr int kTile = kTileGroups * kFp8Group;
-    const int64_t tiles = (a.cols + kTile - 1) / kTile;
-    const dim3 grid((unsigned)std::min<int64_t>(a.rows, (int64_t)1 << 30));
-    if (tiles <= 16) return launch_ops(k_block_norm<TB, TR, VEC, 1>, grid, dim3(32 * (unsigned)tiles), 0, st, a);
-    if (tiles <= 32)
-        return launch_ops(k_block_norm<TB, TR, VEC, 2>, grid, dim3(32 * (unsigned)((tiles + 1) / 2)), 0, st, a);
-    return launch_ops(k_block_norm_long<TB, TR, VEC>, grid, dim3(512), 0, st, a);
+    const int tiles = (a.cols + kTile - 1) / kTile;
+    if (tiles > 32)
+        return launch_ops(k_block_norm_long<TB, TR, G>, dim3((unsigned)std::min<int64_t>(a.rows, (int64_t)sms * 4)),
+                          dim3(512), 0, st, a);
+    const int c = tiles > 8 ? 2 : 1, nw = (tiles + c - 1) / c, teams = std::max(1, 8 / nw);
+    // as many CTAs as fit the SMs (the kernels' launch bounds), every team on
+    // its next row's loads while it works on one
+    const int64_t want = (a.rows + teams - 1) / teams;
+    const int64_t fit = (int64_t)sms * (c == 1 ? 3 * std::max(1, 8 / (teams * nw)) : std::max(1, 16 / nw));
+    const dim3 grid((unsigned)std::min(want, fit)), block((unsigned)(32 * teams * nw));
+    return c == 1 ? launch_ops(k_block_norm<TB, TR, G, 1>, grid, block, 0, st, a, nw)
+                  : launch_ops(k_block_norm<TB, TR, G, 2>, grid, block, 0, st, a, nw);
 }
 
-int launch(const NormArgs& a, bool vec, cudaStream_t st) {
+int launch(const NormArgs& a, int tb, int tr, bool vec, cudaStream_t st) {
     int sms = 0;
     RENG_CUDA_TRY(current_sms(&sms));
     constexpr int B = RENG_TYPE_BF16, F = RENG_TYPE_F32;
     auto pick = [&](auto v) {
-        constexpr bool V = decltype(v)::value;
-        if (a.tr == B) return a.tb == B ? launch_row<B, B, V>(a, sms, st) : launch_row<F, B, V>(a, sms, st);
-        return a.tb == B ? launch_row<B, F, V>(a, sms, st) : launch_row<F, F, V>(a, sms, st);
+        constexpr int V = decltype(v)::value;
+        if (tr == B) return tb == B ? launch_row<B, B, V>(a, sms, st) : launch_row<F, B, V>(a, sms, st);
+        return tb == B ? launch_row<B, F, V>(a, sms, st) : launch_row<F, F, V>(a, sms, st);
     };
-    const cudaError_t e = vec ? pick(std::true_type()) : pick(std::false_type());
+    const cudaError_t e = vec ? pick(std::integral_constant<int, 2>()) : pick(std::integral_constant<int, 4>());
     if (e != cudaSuccess) return fail(RENG_E_CUDA, std::string("reng_block_norm: ") + cudaGetErrorString(e));
     return RENG_OK;
 }
@@ -332,7 +394,7 @@ using namespace reng;
 extern "C" int reng_block_norm(const reng_block_norm_desc *d, void *stream) {
     const std::string f = "reng_block_norm: ";
     RENG_CHECK_ARG(d != nullptr, f + "desc is NULL");
-    RENG_CHECK_ARG(d->rows >= 0 && d->cols >= 1, f + "rows >= 0 and cols >= 1, not " + std::to_string(d->rows) +
+    RENG_CHECK_ARG(d->rows >= 0 && d->cols >= 1 && d->cols <= kOpsMaxCols, f + "rows >= 0 and cols in [1, 2^30], not " + std::to_string(d->rows) +
                                                      " x " + std::to_string(d->cols));
     RENG_CHECK_ARG(type_ok(d->residual_type) && (!d->branch || type_ok(d->branch_type)) &&
                        (!d->gate || type_ok(d->gate_type)),
@@ -362,21 +424,21 @@ extern "C" int reng_block_norm(const reng_block_norm_desc *d, void *stream) {
     a.post = d->post_gain;
     a.pre = d->pre_gain;
     a.rows = d->rows;
-    a.cols = d->cols;
+    a.cols = (int)d->cols;
+    a.inv_n = 1.0f / (float)d->cols;
     a.ldb = d->ld_branch;
     a.ldr = d->ld_residual;
     a.ldg = d->ld_gate;
     a.ldy = d->ld_y;
     a.ldh = d->ld_h;
     a.lds = d->ld_scales;
-    a.tb = d->branch ? d->branch_type : d->residual_type;
-    a.tr = d->residual_type;
+    const int tb = d->branch ? d->branch_type : d->residual_type, tr = d->residual_type;
     a.tg = d->gate_type;
     a.out = d->out;
     a.scale = d->scale;
     a.eps = d->eps;
     auto aligned = [](const void* p, int64_t ld, int esz, int n) { return !p || ops_aligned(p, ld * esz, n); };
-    const int eb = host_esize(a.tb), er = host_esize(a.tr), eg = host_esize(a.tg);
+    const int eb = host_esize(tb), er = host_esize(tr), eg = host_esize(a.tg);
     const int eh = fp8 ? 1 : (a.out == OUT_BF16 ? 2 : 4);
     const void* y = d->branch ? d->y : nullptr;
     const void* h = a.out == OUT_NONE ? nullptr : d->h;
@@ -385,8 +447,8 @@ extern "C" int reng_block_norm(const reng_block_norm_desc *d, void *stream) {
                        aligned(a.post, 0, 4, 4) && aligned(a.pre, 0, 4, 4) &&
                        (!fp8 || aligned(a.scales, a.lds, 4, 4)),
                    f + "a buffer is not aligned to its element");
-    const bool vec = a.cols % 16 == 0 && aligned(a.branch, a.ldb, eb, 16) && aligned(a.residual, a.ldr, er, 16) &&
+    const bool vec = a.cols % 8 == 0 && aligned(a.branch, a.ldb, eb, 16) && aligned(a.residual, a.ldr, er, 16) &&
                      aligned(a.gate, a.ldg, eg, 16) && aligned(y, a.ldy, er, 16) &&
-                     aligned(h, a.ldh, eh, 16) && aligned(a.post, 0, 4, 16) && aligned(a.pre, 0, 4, 16);
-    return launch(a, vec, (cudaStream_t)stream);
+                     aligned(h, a.ldh, eh, fp8 ? 8 : 16) && aligned(a.post, 0, 4, 16) && aligned(a.pre, 0, 4, 16);
+    return launch(a, tb, tr, vec, (cudaStream_t)stream);
 }

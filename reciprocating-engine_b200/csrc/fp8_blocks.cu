@@ -20,7 +20,8 @@ namespace {
 struct GroupArgs {
     const void* x;   // values; the gate of the SwiGLU form
     const void* up;  // SwiGLU only
-    int64_t rows, cols, ldx;
+    int64_t rows, ldx;
+    int cols;
     uint8_t* codes;
     int64_t ldc;
     float* scales;
@@ -29,157 +30,186 @@ struct GroupArgs {
     FastDiv per_row;  // of one row (of blocks)
 };
 
-// g / (1 + exp(-g)) * u.  exp(-g) is 2^t by the hardware's ex2, t = -g log2(e)
+// silu(g) u = g / (1 + exp(-g)) u for g whose exponential is out of the sum's
+// reach: g u, or the zero of the limit (NaN for g = -inf, which has none).
+__device__ __forceinline__ float swiglu_far(float g, float u) { return (g > 0.f ? g : g * 0.f) * u; }
+
+// v[i] = silu(v[i]) u[i].  exp(-g) is 2^t by the hardware's ex2, t = -g log2(e)
 // in two parts so that the rounding of t (which |g| magnifies) does not reach
-// the result: 2^(hi + lo) = 2^hi (1 + lo ln 2).  It overflows to infinity for
-// g below about -88, where the quotient is the (negative) zero of the limit;
-// where 2^t is out of reach of the sum the correction is left out.
-// About 10 roundings in all (ex2 4, rcp 2, the rest one each).
-__device__ __forceinline__ float swiglu(float g, float u) {
-    const float hi = __fmul_rn(g, -1.44269504f);
-    const float lo = fmaf(g, -1.92596299e-8f, fmaf(g, -1.44269504f, -hi));
-    float e, r;
-    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(hi));
-    e = fabsf(hi) < 126.f ? fmaf(e, lo * 0.693147181f, e) : e;
-    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.0f + e));
-    return g * r * u;
+// the result: 2^(hi + lo) = 2^hi (1 + lo ln 2).  The quotient is rcp's,
+// corrected by its residual.  About 6 roundings in all.
+__device__ __forceinline__ void swiglu(f2 (&v)[8], const f2 (&u)[8]) {
+    constexpr float kFar = 87.0f;  // 2^t stays normal below
+    float top = 0.f;
+    f2 h[8];
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        const f2 g = v[i];
+        float g0, g1, e0, e1, d0, d1;
+        split_f2(g, g0, g1);
+        top = absmax_nan(absmax_nan(top, g0), g1);
+        const f2 hi = mul_f2(g, make_f2(-1.44269504f));
+        const f2 neg = mul_f2(hi, make_f2(-1.0f));
+        const f2 lo = fma_f2(g, make_f2(-1.33497580e-8f), mul_f2(fma_f2(g, make_f2(-1.44269504f), neg), make_f2(0.693147181f)));
+        split_f2(hi, e0, e1);
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(e0));
+        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(e1));
+        const f2 e = make_f2(e0, e1), d = add_f2(fma_f2(e, lo, e), make_f2(1.0f));
+        split_f2(d, d0, d1);
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d0) : "f"(d0));
+        asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d1) : "f"(d1));
+        const f2 r = make_f2(d0, d1), y = mul_f2(g, r), ny = mul_f2(y, make_f2(-1.0f));
+        h[i] = mul_f2(fma_f2(fma_f2(ny, d, g), r, y), u[i]);
+    }
+    if (!(top < kFar)) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            float g0, g1, u0, u1, h0, h1;
+            split_f2(v[i], g0, g1);
+            split_f2(u[i], u0, u1);
+            split_f2(h[i], h0, h1);
+            h[i] = make_f2(fabsf(g0) < kFar ? h0 : swiglu_far(g0, u0), fabsf(g1) < kFar ? h1 : swiglu_far(g1, u1));
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; i++) v[i] = h[i];
 }
 
-template <int TYPE, bool VEC>
+template <int TYPE>
 __device__ __forceinline__ const void* elem(const void* base, int64_t at) {
     return static_cast<const char*>(base) + at * (TYPE == RENG_TYPE_BF16 ? 2 : 4);
 }
 
 // 1 x 128 groups: one warp tile of 4 consecutive groups (of any rows) each,
 // codes and scales straight from registers.
-template <int TYPE, int FMT, bool VEC, bool SWIGLU>
+template <int TYPE, int FMT, int G, bool SWIGLU>
 __global__ void __launch_bounds__(256) k_fp8_groups(GroupArgs a) {
-    constexpr int G = VEC ? 1 : kTileGroups;
-    const int lane = threadIdx.x & 31;
-    const uint32_t t0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kTileGroups + (VEC ? lane >> 3 : 0);
+    const uint32_t t0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kTileGroups;
     pdl_wait();
     pdl_launch();
     uint32_t row[G], grp[G];
-    int64_t c[G];
+    int c[G];
     bool live[G];
-    Raw16<TYPE, VEC> x, u;
+    Raw16<TYPE, G> x, u;
     raw_zero(x);
     if (SWIGLU) raw_zero(u);
 #pragma unroll
     for (int g = 0; g < G; g++) {
-        row[g] = a.per_row.div(t0 + g);
-        grp[g] = t0 + g - row[g] * a.per_row.d;
-        c[g] = (int64_t)grp[g] * kFp8Group + (VEC ? (lane & 7) * 16 : 0);
-        live[g] = t0 + g < a.blocks && c[g] < a.cols;
+        const uint32_t t = t0 + lane_group<G>(g);
+        row[g] = a.per_row.div(t);
+        grp[g] = t - row[g] * a.per_row.d;
+        c[g] = (int)(grp[g] * kFp8Group) + lane_col<G>();
+        live[g] = t < a.blocks && c[g] < a.cols;
         if (live[g]) {
             const int64_t at = row[g] * a.ldx;
-            if constexpr (VEC) {
-                raw_load<TYPE>(elem<TYPE, VEC>(a.x, at + c[g]), x);
-                if (SWIGLU) raw_load<TYPE>(elem<TYPE, VEC>(a.up, at + c[g]), u);
+            if constexpr (G < 4) {
+                raw_load<TYPE>(elem<TYPE>(a.x, at + c[g]), g, x);
+                if (SWIGLU) raw_load<TYPE>(elem<TYPE>(a.up, at + c[g]), g, u);
             } else {
-                raw_load<TYPE>(elem<TYPE, VEC>(a.x, at), c[g], a.cols, g, x);
-                if (SWIGLU) raw_load<TYPE>(elem<TYPE, VEC>(a.up, at), c[g], a.cols, g, u);
+                raw_load<TYPE>(elem<TYPE>(a.x, at), c[g], a.cols, g, x);
+                if (SWIGLU) raw_load<TYPE>(elem<TYPE>(a.up, at), c[g], a.cols, g, u);
             }
         }
     }
-    float v[16];
+    f2 v[8];
     raw_floats(x, v);
     if (SWIGLU) {
-        float w[16];
+        f2 w[8];
         raw_floats(u, w);
-#pragma unroll
-        for (int i = 0; i < 16; i++) v[i] = swiglu(v[i], w[i]);
+        swiglu(v, w);
     }
-    uint32_t m[G];
+    float m[G], s[G], r[G];
     bool odd;
-    tile_absmax<VEC>(v, m, odd);
-    group_max<VEC>(m);
-    float s[G];
-#pragma unroll
-    for (int g = 0; g < G; g++) s[g] = fp8_block_scale<FMT>(__uint_as_float(m[g]));
-    const uint4 q = tile_codes<FMT, VEC>(v, s, odd);
+    tile_absmax(v, m, odd);
+    group_max(m);
+    tile_scales<FMT>(m, s, r);
+    uint32_t w[4];
+    tile_codes<FMT>(v, s, r, odd, w);
 #pragma unroll
     for (int g = 0; g < G; g++) {
         if (!live[g]) continue;
-        if ((lane & (VEC ? 7 : 31)) == 0) a.scales[row[g] * a.lds + grp[g]] = s[g];
-        uint8_t* dst = a.codes + row[g] * a.ldc;
-        if constexpr (VEC) *reinterpret_cast<uint4*>(dst + c[g]) = q;
-        else store_codes(dst, c[g], a.cols, g == 0 ? q.x : g == 1 ? q.y : g == 2 ? q.z : q.w);
+        if (lane_first<G>()) a.scales[row[g] * a.lds + grp[g]] = s[g];
+        tile_store_codes<G>(a.codes + row[g] * a.ldc, c[g], a.cols, g, w);
     }
 }
 
 // 128 x 128 blocks: one CTA per block, the block in registers between the
 // absmax and the codes: 4 tiles per warp, a tile 4 rows of the block.
-template <int TYPE, int FMT, bool VEC>
+template <int TYPE, int FMT, int G>
 __global__ void __launch_bounds__(256) k_fp8_blocks(GroupArgs a) {
-    constexpr int G = VEC ? 1 : kTileGroups;
-    __shared__ uint32_t red[8];
+    __shared__ float red[8];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const uint32_t rb = a.per_row.div(blockIdx.x), grp = blockIdx.x - rb * a.per_row.d;
-    const int64_t c = (int64_t)grp * kFp8Group + (VEC ? (lane & 7) * 16 : 0);
-    // the first row of tile i (VEC: this lane's row)
-    auto row_of = [&](int i) { return (int64_t)rb * kFp8Group + 32 * i + 4 * warp + (VEC ? lane >> 3 : 0); };
+    const int c = (int)(grp * kFp8Group) + lane_col<G>();
+    // the row of this lane's group g in tile i
+    auto row_of = [&](int i, int g) { return (int64_t)rb * kFp8Group + 32 * i + 4 * warp + lane_group<G>(g); };
     pdl_wait();
     pdl_launch();
-    Raw16<TYPE, VEC> x[4];
+    Raw16<TYPE, G> x[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
         raw_zero(x[i]);
 #pragma unroll
         for (int g = 0; g < G; g++) {
-            const int64_t row = row_of(i) + g;
+            const int64_t row = row_of(i, g);
             if (row < a.rows && c < a.cols) {
-                if constexpr (VEC) raw_load<TYPE>(elem<TYPE, VEC>(a.x, row * a.ldx + c), x[i]);
-                else raw_load<TYPE>(elem<TYPE, VEC>(a.x, row * a.ldx), c, a.cols, g, x[i]);
+                if constexpr (G < 4) raw_load<TYPE>(elem<TYPE>(a.x, row * a.ldx + c), g, x[i]);
+                else raw_load<TYPE>(elem<TYPE>(a.x, row * a.ldx), c, a.cols, g, x[i]);
             }
         }
     }
-    uint32_t top = 0u;
+    float top = 0.f;
     bool odd = false;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        float v[16];
-        uint32_t m[G];
+        f2 v[8];
+        float m[G];
         bool o;
         raw_floats(x[i], v);
-        tile_absmax<VEC>(v, m, o);
+        tile_absmax(v, m, o);
         odd = odd || o;
 #pragma unroll
-        for (int g = 0; g < G; g++) top = max(top, m[g]);
+        for (int g = 0; g < G; g++) top = fmaxf(top, m[g]);
     }
-    top = __reduce_max_sync(0xffffffffu, top);
+    top = warp_max(top);
     if (lane == 0) red[warp] = top;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < 8; w++) top = max(top, red[w]);
+    for (int w = 0; w < 8; w++) top = fmaxf(top, red[w]);
     // a warp whose values are finite still divides by an infinite scale
-    odd = odd || top >= 0x7f800000u;
-    float s[G];
+    odd = odd || top == __int_as_float(0x7f800000);
+    // the codes start from the raw values again: as floats they would take
+    // twice the registers meanwhile, and the SM hold one CTA less
 #pragma unroll
-    for (int g = 0; g < G; g++) s[g] = fp8_block_scale<FMT>(__uint_as_float(top));
+    for (int i = 0; i < 4; i++)
+#pragma unroll
+        for (int k = 0; k < Raw16<TYPE, G>::N; k++) asm volatile("" : "+r"(x[i].w[k]));
+    float s[G], r[G];
+    s[0] = fp8_block_scale<FMT>(top);
+    r[0] = __frcp_rn(s[0]);
+#pragma unroll
+    for (int g = 1; g < G; g++) s[g] = s[0], r[g] = r[0];
     if (threadIdx.x == 0) a.scales[rb * a.lds + grp] = s[0];
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        float v[16];
+        f2 v[8];
         raw_floats(x[i], v);
-        const uint4 q = tile_codes<FMT, VEC>(v, s, odd);
+        uint32_t w[4];
+        tile_codes<FMT>(v, s, r, odd, w);
 #pragma unroll
         for (int g = 0; g < G; g++) {
-            const int64_t row = row_of(i) + g;
-            if (row >= a.rows || c >= a.cols) continue;
-            uint8_t* dst = a.codes + row * a.ldc;
-            if constexpr (VEC) *reinterpret_cast<uint4*>(dst + c) = q;
-            else store_codes(dst, c, a.cols, g == 0 ? q.x : g == 1 ? q.y : g == 2 ? q.z : q.w);
+            const int64_t row = row_of(i, g);
+            if (row < a.rows && c < a.cols) tile_store_codes<G>(a.codes + row * a.ldc, c, a.cols, g, w);
         }
     }
 }
 
-template <int TYPE, int FMT, bool VEC>
+template <int TYPE, int FMT, int G>
 cudaError_t launch_blocks(const GroupArgs& a, int block_rows, bool swiglu, cudaStream_t st) {
-    if (block_rows > 1) return launch_ops(k_fp8_blocks<TYPE, FMT, VEC>, dim3(a.blocks), dim3(256), 0, st, a);
+    if (block_rows > 1) return launch_ops(k_fp8_blocks<TYPE, FMT, G>, dim3(a.blocks), dim3(256), 0, st, a);
     const dim3 grid((a.blocks + 31) / 32);  // 8 warps of 4 groups
-    return swiglu ? launch_ops(k_fp8_groups<TYPE, FMT, VEC, true>, grid, dim3(256), 0, st, a)
-                  : launch_ops(k_fp8_groups<TYPE, FMT, VEC, false>, grid, dim3(256), 0, st, a);
+    return swiglu ? launch_ops(k_fp8_groups<TYPE, FMT, G, true>, grid, dim3(256), 0, st, a)
+                  : launch_ops(k_fp8_groups<TYPE, FMT, G, false>, grid, dim3(256), 0, st, a);
 }
 
 template <int TYPE, int FMT>
@@ -187,8 +217,8 @@ cudaError_t pick_vec(const GroupArgs& a, int block_rows, bool swiglu, cudaStream
     const int esz = TYPE == RENG_TYPE_BF16 ? 2 : 4;
     const bool vec = a.cols % 16 == 0 && ops_aligned(a.x, a.ldx * esz, 16) &&
                      (!swiglu || ops_aligned(a.up, a.ldx * esz, 16)) && ops_aligned(a.codes, a.ldc, 16);
-    return vec ? launch_blocks<TYPE, FMT, true>(a, block_rows, swiglu, st)
-               : launch_blocks<TYPE, FMT, false>(a, block_rows, swiglu, st);
+    return vec ? launch_blocks<TYPE, FMT, 1>(a, block_rows, swiglu, st)
+               : launch_blocks<TYPE, FMT, 4>(a, block_rows, swiglu, st);
 }
 
 int quantize(const char* who, const GroupArgs& a, int type, int block_rows, int fmt, bool swiglu, cudaStream_t st) {
@@ -205,7 +235,7 @@ int quantize(const char* who, const GroupArgs& a, int type, int block_rows, int 
 
 int check_quantize(const std::string& f, const void* x, const void* up, int type, int64_t rows, int64_t cols,
                    int64_t ldx, int fmt, const void* codes, int64_t ldc, const void* scales, int64_t lds) {
-    RENG_CHECK_ARG(rows >= 0 && cols >= 1, f + "rows >= 0 and cols >= 1, not " + std::to_string(rows) + " x " +
+    RENG_CHECK_ARG(rows >= 0 && cols >= 1 && cols <= kOpsMaxCols, f + "rows >= 0 and cols in [1, 2^30], not " + std::to_string(rows) + " x " +
                                                std::to_string(cols));
     RENG_CHECK_ARG(type == RENG_TYPE_BF16 || type == RENG_TYPE_F32, f + "unknown element type");
     RENG_CHECK_ARG(fmt == RENG_FP8_E4M3 || fmt == RENG_FP8_E5M2, f + "unknown format");
@@ -234,7 +264,7 @@ extern "C" int reng_fp8_quantize_blocks(const void *x, int type, int64_t rows, i
     const int rc = check_quantize("reng_fp8_quantize_blocks: ", x, x, type, rows, cols, ldx, fmt, codes, ldc, scales, lds);
     if (rc || rows == 0) return rc;
     const int64_t groups = ops_groups(cols), per = (rows + block_rows - 1) / block_rows * groups;
-    GroupArgs a{x, nullptr, rows, cols, ldx, codes, ldc, scales, lds, (uint32_t)per, FastDiv((uint32_t)groups)};
+    GroupArgs a{x, nullptr, rows, ldx, (int)cols, codes, ldc, scales, lds, (uint32_t)per, FastDiv((uint32_t)groups)};
     return quantize("reng_fp8_quantize_blocks", a, type, block_rows, fmt, false, (cudaStream_t)stream);
 }
 
@@ -245,6 +275,6 @@ extern "C" int reng_fp8_swiglu_quantize(const void *gate, const void *up, int ty
         check_quantize("reng_fp8_swiglu_quantize: ", gate, up, type, rows, cols, ldx, fmt, codes, ldc, scales, lds);
     if (rc || rows == 0) return rc;
     const int64_t groups = ops_groups(cols);
-    GroupArgs a{gate, up, rows, cols, ldx, codes, ldc, scales, lds, (uint32_t)(rows * groups), FastDiv((uint32_t)groups)};
+    GroupArgs a{gate, up, rows, ldx, (int)cols, codes, ldc, scales, lds, (uint32_t)(rows * groups), FastDiv((uint32_t)groups)};
     return quantize("reng_fp8_swiglu_quantize", a, type, 1, fmt, true, (cudaStream_t)stream);
 }

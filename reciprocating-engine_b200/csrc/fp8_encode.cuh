@@ -45,43 +45,62 @@ __device__ __forceinline__ float div_host(float x, float s) {
 
 constexpr int kFp8Group = 128;  // columns (and, of a weight block, rows) that share one scale
 
-template <int FMT>
-__device__ __forceinline__ float fp8_max_finite() {
-    return FMT == RENG_FP8_E4M3 ? 240.0f : 57344.0f;
-}
-
-// absmax / max_finite, 1 for a block of zeros.  No lower than the smallest
-// normal f32: a quotient that underflowed to 0 would make the block's zeros
-// 0 / 0, and a subnormal one has too few bits to divide by.
+// absmax / max_finite, 1 for a block of zeros: the correctly rounded quotient
+// by fp8_product.h's correction (checked for both constants over every
+// mantissa), an infinite absmax as itself.  No lower than the smallest normal
+// f32: a quotient that underflowed to 0 would make the block's zeros 0 / 0,
+// and a subnormal one has too few bits to divide by.
 template <int FMT>
 __device__ __forceinline__ float fp8_block_scale(float absmax) {
-    return absmax > 0.0f ? fmaxf(__fdiv_rn(absmax, fp8_max_finite<FMT>()), 1.17549435e-38f) : 1.0f;
+    constexpr float d = FMT == RENG_FP8_E4M3 ? 240.0f : 57344.0f, r = 1.0f / d;
+    const float y = __fmul_rn(absmax, r), q = __fmaf_rn(__fmaf_rn(-y, d, absmax), r, y);
+    const float s = absmax < __int_as_float(0x7f800000) ? fmaxf(q, 1.17549435e-38f) : absmax;
+    return absmax > 0.0f ? s : 1.0f;
 }
 
 // ------------------------------------------------------------ warp tiles --
 // The block operators work on a warp tile: 4 groups of 128 values, 16 values
-// per lane.  Two ways to lay a tile over the lanes:
-//   VEC      lane l holds columns 16 (l % 8) .. + 15 of group l / 8: wide
-//            loads and stores; needs rows on 16 bytes and whole 16-column
-//            chunks;
-//   not VEC  value e of lane l is column 32 (e % 4) + l of group e / 4: one
-//            element per access, consecutive lanes on consecutive elements,
-//            for any pitch, alignment and width.
-// A group's (row pointer, first column) is the caller's; columns at or past
-// `cols` read as 0, which no absmax or sum notices, and are not written.
+// per lane, in G groups of the lane's own.  Three ways to lay it out:
+//   G 1  lane l holds columns 16 (l % 8) .. + 15 of group l / 8: the fewest
+//        scales and shuffles, 32 bytes of a bf16 row a lane (the quantizers);
+//   G 2  columns 8 (l % 16) .. + 7 of groups l / 16 and 2 + l / 16:
+//        consecutive lanes on consecutive 16 bytes of a bf16 row and 32 of an
+//        f32 one (the norm, whose gains are f32 and come from L1);
+//   G 4  columns l, 32 + l, 64 + l and 96 + l of every group: one element per
+//        access, consecutive lanes on consecutive elements, for any pitch,
+//        alignment and width.
+// Columns are below 2^31.  G 1 and 2 need rows on 16 bytes and whole 16- or 8-column chunks.  A group's
+// (row pointer, first column) is the caller's; columns at or past `cols` read
+// as 0, which no absmax or sum notices, and are not written.
 constexpr int kTileGroups = 4;
+// This lane's group of index g among the tile's 4, and its first column there.
+template <int G>
+__device__ __forceinline__ int lane_group(int g) {
+    const int lane = threadIdx.x & 31;
+    return G == 1 ? lane >> 3 : G == 2 ? 2 * g + (lane >> 4) : g;
+}
+template <int G>
+__device__ __forceinline__ int lane_col() {
+    const int lane = threadIdx.x & 31;
+    return G == 1 ? (lane & 7) * 16 : G == 2 ? (lane & 15) * 8 : 0;
+}
+// Whether this lane writes its groups' scales.
+template <int G>
+__device__ __forceinline__ bool lane_first() {
+    return (threadIdx.x & (8 * G - 1)) == 0;
+}
 
-// The raw elements of a lane's 16 values.
-template <int TYPE, bool VEC>
+// The raw elements of a lane's 16 values, group by group.
+template <int TYPE, int G>
 struct Raw16 {
-    static constexpr int N = TYPE == RENG_TYPE_BF16 && VEC ? 8 : 16;
+    static constexpr int N = TYPE == RENG_TYPE_BF16 && G < 4 ? 8 : 16;
     uint32_t w[N];
 };
 
-template <int TYPE, bool VEC>
-__device__ __forceinline__ void raw_zero(Raw16<TYPE, VEC>& r) {
+template <int TYPE, int G>
+__device__ __forceinline__ void raw_zero(Raw16<TYPE, G>& r) {
 #pragma unroll
-    for (int i = 0; i < Raw16<TYPE, VEC>::N; i++) r.w[i] = 0u;
+    for (int i = 0; i < Raw16<TYPE, G>::N; i++) r.w[i] = 0u;
 }
 
 // Loads go past L1 (each element is read once) unless KEEP, for the vectors
@@ -91,36 +110,67 @@ __device__ __forceinline__ T ld_elem(const T* p) {
     return KEEP ? *p : __ldcg(p);
 }
 
-// VEC: 16 elements from p (16-byte aligned).
-template <int TYPE, bool KEEP = false>
-__device__ __forceinline__ void raw_load(const void* p, Raw16<TYPE, true>& r) {
+// G 1, 2: group g's values of this lane, from p (16-byte aligned).
+template <int TYPE, bool KEEP = false, int G>
+__device__ __forceinline__ void raw_load(const void* p, int g, Raw16<TYPE, G>& r) {
+    constexpr int n = Raw16<TYPE, G>::N / (4 * G);  // 16-byte loads
 #pragma unroll
-    for (int i = 0; i < Raw16<TYPE, true>::N / 4; i++) {
+    for (int i = 0; i < n; i++) {
         const uint4 q = ld_elem<KEEP>(static_cast<const uint4*>(p) + i);
-        r.w[4 * i] = q.x, r.w[4 * i + 1] = q.y, r.w[4 * i + 2] = q.z, r.w[4 * i + 3] = q.w;
+        const int k = 4 * (n * g + i);
+        r.w[k] = q.x, r.w[k + 1] = q.y, r.w[k + 2] = q.z, r.w[k + 3] = q.w;
     }
 }
 
-// not VEC: group g's 4 values of this lane, from column c0 of `row`.
+// G 4: group g's 4 values of this lane, from column c0 of `row`.
 template <int TYPE, bool KEEP = false>
-__device__ __forceinline__ void raw_load(const void* row, int64_t c0, int64_t cols, int g, Raw16<TYPE, false>& r) {
+__device__ __forceinline__ void raw_load(const void* row, int c0, int cols, int g, Raw16<TYPE, 4>& r) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int i = 0; i < 4; i++) {
-        const int64_t c = c0 + 32 * i + lane;
+        const int c = c0 + 32 * i + lane;
         if (c < cols)
             r.w[4 * g + i] = TYPE == RENG_TYPE_BF16 ? (uint32_t)ld_elem<KEEP>(static_cast<const uint16_t*>(row) + c)
                                                     : ld_elem<KEEP>(static_cast<const uint32_t*>(row) + c);
     }
 }
 
-template <int TYPE, bool VEC>
-__device__ __forceinline__ void raw_floats(const Raw16<TYPE, VEC>& r, float (&v)[16]) {
+// A lane's values are handled two at a time: one instruction on a register
+// pair, which these kernels' arithmetic needs (they are bound by instruction
+// issue as soon as HBM streams).
+typedef unsigned long long f2;
+__device__ __forceinline__ f2 make_f2(float lo, float hi) {
+    f2 r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
+    return r;
+}
+__device__ __forceinline__ f2 make_f2(float v) { return make_f2(v, v); }
+__device__ __forceinline__ void split_f2(f2 v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ f2 mul_f2(f2 a, f2 b) {
+    f2 r;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 add_f2(f2 a, f2 b) {
+    f2 r;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+    return r;
+}
+__device__ __forceinline__ f2 fma_f2(f2 a, f2 b, f2 c) {
+    f2 r;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+    return r;
+}
+
+template <int TYPE, int G>
+__device__ __forceinline__ void raw_floats(const Raw16<TYPE, G>& r, f2 (&v)[8]) {
 #pragma unroll
-    for (int i = 0; i < 16; i++) {
-        if (TYPE == RENG_TYPE_F32) v[i] = __uint_as_float(r.w[i]);
-        else if (VEC) v[i] = (i & 1) ? bf16hi(r.w[i / 2]) : bf16lo(r.w[i / 2]);
-        else v[i] = bf16lo(r.w[i]);
+    for (int i = 0; i < 8; i++) {
+        if (TYPE == RENG_TYPE_F32) v[i] = make_f2(__uint_as_float(r.w[2 * i]), __uint_as_float(r.w[2 * i + 1]));
+        else if (G < 4) v[i] = make_f2(bf16lo(r.w[i]), bf16hi(r.w[i]));
+        else v[i] = make_f2(bf16lo(r.w[2 * i]), bf16lo(r.w[2 * i + 1]));
     }
 }
 
@@ -131,93 +181,131 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
     return r;
 }
 
-__device__ __forceinline__ uint32_t abs_bits(float x) { return __float_as_uint(x) & 0x7fffffffu; }
-
-// Maximum over a group's lanes of each group's value: VEC has one value per
-// lane (8 lanes a group), else 4 values per lane (all lanes).
-template <bool VEC>
-__device__ __forceinline__ void group_max(uint32_t (&m)[VEC ? 1 : kTileGroups]) {
-#pragma unroll
-    for (int o = VEC ? 4 : 16; o > 0; o >>= 1)
-#pragma unroll
-        for (int g = 0; g < (VEC ? 1 : kTileGroups); g++) m[g] = max(m[g], __shfl_xor_sync(0xffffffffu, m[g], o));
+// max(m, |x|), NaN if x is.
+__device__ __forceinline__ float absmax_nan(float m, float x) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+    return r;
 }
 
-// The absmax bits of a tile's groups.  Bits of magnitudes order as their
-// values do, with NaN above infinity, so one integer maximum also tells
-// whether a value is not finite; `odd` says so for the whole warp, and then
-// the maximum is taken again without the NaNs.
-template <bool VEC>
-__device__ __forceinline__ void tile_absmax(const float (&v)[16], uint32_t (&m)[VEC ? 1 : kTileGroups], bool& odd) {
+// Maximum over a group's lanes (8 G of them) of each group's value.
+template <int G>
+__device__ __forceinline__ void group_max(float (&m)[G]) {
 #pragma unroll
-    for (int g = 0; g < (VEC ? 1 : kTileGroups); g++) {
-        m[g] = 0u;
+    for (int o = 4 * G; o > 0; o >>= 1)
 #pragma unroll
-        for (int i = 0; i < (VEC ? 16 : 4); i++) m[g] = max(m[g], abs_bits(v[4 * g + i]));
+        for (int g = 0; g < G; g++) m[g] = fmaxf(m[g], __shfl_xor_sync(0xffffffffu, m[g], o));
+}
+
+// The scales of a lane's groups and their reciprocals, rounded to nearest.
+// The lanes of a group share the work: each forms one of their G (a division
+// and a reciprocal take some 30 instructions).
+template <int FMT, int G>
+__device__ __forceinline__ void tile_scales(const float (&m)[G], float (&s)[G], float (&r)[G]) {
+    const int lane = threadIdx.x & 31, mine = lane & (G - 1);
+    float own = m[0];
+#pragma unroll
+    for (int g = 1; g < G; g++) own = mine == g ? m[g] : own;
+    const float sc = fp8_block_scale<FMT>(own), rc = __frcp_rn(sc);
+#pragma unroll
+    for (int g = 0; g < G; g++) {
+        s[g] = G == 1 ? sc : __shfl_sync(0xffffffffu, sc, (lane & ~(G - 1)) + g);
+        r[g] = G == 1 ? rc : __shfl_sync(0xffffffffu, rc, (lane & ~(G - 1)) + g);
     }
-    uint32_t top = m[0];
+}
+
+// The absmax of a lane's values in each of its groups, without the NaNs, and
+// whether any value of the warp is not finite (`odd`): a maximum that keeps
+// NaN shows it, and only then the values are looked at again.
+template <int G>
+__device__ __forceinline__ void tile_absmax(const f2 (&v)[8], float (&m)[G], bool& odd) {
+    constexpr int P = 8 / G;
+    float top = 0.f;
 #pragma unroll
-    for (int g = 1; g < (VEC ? 1 : kTileGroups); g++) top = max(top, m[g]);
-    odd = __any_sync(0xffffffffu, top >= 0x7f800000u);
+    for (int g = 0; g < G; g++) {
+        m[g] = 0.f;
+#pragma unroll
+        for (int i = 0; i < P; i++) {
+            float a, b;
+            split_f2(v[P * g + i], a, b);
+            m[g] = absmax_nan(absmax_nan(m[g], a), b);
+        }
+        top = absmax_nan(top, m[g]);
+    }
+    odd = __any_sync(0xffffffffu, !(top < __int_as_float(0x7f800000)));
     if (odd) {
 #pragma unroll
-        for (int g = 0; g < (VEC ? 1 : kTileGroups); g++) {
-            m[g] = 0u;
+        for (int g = 0; g < G; g++) {
+            m[g] = 0.f;
 #pragma unroll
-            for (int i = 0; i < (VEC ? 16 : 4); i++) {
-                const uint32_t a = abs_bits(v[4 * g + i]);
-                if (a <= 0x7f800000u) m[g] = max(m[g], a);
+            for (int i = 0; i < P; i++) {
+                float a, b;
+                split_f2(v[P * g + i], a, b);
+                m[g] = fmaxf(fmaxf(m[g], fabsf(a)), fabsf(b));  // fmaxf passes a NaN over
             }
         }
     }
 }
 
-// Codes of two finite values whose scale holds their block's absmax: the
-// quotients are at most max_finite and a rounding, which the converter
-// brings back to max_finite, so nothing is clamped and no NaN is looked for.
-// r = RN(1 / s); s of at least 2^-60 takes fp8_product.h's correction (the
-// correctly rounded quotient), a smaller one the division.
-template <int FMT>
-__device__ __forceinline__ uint32_t fp8_codes2(float a, float b, float s, float r) {
-    const bool product = s >= 8.6736174e-19f;
-    const float qa = product ? fp_quotient(a, s, r) : __fdiv_rn(a, s);
-    const float qb = product ? fp_quotient(b, s, r) : __fdiv_rn(b, s);
-    return FMT == RENG_FP8_E4M3 ? cvt_e4m3x2(qa, qb) : cvt_e5m2x2(qa, qb);
-}
-
-// The codes of a lane's 16 values, 4 to a word in order, given the scale of
-// each of its groups.
-template <int FMT, bool VEC>
-__device__ __forceinline__ uint4 tile_codes(const float (&v)[16], const float (&s)[VEC ? 1 : kTileGroups], bool odd) {
-    uint32_t w[4];
-    if (odd) {
+// The codes of a lane's 16 values, 4 to a word in order, given the scale s of
+// each of its groups and r = RN(1 / s).  Finite tiles: the quotients are at most max_finite and
+// a rounding, which the converter brings back to max_finite, so nothing is
+// clamped and no NaN is looked for; scales of at least 2^-60 take
+// fp8_product.h's correction of x * RN(1 / s) (the correctly rounded
+// quotient, with the sign of x put on a zero), smaller ones the division.
+template <int FMT, int G>
+__device__ __forceinline__ void tile_codes(const f2 (&v)[8], const float (&s)[G], const float (&rs)[G], bool odd,
+                                           uint32_t (&w)[4]) {
+    bool product = !odd;
+#pragma unroll
+    for (int g = 0; g < G; g++) product = product && s[g] >= 8.6736174e-19f;
+    if (product) {
+        f2 r[G], n[G];
+#pragma unroll
+        for (int g = 0; g < G; g++) r[g] = make_f2(rs[g]), n[g] = make_f2(-s[g]);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float sc = s[VEC ? 0 : i];
-            w[i] = encode2<FMT>(div_host(v[4 * i], sc), div_host(v[4 * i + 1], sc)) |
-                   encode2<FMT>(div_host(v[4 * i + 2], sc), div_host(v[4 * i + 3], sc)) << 16;
+            const int g = i * G / 4;
+            uint32_t c[2];
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                const f2 x = v[2 * i + h], y = mul_f2(x, r[g]);
+                const f2 q = fma_f2(fma_f2(y, n[g], x), r[g], y);
+                float q0, q1, x0, x1;
+                split_f2(q, q0, q1);
+                split_f2(x, x0, x1);
+                q0 = __uint_as_float(__float_as_uint(q0) | (__float_as_uint(x0) & 0x80000000u));
+                q1 = __uint_as_float(__float_as_uint(q1) | (__float_as_uint(x1) & 0x80000000u));
+                c[h] = FMT == RENG_FP8_E4M3 ? cvt_e4m3x2(q0, q1) : cvt_e5m2x2(q0, q1);
+            }
+            w[i] = __byte_perm(c[0], c[1], 0x5410);
         }
     } else {
-        float r[VEC ? 1 : kTileGroups];
-#pragma unroll
-        for (int g = 0; g < (VEC ? 1 : kTileGroups); g++) r[g] = __frcp_rn(s[g]);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
-            const float sc = s[VEC ? 0 : i], rc = r[VEC ? 0 : i];
-            w[i] = fp8_codes2<FMT>(v[4 * i], v[4 * i + 1], sc, rc) |
-                   fp8_codes2<FMT>(v[4 * i + 2], v[4 * i + 3], sc, rc) << 16;
+            const float sc = s[i * G / 4];
+            float a, b, c, d;
+            split_f2(v[2 * i], a, b);
+            split_f2(v[2 * i + 1], c, d);
+            w[i] = encode2<FMT>(div_host(a, sc), div_host(b, sc)) | encode2<FMT>(div_host(c, sc), div_host(d, sc)) << 16;
         }
     }
-    return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-// not VEC: group g's 4 codes of this lane.
-__device__ __forceinline__ void store_codes(uint8_t* row, int64_t c0, int64_t cols, uint32_t codes) {
-    const int lane = threadIdx.x & 31;
+// A lane's codes of group g into the row at column c (G 1, 2: of this lane).
+template <int G>
+__device__ __forceinline__ void tile_store_codes(uint8_t* row, int c, int cols, int g, const uint32_t (&w)[4]) {
+    if (G == 1) {
+        *reinterpret_cast<uint4*>(row + c) = make_uint4(w[0], w[1], w[2], w[3]);
+    } else if (G == 2) {
+        *reinterpret_cast<uint2*>(row + c) = make_uint2(w[(2 * g) & 3], w[(2 * g + 1) & 3]);
+    } else {
+        const int lane = threadIdx.x & 31;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int64_t c = c0 + 32 * i + lane;
-        if (c < cols) row[c] = (uint8_t)(codes >> (8 * i));
+        for (int i = 0; i < 4; i++) {
+            const int at = c + 32 * i + lane;
+            if (at < cols) row[at] = (uint8_t)(w[g] >> (8 * i));
+        }
     }
 }
 

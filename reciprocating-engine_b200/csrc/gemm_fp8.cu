@@ -11,24 +11,32 @@
 //
 //   acc[m][n] = fma(s, d[m][n], acc[m][n]),  s = sx[m][b] * sw[n / 128][b]
 //
-// Tile: 128 token rows (the MMA's M, one TMEM lane each) x BN weight rows
-// (its N).  A lane's scale is one value for a whole 128-column weight block,
-// so the step out of TMEM is one FMA per element.  Both operands are copied
-// by TMA as {128 k, rows} boxes with the 128-byte swizzle, which is the
-// K-major operand layout; rows and columns past the matrix read as zeros.
-// Roles: warp 0 copies, warp 1 owns TMEM and issues the MMAs, warps 2.. hold
-// the accumulators (a warp reads the TMEM lanes of its quarter, warp % 4).
-// The MMAs of block b + 1 run into another TMEM buffer while block b's sum is
-// added.  Few tiles (decode): K is split over the CTAs of a cluster, each
-// leaves its f32 partial in its own shared memory and all of them add a share
-// of the columns in rank order over distributed shared memory, so the result
-// does not depend on arrival order and no workspace is needed.
+// Tile: 128 token rows (the MMA's M, one TMEM lane each) x bn weight rows
+// (its N, a multiple of 32 up to 256 chosen per call).  A lane's scale is one
+// value for all columns of a weight block, so the step out of TMEM is one FMA
+// per element.  Both operands are copied by TMA as {128 k, rows} boxes with
+// the 128-byte swizzle, which is the K-major operand layout; rows and columns
+// past the matrix read as zeros.
+// Roles (384 threads): warp 0 copies, warp 1 owns TMEM and issues the MMAs,
+// warps 4-11 hold the accumulators (a warp reads the TMEM lanes of its
+// quarter, warp % 4, and one half of the columns; 128 accumulators a thread,
+// so the copy warps hand them their registers).  The MMAs of block b + 1 run
+// into the other TMEM buffer while block b's sum is added.
+//   * Many rows (PAIR): two CTAs of a cluster multiply one 256-row tile with
+//     tcgen05 cta_group::2; each loads its own 128 token rows and half of the
+//     weight rows, so the bytes an SM takes from L2 per block drop from 48 to
+//     32 KB at bn = 256.
+//   * Few tiles (decode): K is split over the CTAs of a cluster, each leaves
+//     its f32 partial in its own shared memory and all of them add a share of
+//     the columns in rank order over distributed shared memory, so the result
+//     does not depend on arrival order and no workspace is needed.
 // Every wait is bounded (tc.cuh); one that runs out records RENG_E_TIMEOUT in
 // a device word, and the call's results are invalid.
 #include <cooperative_groups.h>
 #include <cuda.h>
 
 #include <algorithm>
+#include <atomic>
 #include <mutex>
 #include <string>
 
@@ -39,12 +47,34 @@
 namespace reng {
 using namespace tc;
 
+int gemv_fp8_blocks(const uint8_t* x, int64_t ldx, const float* sx, int64_t ldsx, int x_fmt, const uint8_t* w,
+                    int64_t ldw, const float* sw, int64_t ldsw, int w_fmt, int M, int N, int K, void* y, int y_type,
+                    int64_t ldy, cudaStream_t st);
+
 namespace {
 
-constexpr int kRows = 128;       // token rows of a tile (the MMA's M)
+// Weight elements up to which gemv_fp8.cu runs calls of at most 8, and of 9 to
+// 16, token rows.  Measured on B200 (us, that kernel against this one): 8 rows
+// 6144 x 4096 7.1 / 12.3, 4096 x 14336 13.0 / 17.2, 28672 x 4096 27.2 / 22.9;
+// 16 rows 6144 x 4096 11.6 / 13.2, 28672 x 4096 44.7 / 23.2.
+constexpr int64_t kGemvElems[2] = {(int64_t)1 << 26, (int64_t)1 << 25};
+
+constexpr int kRows = 128;       // token rows of a CTA (one TMEM lane each)
 constexpr int kBK = 128;         // k of a block: one swizzled row of 8-bit codes
+constexpr int kMaxBn = 256;      // TMEM columns of a buffer; two buffers fill TMEM
 constexpr int kMaxStages = 12;
-constexpr int kMaxSplit = 8;     // a portable cluster
+constexpr int kMaxSplit = 4;     // K splits of a tile (CTAs of a cluster): 1, 2 or 4
+constexpr int kPartRows = 132;   // a split's partial: rows of a column, padded
+constexpr int kThreads = 384;    // a warpgroup of roles, two of accumulators
+constexpr int kAccWarps = 8;
+// an accumulator warp's staging for its output: 32 rows of 16 columns, 17
+// apart, or (PAIR) as many swizzled 32 x 32 boxes as fit 8 KB
+constexpr int kStageOut = 32 * 17 * 4, kStageOutPair = 8192;
+constexpr int kScaleSlots = 4;   // scales in flight, 4 blocks a slot:
+constexpr int kScaleSlot = kRows * 16 + 64;  // [128 rows][4] of x, [3 weight blocks][4] of w
+// registers per thread after the hand-over: 128 x 40 + 256 x 232 = 384 x 168,
+// the registers that the block is launched with
+constexpr int kRegsRole = 40, kRegsAcc = 232;
 
 __device__ int g_fp8_gemm_err;   // set by a product whose waits ran out
 
@@ -53,10 +83,13 @@ struct Fp8Gemm {
     void* y;
     int64_t ldsx, ldsw, ldy;
     int M, N, kb;      // rows, columns, 128-k blocks
-    int mt, nt;        // tiles
-    int ks;            // K splits (CTAs of a cluster)
+    int mt, nt, bn;    // tiles and their width
+    int group;         // row tiles walked before the next column tile
+    int ks;            // K splits (CTAs of a cluster; 1 with PAIR)
     int stages, mbox;  // pipeline stages, token rows of an x copy
-    int y_f32, vec;    // output type; 16-byte stores allowed
+    int y_f32;         // output type
+    int y_vec, y_tma;  // y's rows start on 32 bytes; y is written by tensor copies (PAIR)
+    int sx_vec;        // x's scales can be copied 4 at a time
     uint32_t idesc;
     int* err;
 };
@@ -81,221 +114,670 @@ __device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
                    "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
                    "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
-__device__ __forceinline__ void umma_f8(uint32_t tmem, uint64_t adesc, uint64_t bdesc, uint32_t idesc, uint32_t acc) {
+// Two f32 in one register pair, and acc = s * v + acc on both.
+__device__ __forceinline__ unsigned long long pair2(uint32_t lo, uint32_t hi) {
+    unsigned long long r;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
+    return r;
+}
+__device__ __forceinline__ void unpair2(unsigned long long v, float& lo, float& hi) {
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
+}
+__device__ __forceinline__ void fma2(unsigned long long& acc, unsigned long long v, unsigned long long s) {
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s));
+}
+// One MMA of 32 k: the operands' descriptors are K-major, 128-byte swizzle
+// (tc.cuh, umma_desc), given by their low words (address / 16, the only part
+// that changes).
+constexpr uint32_t kDescLo = 1u << 16, kDescHi = (1024u >> 4) | 1u << 14 | 2u << 29;
+template <bool PAIR>
+__device__ __forceinline__ void umma_f8(uint32_t tmem, uint32_t alo, uint32_t blo, uint32_t idesc, bool acc) {
+    if (PAIR)
+        asm volatile(
+            "{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::2.kind::f8f6f4 [%0], a, b, %3, p;\n}\n" ::"r"(tmem),
+            "r"(alo), "r"(blo), "r"(idesc), "r"((uint32_t)acc), "r"(kDescHi)
+            : "memory");
+    else
+        asm volatile(
+            "{\n .reg .pred p;\n .reg .b64 a, b;\n mov.b64 a, {%1, %5};\n mov.b64 b, {%2, %5};\n setp.ne.b32 p, %4, 0;\n"
+            " tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n}\n" ::"r"(tmem),
+            "r"(alo), "r"(blo), "r"(idesc), "r"((uint32_t)acc), "r"(kDescHi)
+            : "memory");
+}
+// Arrives at `bar` (in both CTAs of a pair) when the MMAs issued so far are done.
+template <bool PAIR>
+__device__ __forceinline__ void commit(uint32_t bar) {
+    if (PAIR)
+        asm volatile(
+            "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;" ::"r"(bar),
+            "h"((uint16_t)3)
+            : "memory");
+    else
+        umma_commit(bar);
+}
+// The address of a shared-memory object of the pair's (or split's) CTA `rank`.
+__device__ __forceinline__ uint32_t map_cta(uint32_t saddr, uint32_t rank) {
+    uint32_t r;
+    asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(saddr), "r"(rank));
+    return r;
+}
+// A tile copy whose bytes are counted at the pair leader's barrier.
+__device__ __forceinline__ void pair_g2s(uint32_t dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
     asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n}\n" ::
-            "r"(tmem),
-        "l"(adesc), "l"(bdesc), "r"(idesc), "r"(acc)
+        "cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], "
+        "[%4];" ::"r"(dst),
+        "l"(map), "r"(x), "r"(y), "r"(bar)
         : "memory");
 }
-// A bounded wait whose outcome every lane of the warp shares.
-__device__ __forceinline__ bool warp_wait(uint32_t b, uint32_t parity) {
-    return __all_sync(0xffffffffu, bar_wait(b, parity));
+__device__ __forceinline__ void tensor_s2g(const CUtensorMap* map, int x, int y, uint32_t src) {
+    asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%1, %2}], [%3];" ::"l"(map), "r"(x), "r"(y),
+                 "r"(src)
+                 : "memory");
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+}
+// At most `N` of this thread's output copies still read their staging.
+template <int N>
+__device__ __forceinline__ void s2g_wait_read() {
+    asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void st_shared16(uint32_t addr, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
+    asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(addr), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
+}
+// The role warps run their loops whole, with one elected lane issuing: their
+// addresses and descriptors then live in uniform registers, where the copy
+// and MMA instructions take them (run by one lane of a divergent warp, the
+// four MMAs of a block took 365 cycles to issue).
+__device__ __forceinline__ bool elect_lane() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred q;\n elect.sync _|q, 0xffffffff;\n selp.u32 %0, 1, 0, q;\n}\n" : "=r"(p));
+    return p != 0;
+}
+// A bounded wait: some tries without a look at the clock (a wait is taken at
+// every block, and most succeed at once), then tc.cuh's.  `bad` is sticky and
+// per lane: once a wait ran out a lane waits no more and runs on through its
+// loop on whatever is there, in bounds and to the same end as its warp, so
+// nothing diverges at the warp-wide TMEM loads.
+__device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, bool& bad) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n .reg .u32 n;\n mov.u32 n, 0;\n"
+        "TRY: mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n @p bra DONE;\n"
+        " add.u32 n, n, 1;\n setp.lt.u32 p, n, 32;\n @p bra TRY;\n setp.ne.u32 p, n, n;\n"
+        "DONE: selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    if (!ok && !bad) bad = !bar_wait(bar, parity);
+}
+// The answer to a wait takes over 100 cycles even when the phase is complete,
+// so the loops ask for their next one ahead of the work between (`early`,
+// which does not block) and wait only if that answer was no.
+__device__ __forceinline__ uint32_t early(uint32_t bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(bar), "r"(parity)
+        : "memory");
+    return ok;
+}
+__device__ __forceinline__ void wait(uint32_t asked, uint32_t bar, uint32_t parity, bool& bad) {
+    if (!asked) wait(bar, parity, bad);
+}
+// Lane 0's arrival, at a barrier of this CTA or (PAIR) of the pair's leader.
+template <bool PAIR>
+__device__ __forceinline__ void lane0_arrive(uint32_t bar, int lane) {
+    if (PAIR)
+        asm volatile(
+            "{\n .reg .pred p;\n .reg .b32 r;\n setp.eq.s32 p, %1, 0;\n mapa.shared::cluster.u32 r, %0, 0;\n"
+            " @p mbarrier.arrive.shared::cluster.b64 _, [r];\n}\n" ::"r"(bar), "r"(lane) : "memory");
+    else
+        asm volatile("{\n .reg .pred p;\n setp.eq.s32 p, %1, 0;\n @p mbarrier.arrive.shared::cta.b64 _, [%0];\n}\n" ::"r"(bar),
+                     "r"(lane)
+                     : "memory");
+}
+// Asynchronous copies of 16 and 4 bytes, and an arrival when this lane's are in.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t dst, const void* src) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void copies_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ float lds_f(uint32_t addr) {
+    float v;
+    asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sts_f(uint32_t addr, float v) {
+    asm volatile("st.shared.f32 [%0], %1;" ::"r"(addr), "f"(v) : "memory");
+}
+// 32 bytes, a whole sector, at once.
+__device__ __forceinline__ void st_global32(void* p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]),
+                 "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
 }
 
-// BN: weight rows of a tile; EW: accumulator warps (4, or 8 sharing the
-// columns of a lane quarter); NB: TMEM buffers of BN columns.
-template <int BN, int EW, int NB>
-__global__ void __launch_bounds__(64 + 32 * EW, 1)
-    k_gemm_fp8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap, Fp8Gemm a) {
+// The tile of index t: row tiles fastest within groups of `group`, so the
+// CTAs at work together share a few row and column tiles in L2.
+struct TileAt {
+    int mi, ni;
+};
+__device__ __forceinline__ TileAt tile_at(const Fp8Gemm& a, long long t) {
+    const long long per = (long long)a.group * a.nt;
+    const int g = (int)(t / per), first = g * a.group, rows = min(a.group, a.mt - first);
+    const int in = (int)(t - g * per);
+    return {first + in % rows, in / rows};
+}
+
+// The barriers of a CTA: operand stages filled and free, halves of TMEM
+// buffers filled and free ([buffer][half]), scale slots filled and free, the
+// last MMA done.
+enum : int {
+    B_FULL = 0,
+    B_EMPTY = B_FULL + kMaxStages,
+    B_TFULL = B_EMPTY + kMaxStages,
+    B_TEMPTY = B_TFULL + 4,
+    B_SFULL = B_TEMPTY + 4,
+    B_SEMPTY = B_SFULL + kScaleSlots,
+    B_DRAIN = B_SEMPTY + kScaleSlots,
+    kBars
+};
+
+// What an accumulator warp does with the blocks k0 .. k1 - 1 of a tile: NC
+// chunks of 32 columns, of one weight block or (TWO) of two, the second from
+// column `edge` (a multiple of 32) on.  NC 0: the warp has no outputs here and
+// only keeps the barriers' count.
+struct AccState {
+    uint32_t tmem, bar0;     // this warp's TMEM lanes and columns; the barriers
+    int half;                // its half of the columns
+    uint32_t sx, sw;         // scales in slot 0: this lane's row, this warp's weight block
+    int lane, d, slot;       // the TMEM buffer and the scale slot of the next block
+    uint32_t dph, sph;       // their phases
+    bool bad;
+};
+template <bool PAIR, int NC, bool TWO>
+__device__ __forceinline__ void add_blocks(AccState& st, int k0, int k1, int edge, unsigned long long (&acc)[64]) {
+    uint32_t td = 0, ts = 0;  // early answers for the next block's sum and the next slot of scales
+    float x = 0.f, w0 = 0.f, w1 = 0.f;  // the next block's scales
+    wait(st.bar0 + 8u * (B_SFULL + st.slot), st.sph, st.bad);
+    if (NC > 0) {
+        x = lds_f(st.sx + st.slot * kScaleSlot);
+        w0 = lds_f(st.sw + st.slot * kScaleSlot);
+        if (TWO) w1 = lds_f(st.sw + st.slot * kScaleSlot + 16);
+    }
+    for (int b = k0; b < k1; b++) {
+        const float s0 = x * w0, s1 = x * w1;
+        const uint32_t src = st.tmem + st.d * kMaxBn, tempty = st.bar0 + 8u * (B_TEMPTY + 2 * st.d + st.half);
+        wait(td, st.bar0 + 8u * (B_TFULL + 2 * st.d + st.half), st.dph, st.bad);
+        if ((st.d ^= 1) == 0) st.dph ^= 1u;
+        __syncwarp();
+        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+        // two chunks at a time: half of the sum is read before the first
+        // half is added, and the buffer is free before the second is
+#pragma unroll
+        for (int g = 0; g < (NC > 0 ? NC : 1); g += 2) {
+            uint32_t v[2][32];
+            if (NC > g) tmem_ld32(src + 32 * g, v[0]);
+            if (NC > g + 1) tmem_ld32(src + 32 * g + 32, v[1]);
+            if (NC > g) tmem_wait32(v[0]);
+            if (NC > g + 1) tmem_wait32(v[1]);
+            if (g + 2 >= NC) {
+                asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                __syncwarp();
+                lane0_arrive<PAIR>(tempty, st.lane);
+                td = early(st.bar0 + 8u * (B_TFULL + 2 * st.d + st.half), st.dph);
+                const int q = (b - k0) & 3;
+                if (q == 2) {
+                    const int next = st.slot + 1 == kScaleSlots ? 0 : st.slot + 1;
+                    ts = early(st.bar0 + 8u * (B_SFULL + next), next ? st.sph : st.sph ^ 1u);
+                }
+                if (q == 3 || b + 1 == k1) {
+                    lane0_arrive<false>(st.bar0 + 8u * (B_SEMPTY + st.slot), st.lane);
+                    if (++st.slot == kScaleSlots) st.slot = 0, st.sph ^= 1u;
+                    if (b + 1 < k1) wait(ts, st.bar0 + 8u * (B_SFULL + st.slot), st.sph, st.bad);
+                }
+                if (NC > 0 && b + 1 < k1) {
+                    const uint32_t at = st.slot * kScaleSlot + ((b + 1 - k0) & 3) * 4;
+                    x = lds_f(st.sx + at);
+                    w0 = lds_f(st.sw + at);
+                    if (TWO) w1 = lds_f(st.sw + at + 16);
+                }
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if (g + h >= NC) break;
+                const float s = TWO && 32 * (g + h) >= edge ? s1 : s0;
+                const unsigned long long ss = pair2(__float_as_uint(s), __float_as_uint(s));
+#pragma unroll
+                for (int i = 0; i < 16; i++) fma2(acc[16 * (g + h) + i], pair2(v[h][2 * i], v[h][2 * i + 1]), ss);
+            }
+        }
+    }
+}
+template <bool PAIR>
+__device__ __forceinline__ void add_tile(AccState& st, int nc, bool two, int k0, int k1, int edge,
+                                         unsigned long long (&acc)[64]) {
+    if (nc == 0) add_blocks<PAIR, 0, false>(st, k0, k1, edge, acc);
+    else if (nc == 4 && !two) add_blocks<PAIR, 4, false>(st, k0, k1, edge, acc);
+    else if (nc == 4) add_blocks<PAIR, 4, true>(st, k0, k1, edge, acc);
+    else if (nc == 3) add_blocks<PAIR, 3, true>(st, k0, k1, edge, acc);
+    else if (nc == 2) add_blocks<PAIR, 2, true>(st, k0, k1, edge, acc);
+    else add_blocks<PAIR, 1, false>(st, k0, k1, edge, acc);
+}
+
+// Every thread of the CTA (of a pair: of both) is through with TMEM.
+template <bool PAIR>
+__device__ __forceinline__ void cta_end() {
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    if (PAIR) cooperative_groups::this_cluster().sync();
+    else __syncthreads();
+}
+
+// The sum of a cluster's partials of one tile, in rank order: CTA `rank` adds
+// the columns from rank * share on.  An accumulator thread takes 4 rows of one
+// column at a time, two such items and all ranks' reads in flight, since a
+// read of a peer's shared memory takes about a microsecond.
+__device__ __forceinline__ void add_partials(const Fp8Gemm& a, float* part, int m0, int n0, int rank) {
+    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
+    const int rows = min(kRows, a.M - m0), cols = min(a.bn, a.N - n0);
+    const int share = (cols + a.ks - 1) / a.ks, c0 = rank * share, nc = min(share, cols - c0);
+    const int items = nc > 0 ? (rows + 3) / 4 * nc : 0;
+    for (int i = threadIdx.x - (kThreads - 32 * kAccWarps); i < items; i += 2 * 32 * kAccWarps) {
+        float4 v[2][kMaxSplit];
+        int c[2], row[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            const int j = i + u * 32 * kAccWarps;
+            row[u] = j < items ? j / nc * 4 : rows;
+            c[u] = c0 + j % nc;
+#pragma unroll
+            for (int q = 0; q < kMaxSplit; q++)
+                if (q < a.ks && j < items)
+                    v[u][q] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&part[c[u] * kPartRows + row[u]], q));
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            float s[4] = {0.f, 0.f, 0.f, 0.f};
+            if (row[u] < rows) {
+#pragma unroll
+                for (int q = 0; q < kMaxSplit; q++)
+                    if (q < a.ks) s[0] += v[u][q].x, s[1] += v[u][q].y, s[2] += v[u][q].z, s[3] += v[u][q].w;
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                if (row[u] + e >= rows) break;
+                const size_t to = (size_t)(m0 + row[u] + e) * a.ldy + n0 + c[u];
+                if (a.y_f32) static_cast<float*>(a.y)[to] = s[e];
+                else static_cast<uint16_t*>(a.y)[to] = (uint16_t)bf16x2(s[e], 0.f);
+            }
+        }
+    }
+}
+
+template <bool PAIR>
+__global__ void __launch_bounds__(kThreads, 1)
+    k_gemm_fp8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
+               const __grid_constant__ CUtensorMap ymap, const Fp8Gemm a) {
     namespace cg = cooperative_groups;
-    constexpr int CW = BN / (EW / 4);  // columns of one accumulator warp
-    static_assert(CW % 32 == 0 && CW <= 128 && NB * BN <= 512, "tile shape");
     extern __shared__ __align__(1024) uint8_t smem_raw[];
-    __shared__ __align__(8) unsigned long long full[kMaxStages], empty[kMaxStages], tfull[NB], tempty[NB], drain;
+    __shared__ __align__(8) unsigned long long bars[kBars];
     __shared__ uint32_t tmem_base_s;
 
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int warp = __shfl_sync(0xffffffffu, threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     const uint32_t smem0 = ((uint32_t)__cvta_generic_to_shared(smem_raw) + 1023u) & ~1023u;
-    const uint32_t abytes = (uint32_t)a.mbox * kBK, bbytes = (uint32_t)BN * kBK;
+    const uint32_t brows = PAIR ? (uint32_t)a.bn / 2 : (uint32_t)a.bn;
+    const uint32_t abytes = (uint32_t)a.mbox * kBK, bbytes = brows * kBK;
     // x stages first: the MMA reads 128 rows from each, past a shorter box
     // into what follows, and the lanes of those rows are never used
-    const uint32_t sA = smem0, sB = smem0 + (uint32_t)a.stages * abytes;
-    auto bar = [](unsigned long long* b) { return (uint32_t)__cvta_generic_to_shared(b); };
+    const uint32_t sA = smem0, sB = sA + (uint32_t)a.stages * abytes, sOut = sB + (uint32_t)a.stages * bbytes,
+                   sScale = sOut + kAccWarps * (PAIR ? kStageOutPair : kStageOut);  // 16-byte aligned
+    const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(bars);
+    auto bar = [bar0](int first, int i = 0) { return bar0 + 8u * (uint32_t)(first + i); };
+    const bool clustered = PAIR || a.ks > 1;
+    const int rank = clustered ? (int)cg::this_cluster().block_rank() : 0;
+    int* const err = a.err ? a.err : &g_fp8_gemm_err;
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; s++) {
-            bar_init(bar(&full[s]), 1);
-            bar_init(bar(&empty[s]), 1);
+            bar_init(bar(B_FULL, s), 1);
+            bar_init(bar(B_EMPTY, s), 1);
         }
-        for (int s = 0; s < NB; s++) {
-            bar_init(bar(&tfull[s]), 1);
-            bar_init(bar(&tempty[s]), EW);
+        for (int s = 0; s < 4; s++) {
+            bar_init(bar(B_TFULL, s), 1);
+            bar_init(bar(B_TEMPTY, s), kAccWarps);  // a pair's: half the warps of two CTAs
         }
-        bar_init(bar(&drain), 1);
+        for (int s = 0; s < kScaleSlots; s++) {
+            bar_init(bar(B_SFULL, s), 32);
+            bar_init(bar(B_SEMPTY, s), kAccWarps);
+        }
+        bar_init(bar(B_DRAIN), 1);
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
     }
     if (warp == 1) {
         const uint32_t dst = (uint32_t)__cvta_generic_to_shared(&tmem_base_s);
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(dst), "r"(NB * BN)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        if (PAIR) {
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dst) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        } else {
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(dst) : "memory");
+            asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+        }
     }
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
+    if (PAIR) cg::this_cluster().sync();  // the peer's barriers and TMEM are ready too
+    else __syncthreads();
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t tmem = tmem_base_s;
     pdl_wait();
     pdl_launch();
 
-    const int rank = a.ks > 1 ? (int)cg::this_cluster().block_rank() : 0;
-    const int k0 = (int)((long long)rank * a.kb / a.ks), k1 = (int)((long long)(rank + 1) * a.kb / a.ks);
-    const long long tiles = (long long)a.mt * a.nt, tstep = gridDim.x / a.ks;
+    const int h0 = (a.bn / 2 + 31) / 32 * 32;  // columns of the first half
+    const int split = PAIR ? 0 : rank, span = PAIR ? 2 : a.ks;  // CTAs per tile
+    const int k0 = (int)((long long)split * a.kb / a.ks), k1 = (int)((long long)(split + 1) * a.kb / a.ks);
+    const long long tiles = (long long)a.mt * a.nt, first = blockIdx.x / span, tstep = gridDim.x / span;
+    constexpr int kTileRows_ = PAIR ? 2 * kRows : kRows;
 
-    if (warp == 0) {
-        if (lane == 0) {
+    if (warp < 4) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kRegsRole));
+        const bool leader = elect_lane();
+        bool bad = false;
+        if (warp == 0) {
+            // ---- copies of the operands' codes ----
             int s = 0, issued = 0;
             uint32_t ph = 0;
-            bool ok = true;
-            for (long long t = blockIdx.x / a.ks; t < tiles && ok; t += tstep) {
-                const int m0 = (int)(t % a.mt) * kRows, n0 = (int)(t / a.mt) * BN;
+            for (long long t = first; t < tiles && !bad; t += tstep) {
+                const TileAt at = tile_at(a, t);
+                const int m0 = at.mi * kTileRows_ + (PAIR ? rank * kRows : 0);
+                const int n0 = at.ni * a.bn + (PAIR ? rank * (int)brows / 2 : 0);
                 for (int b = k0; b < k1; b++) {
-                    if (issued >= a.stages && !(ok = bar_wait(bar(&empty[s]), ph ^ 1u))) break;
-                    bar_expect_tx(bar(&full[s]), abytes + bbytes);
-                    tensor_g2s(sA + (uint32_t)s * abytes, &xmap, b * kBK, m0, bar(&full[s]));
-                    tensor_g2s(sB + (uint32_t)s * bbytes, &wmap, b * kBK, n0, bar(&full[s]));
+                    if (issued >= a.stages) {
+                        wait(bar(B_EMPTY, s), ph ^ 1u, bad);
+                        if (__any_sync(0xffffffffu, bad)) break;
+                    }
+                    const uint32_t xs = sA + (uint32_t)s * abytes, ws = sB + (uint32_t)s * bbytes;
+                    if (leader) {
+                        if (PAIR) {
+                            // the leader CTA's barrier counts the bytes of both
+                            if (rank == 0) bar_expect_tx(bar(B_FULL, s), 2 * (abytes + bbytes));
+                            const uint32_t fb = map_cta(bar(B_FULL, s), 0);
+                            pair_g2s(xs, &xmap, b * kBK, m0, fb);
+                            // each half of the columns: this CTA's half of its rows
+                            pair_g2s(ws, &wmap, b * kBK, n0, fb);
+                            pair_g2s(ws + bbytes / 2, &wmap, b * kBK, n0 + a.bn / 2, fb);
+                        } else {
+                            bar_expect_tx(bar(B_FULL, s), abytes + bbytes);
+                            tensor_g2s(xs, &xmap, b * kBK, m0, bar(B_FULL, s));
+                            tensor_g2s(ws, &wmap, b * kBK, n0, bar(B_FULL, s));
+                        }
+                    }
                     issued = issued < a.stages ? issued + 1 : issued;
                     if (++s == a.stages) s = 0, ph ^= 1u;
                 }
+                bad = __any_sync(0xffffffffu, bad);
             }
-            if (!ok) {
-                atomicExch(a.err ? a.err : &g_fp8_gemm_err, RENG_E_TIMEOUT);
+            if (bad) {
+                if (leader) atomicExch(err, RENG_E_TIMEOUT);
                 // the last copy into each stage lands before the CTA may exit
-                for (int i = 0; i < issued; i++) {
-                    s = s == 0 ? (ph ^= 1u, a.stages - 1) : s - 1;
-                    if (!bar_wait(bar(&full[s]), ph)) break;
+                // (a pair's follower is kept by the cluster barrier at the end)
+                for (int i = 0; i < issued && (!PAIR || rank == 0); i++) {
+                    if (s == 0) s = a.stages, ph ^= 1u;
+                    s--;
+                    if (!__all_sync(0xffffffffu, bar_wait(bar(B_FULL, s), ph))) break;
                 }
             }
-        }
-    } else if (warp == 1) {
-        if (lane == 0) {
+        } else if (warp == 1 && (!PAIR || rank == 0)) {
+            // ---- MMAs; a pair's in two halves of the columns, so that one
+            // half's sum is taken out while the other's runs ----
             int s = 0, d = 0, used = 0;
-            uint32_t ph = 0, dph = 0;
-            bool ok = true;
-            for (long long t = blockIdx.x / a.ks; t < tiles && ok; t += tstep) {
+            uint32_t ph = 0, dph = 0, af = 0, ae[2] = {0, 0};  // early answers: the stage, the buffer's halves
+            const uint32_t alo0 = kDescLo | sA >> 4, blo0 = kDescLo | sB >> 4;
+            const uint32_t idesc = a.idesc | (uint32_t)((PAIR ? a.bn / 2 : a.bn) >> 3) << 17;
+            for (long long t = first; t < tiles; t += tstep) {
                 for (int b = k0; b < k1; b++) {
-                    ok = bar_wait(bar(&full[s]), ph) && (used < NB || bar_wait(bar(&tempty[d]), dph ^ 1u));
-                    if (!ok) break;
+                    const uint32_t alo = alo0 + ((uint32_t)s * abytes >> 4), blo = blo0 + ((uint32_t)s * bbytes >> 4);
+                    const uint32_t dst = tmem + d * kMaxBn, done = bar(B_TFULL, 2 * d), gone = bar(B_EMPTY, s);
+                    const uint32_t free0 = bar(B_TEMPTY, 2 * d), fph = dph ^ 1u;
+                    wait(af, bar(B_FULL, s), ph, bad);
+                    if (used >= 2) wait(ae[0], free0, fph, bad);
+                    __syncwarp();
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    if (leader && !bad) {
 #pragma unroll
-                    for (int kk = 0; kk < 4; kk++)
-                        umma_f8(tmem + d * BN, umma_desc(sA + (uint32_t)s * abytes + kk * 32),
-                                umma_desc(sB + (uint32_t)s * bbytes + kk * 32), a.idesc, kk ? 1u : 0u);
-                    umma_commit(bar(&empty[s]));
-                    umma_commit(bar(&tfull[d]));
-                    used = used < NB ? used + 1 : used;
+                        for (int kk = 0; kk < 4; kk++) umma_f8<PAIR>(dst, alo + 2 * kk, blo + 2 * kk, idesc, kk != 0);
+                        commit<PAIR>(done);
+                        if (!PAIR) commit<PAIR>(gone);
+                    }
                     if (++s == a.stages) s = 0, ph ^= 1u;
-                    if (++d == NB) d = 0, dph ^= 1u;
+                    if ((d ^= 1) == 0) dph ^= 1u;
+                    if (PAIR) {
+                        if (used >= 2) wait(ae[1], free0 + 8u, fph, bad);
+                        __syncwarp();
+                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                        ae[1] = early(bar(B_TEMPTY, 2 * d + 1), dph ^ 1u);
+                    }
+                    af = early(bar(B_FULL, s), ph);
+                    ae[0] = early(bar(B_TEMPTY, 2 * d), dph ^ 1u);
+                    used = used < 2 ? used + 1 : used;
+                    if (PAIR && leader && !bad) {
+#pragma unroll
+                        for (int kk = 0; kk < 4; kk++)
+                            umma_f8<PAIR>(dst + h0, alo + 2 * kk, blo + (bbytes / 2 >> 4) + 2 * kk, idesc, kk != 0);
+                        commit<PAIR>(done + 8u);
+                        commit<PAIR>(gone);
+                    }
                 }
             }
-            if (!ok) atomicExch(a.err ? a.err : &g_fp8_gemm_err, RENG_E_TIMEOUT);
             // every MMA issued has completed before TMEM is freed
-            umma_commit(bar(&drain));
-            if (!bar_wait(bar(&drain), 0)) atomicExch(a.err ? a.err : &g_fp8_gemm_err, RENG_E_TIMEOUT);
+            if (leader) {
+                if (PAIR)
+                    asm volatile(
+                        "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar(B_DRAIN))
+                        : "memory");
+                else
+                    umma_commit(bar(B_DRAIN));
+            }
+            bad = !bar_wait(bar(B_DRAIN), 0) || bad;
+            if (bad) atomicExch(err, RENG_E_TIMEOUT);
+            __syncwarp();
+        } else if (warp == 2) {
+            // ---- copies of the scales, 4 blocks at a time ----
+            int slot = 0, used = 0;
+            uint32_t ph = 0;
+            const bool vec = a.sx_vec && (k0 & 3) == 0;
+            for (long long t = first; t < tiles; t += tstep) {
+                const TileAt at = tile_at(a, t);
+                const int m0 = at.mi * kTileRows_ + (PAIR ? rank * kRows : 0);
+                const int wb = min(at.ni * a.bn / kBK + (lane >> 2), (a.N - 1) / kBK);
+                for (int b = k0; b < k1; b += 4) {
+                    if (used >= kScaleSlots) wait(bar(B_SEMPTY, slot), ph ^ 1u, bad);
+                    const uint32_t dst = sScale + slot * kScaleSlot;
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const int r = 32 * i + lane;
+                        if (m0 + r >= a.M) break;
+                        const float* src = a.sx + (size_t)(m0 + r) * a.ldsx + b;
+                        if (vec && b + 4 <= k1) {
+                            copy16(dst + 16 * r, src);
+                        } else {
+                            for (int j = 0; j < 4 && b + j < k1; j++) copy4(dst + 16 * r + 4 * j, src + j);
+                        }
+                    }
+                    if (lane < 12 && b + (lane & 3) < k1)
+                        copy4(dst + kRows * 16 + 4 * lane, a.sw + (size_t)wb * a.ldsw + b + (lane & 3));
+                    copies_arrive(bar(B_SFULL, slot));
+                    used = used < kScaleSlots ? used + 1 : used;
+                    if (++slot == kScaleSlots) slot = 0, ph ^= 1u;
+                }
+            }
+            if (bad) atomicExch(err, RENG_E_TIMEOUT);
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        }
+        // the end of the CTA, said by each side of the register hand-over for
+        // itself: no code after it is shared
+        cta_end<PAIR>();
+        if (warp == 1) {
+            asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+            if (PAIR)
+                asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+            else
+                asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
+        }
+        if (!PAIR && a.ks > 1) {
+            cg::this_cluster().sync();  // the partials are complete (TMEM is already free: a CTA
+            cg::this_cluster().sync();  // that waits for its peers here holds none), and read
         }
     } else {
-        const int half = (warp - 2) >> 2;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsAcc));
+        const int half = (warp - 4) >> 2;
         const int r = 32 * (warp & 3) + lane;
-        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        int d = 0;
-        uint32_t dph = 0;
-        bool ok = true;
-        for (long long t = blockIdx.x / a.ks; t < tiles; t += tstep) {
-            const int m = (int)(t % a.mt) * kRows + r, n0 = (int)(t / a.mt) * BN + half * CW;
-            const bool live = m < a.M;
-            const bool any = m - lane < a.M && n0 < a.N;  // the warp has outputs in this tile
-            float acc[CW];
+        // this warp's columns of a tile (multiples of 32)
+        const int c0 = half ? h0 : 0, cw = half ? a.bn - h0 : h0;
+        const uint32_t out0 = sOut + (uint32_t)(warp - 4) * (PAIR ? kStageOutPair : kStageOut);
+        uint32_t box = 0;  // staging box of the next output copy
+        AccState st;
+        st.tmem = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + c0;
+        st.bar0 = bar0;
+        st.half = PAIR ? half : 0;  // without a pair the buffer is filled and freed whole
+        st.sx = sScale + 16 * r;
+        st.lane = lane;
+        st.d = st.slot = 0;
+        st.dph = st.sph = 0;
+        st.bad = false;
+        for (long long t = first; t < tiles; t += tstep) {
+            const TileAt at = tile_at(a, t);
+            const int mw = at.mi * kTileRows_ + (PAIR ? rank * kRows : 0) + 32 * (warp & 3), m = mw + lane;
+            const int n0 = at.ni * a.bn + c0;
+            const bool any = mw < a.M && n0 < a.N && cw > 0;  // the warp has outputs in this tile
+            unsigned long long acc[64];
 #pragma unroll
-            for (int c = 0; c < CW; c++) acc[c] = 0.f;
-            const float* sx = a.sx + (size_t)(live ? m : 0) * a.ldsx;
-            const float* sw = a.sw + (size_t)(n0 < a.N ? n0 / kBK : 0) * a.ldsw;
-            float sn = any ? sx[k0] * sw[k0] : 0.f;
-            for (int b = k0; b < k1; b++) {
-                const float s = sn;
-                if (any && b + 1 < k1) sn = sx[b + 1] * sw[b + 1];
-                ok = ok && warp_wait(bar(&tfull[d]), dph);
-                if (ok && any) {
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-#pragma unroll
-                    for (int g = 0; g < CW / 32; g++) {
-                        uint32_t v[32];
-                        tmem_ld32(tmem + lanes + d * BN + half * CW + g * 32, v);
-                        tmem_wait32(v);
-#pragma unroll
-                        for (int e = 0; e < 32; e++)
-                            acc[g * 32 + e] = fmaf(s, __uint_as_float(v[e]), acc[g * 32 + e]);
-                    }
-                    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-                }
-                __syncwarp();
-                if (lane == 0) bar_arrive(bar(&tempty[d]));
-                if (++d == NB) d = 0, dph ^= 1u;
-            }
-            if (!ok) {
-                if (lane == 0) atomicExch(a.err ? a.err : &g_fp8_gemm_err, RENG_E_TIMEOUT);
-#pragma unroll
-                for (int c = 0; c < CW; c++) acc[c] = __int_as_float(0x7fc00000);
-            }
-            if (a.ks > 1) {
-                // partial[column][row], 129 rows apart: conflict-free both ways
+            for (int c = 0; c < 64; c++) acc[c] = 0ull;
+            // its columns touch at most two weight blocks; the second starts at column `edge`
+            const int edge = (n0 / kBK + 1) * kBK - n0;
+            st.sw = sScale + kRows * 16 + 16 * (n0 / kBK - at.ni * a.bn / kBK);
+            add_tile<PAIR>(st, any ? cw / 32 : 0, edge < cw, k0, k1, edge, acc);
+            if (!any) continue;
+            if (!PAIR && a.ks > 1) {
+                // partial[column][row], columns kPartRows apart: conflict-free
+                // both ways, and 4 rows of a column are one 16-byte read
                 float* part = reinterpret_cast<float*>(smem_raw + (smem0 - (uint32_t)__cvta_generic_to_shared(smem_raw)));
-                if (any)
 #pragma unroll
-                    for (int c = 0; c < CW; c++) part[(half * CW + c) * 129 + r] = acc[c];
-            } else if (live && any) {
-                if (a.y_f32) {
-                    float* dst = static_cast<float*>(a.y) + (size_t)m * a.ldy + n0;
-                    if (a.vec && n0 + CW <= a.N) {
-#pragma unroll
-                        for (int c = 0; c < CW; c += 4)
-                            *reinterpret_cast<float4*>(dst + c) = make_float4(acc[c], acc[c + 1], acc[c + 2], acc[c + 3]);
-                    } else {
-#pragma unroll
-                        for (int c = 0; c < CW; c++)
-                            if (n0 + c < a.N) dst[c] = acc[c];
+                for (int c = 0; c < 64; c++) {
+                    float lo, hi;
+                    unpair2(acc[c], lo, hi);
+                    if (2 * c < cw) {
+                        part[(c0 + 2 * c) * kPartRows + r] = lo;
+                        part[(c0 + 2 * c + 1) * kPartRows + r] = hi;
                     }
-                } else {
-                    uint16_t* dst = static_cast<uint16_t*>(a.y) + (size_t)m * a.ldy + n0;
-                    if (a.vec && n0 + CW <= a.N) {
+                }
+            } else if (PAIR && a.y_tma) {
+                // 32 rows x 32 columns at a time through this warp's staging
+                // in the copy's swizzle; the copies run on behind the next tile
 #pragma unroll
-                        for (int c = 0; c < CW; c += 8)
-                            *reinterpret_cast<uint4*>(dst + c) =
-                                make_uint4(pack_bf16x2(acc[c], acc[c + 1]), pack_bf16x2(acc[c + 2], acc[c + 3]),
-                                           pack_bf16x2(acc[c + 4], acc[c + 5]), pack_bf16x2(acc[c + 6], acc[c + 7]));
+                for (int g = 0; g < 4; g++) {
+                    if (32 * g >= cw || n0 + 32 * g >= a.N) break;
+                    const unsigned long long* q = acc + 16 * g;
+                    if (a.y_f32) {  // 128-byte rows, two boxes
+                        const uint32_t buf = out0 + box * 4096u;
+                        box = (box + 1) & 1;
+                        if (lane == 0) s2g_wait_read<1>();
+                        __syncwarp();
+#pragma unroll
+                        for (int ch = 0; ch < 8; ch++) {
+                            float f0, f1, f2, f3;
+                            unpair2(q[2 * ch], f0, f1);
+                            unpair2(q[2 * ch + 1], f2, f3);
+                            st_shared16(buf + lane * 128 + ((ch ^ (lane & 7)) << 4), __float_as_uint(f0), __float_as_uint(f1),
+                                        __float_as_uint(f2), __float_as_uint(f3));
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) tensor_s2g(&ymap, n0 + 32 * g, mw, buf);
+                    } else {  // 64-byte rows, four boxes
+                        const uint32_t buf = out0 + box * 2048u;
+                        box = (box + 1) & 3;
+                        if (lane == 0) s2g_wait_read<3>();
+                        __syncwarp();
+#pragma unroll
+                        for (int ch = 0; ch < 4; ch++) {
+                            uint32_t w[4];
+#pragma unroll
+                            for (int i = 0; i < 4; i++) {
+                                float lo, hi;
+                                unpair2(q[4 * ch + i], lo, hi);
+                                w[i] = bf16x2(lo, hi);
+                            }
+                            st_shared16(buf + lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) tensor_s2g(&ymap, n0 + 32 * g, mw, buf);
+                    }
+                }
+            } else {
+#pragma unroll
+                for (int g = 0; g < 8; g++) {
+                    // 16 columns: a lane's row in whole sectors, or (any
+                    // pitch, and the matrix's last columns) by way of this
+                    // warp's staging, consecutive lanes on consecutive columns
+                    const int n = n0 + 16 * g;
+                    if (16 * g >= cw || n >= a.N) break;
+                    const unsigned long long* q = acc + 8 * g;
+                    if (a.y_vec && n + 16 <= a.N) {
+                        if (m < a.M) {
+                            uint32_t w[16];
+#pragma unroll
+                            for (int i = 0; i < 8; i++) {
+                                float lo, hi;
+                                unpair2(q[i], lo, hi);
+                                if (a.y_f32) w[2 * i] = __float_as_uint(lo), w[2 * i + 1] = __float_as_uint(hi);
+                                else w[i] = bf16x2(lo, hi);
+                            }
+                            char* dst = static_cast<char*>(a.y) + ((size_t)m * a.ldy + n) * (a.y_f32 ? 4 : 2);
+                            st_global32(dst, *reinterpret_cast<const uint32_t(*)[8]>(w));
+                            if (a.y_f32) st_global32(dst + 32, *reinterpret_cast<const uint32_t(*)[8]>(w + 8));
+                        }
                     } else {
+                        __syncwarp();
 #pragma unroll
-                        for (int c = 0; c < CW; c++)
-                            if (n0 + c < a.N) dst[c] = f32_to_bf16_bits(acc[c]);
+                        for (int i = 0; i < 8; i++) {
+                            float lo, hi;
+                            unpair2(q[i], lo, hi);
+                            sts_f(out0 + 4 * (lane * 17 + 2 * i), lo);
+                            sts_f(out0 + 4 * (lane * 17 + 2 * i + 1), hi);
+                        }
+                        __syncwarp();
+                        const int c = lane & 15;
+#pragma unroll 4
+                        for (int i = lane >> 4; i < 32; i += 2) {
+                            const float v = lds_f(out0 + 4 * (i * 17 + c));
+                            if (mw + i < a.M && n + c < a.N) {
+                                const size_t to = (size_t)(mw + i) * a.ldy + n + c;
+                                if (a.y_f32) static_cast<float*>(a.y)[to] = v;
+                                else static_cast<uint16_t*>(a.y)[to] = (uint16_t)bf16x2(v, 0.f);
+                            }
+                        }
                     }
                 }
             }
         }
-    }
-    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
-    __syncthreads();
-    if (warp == 1) {
-        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(NB * BN) : "memory");
-    }
-    if (a.ks > 1) {
-        // one tile per cluster: CTA `rank` adds columns rank, rank + ks, ...
-        cg::cluster_group cluster = cg::this_cluster();
-        cluster.sync();
-        float* part = reinterpret_cast<float*>(smem_raw + (smem0 - (uint32_t)__cvta_generic_to_shared(smem_raw)));
-        const long long t = blockIdx.x / a.ks;
-        const int m0 = (int)(t % a.mt) * kRows, n0 = (int)(t / a.mt) * BN;
-        const int rows = min(kRows, a.M - m0), cols = min(BN, a.N - n0);
-        const int share = (cols + a.ks - 1) / a.ks, c0 = rank * share, nc = min(share, cols - c0);
-        for (int i = threadIdx.x; i < rows * nc; i += blockDim.x) {
-            const int row = i / nc, c = c0 + i - row * nc;
-            float v = 0.f;
-            for (int q = 0; q < a.ks; q++) v += *cluster.map_shared_rank(&part[c * 129 + row], q);
-            const size_t at = (size_t)(m0 + row) * a.ldy + n0 + c;
-            if (a.y_f32) static_cast<float*>(a.y)[at] = v;
-            else static_cast<uint16_t*>(a.y)[at] = f32_to_bf16_bits(v);
+        if (st.bad) atomicExch(err, RENG_E_TIMEOUT);
+        // the staging is read before the CTA's shared memory goes away
+        if (PAIR && lane == 0) s2g_wait_read<0>();
+        __syncwarp();
+        cta_end<PAIR>();
+        if (!PAIR && a.ks > 1) {
+            cg::this_cluster().sync();
+            const TileAt at = tile_at(a, first);
+            add_partials(a, reinterpret_cast<float*>(smem_raw + (smem0 - (uint32_t)__cvta_generic_to_shared(smem_raw))),
+                         at.mi * kRows, at.ni * a.bn, rank);
+            cg::this_cluster().sync();  // this CTA's partial stays until its peers have read it
         }
-        cluster.sync();  // this CTA's partial stays until its peers have read it
     }
 }
 
@@ -331,42 +813,102 @@ int codes_map(const uint8_t* p, int64_t rows, int64_t K, int64_t ld, int box_row
     return RENG_OK;
 }
 
+// y [M][ldy] as {32 columns, 32 rows} boxes, swizzled as the warps stage them.
+int y_map(void* y, bool f32, int64_t M, int64_t N, int64_t ldy, CUtensorMap* out) {
+    EncodeTiledFn fn = encode_fn();
+    if (!fn) return fail(RENG_E_CUDA, "cuTensorMapEncodeTiled is not available");
+    cuuint64_t dims[2] = {(cuuint64_t)N, (cuuint64_t)M};
+    cuuint64_t strides[1] = {(cuuint64_t)ldy * (f32 ? 4 : 2)};
+    cuuint32_t box[2] = {32, 32};
+    cuuint32_t estr[2] = {1, 1};
+    const CUresult r = fn(out, f32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, y, dims,
+                          strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          f32 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(RENG_E_CUDA, "cuTensorMapEncodeTiled (y) failed (" + std::to_string((int)r) + ")");
+    return RENG_OK;
+}
+
 constexpr size_t kSmemMax = 227 * 1024 - 1024;  // dynamic shared memory of a CTA, beside its barriers
 
-template <int BN, int EW, int NB>
-int launch_tile(const CUtensorMap& xm, const CUtensorMap& wm, Fp8Gemm& a, int grid, cudaStream_t st) {
-    const size_t stage = (size_t)(a.mbox + BN) * kBK;
-    a.stages = (int)std::min<size_t>(kMaxStages, (kSmemMax - 1024) / stage);
-    size_t smem = a.stages * stage + 1024;
-    // the last x stage is read 128 rows deep; a split leaves [BN][129] partials
+template <bool PAIR>
+int launch_tiles(const CUtensorMap& xm, const CUtensorMap& wm, const CUtensorMap& ym, Fp8Gemm& a, int grid,
+                 cudaStream_t st) {
+    const int brows = PAIR ? a.bn / 2 : a.bn;
+    const size_t stage = (size_t)(a.mbox + brows) * kBK, out = (size_t)kAccWarps * (PAIR ? kStageOutPair : kStageOut) + kScaleSlots * kScaleSlot;
+    const int steps = (int)(((long long)a.mt * a.nt * (PAIR ? 2 : a.ks) + grid - 1) / grid) * ((a.kb + a.ks - 1) / a.ks);
+    a.stages = (int)std::min<size_t>({(size_t)kMaxStages, (kSmemMax - 1024 - out) / stage, (size_t)std::max(steps, 2)});
+    size_t smem = 1024 + a.stages * stage + out;
+    // the last x stage is read 128 rows deep; a split leaves its partial
     smem = std::max(smem, (size_t)1024 + (size_t)(a.stages - 1) * a.mbox * kBK + kRows * kBK);
-    if (a.ks > 1) smem = std::max(smem, (size_t)1024 + (size_t)BN * 129 * 4);
-    static std::once_flag once[16];
-    static cudaError_t prep[16] = {};
+    if (a.ks > 1) smem = std::max(smem, (size_t)1024 + (size_t)a.bn * kPartRows * 4);
+    // a pair holds TMEM on two SMs while its CTAs wait for one another: it
+    // takes all of their shared memory, so that no CTA of another launch that
+    // does the same can sit beside one of them and wait the other way round
+    if (PAIR) smem = kSmemMax;
     int dev = 0;
     RENG_CUDA_TRY(cudaGetDevice(&dev));
-    if (dev < 0 || dev >= 16) return fail(RENG_E_UNSUPPORTED, "reng_gemm_fp8_blocks: device ordinal above 15");
-    std::call_once(once[dev], [&] {
-        prep[dev] = cudaFuncSetAttribute(k_gemm_fp8<BN, EW, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                         (int)kSmemMax);
-    });
-    RENG_CUDA_TRY(prep[dev]);
+    static std::atomic<uint64_t> ready{0};  // devices whose limit is raised
+    if (dev >= 64 || !(ready.load() >> dev & 1)) {
+        RENG_CUDA_TRY(cudaFuncSetAttribute(k_gemm_fp8<PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)kSmemMax));
+        if (dev < 64) ready.fetch_or((uint64_t)1 << dev);
+    }
     cudaLaunchConfig_t cfg = {};
     cudaLaunchAttribute attr[2];
     cfg.gridDim = dim3((unsigned)grid);
-    cfg.blockDim = dim3(64 + 32 * EW);
+    cfg.blockDim = dim3(kThreads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = st;
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = a.ks;
+    attr[1].val.clusterDim.x = PAIR ? 2 : a.ks;
     attr[1].val.clusterDim.y = 1;
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = a.ks > 1 ? 2 : 1;
-    RENG_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm_fp8<BN, EW, NB>, xm, wm, a));
+    cfg.numAttrs = PAIR || a.ks > 1 ? 2 : 1;
+    RENG_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm_fp8<PAIR>, xm, wm, ym, a));
     return RENG_OK;
+}
+
+// Cycles that a plan's busiest SM takes, from what launches took on B200 (bf16
+// output, 2048 x 18944 x 4096 and x 16384): a block costs about 400 + 2.45 bn
+// cycles in one CTA and 600 + 1.5 bn in a pair, and no less than its bytes at
+// 64 a cycle from L2 and 23 from HBM when all SMs stream; a tile has a fixed
+// cost, and a split's exchange 4000 + 50 bn (64 rows x 4096 x 14336: 20.4 us
+// split by 4 against 34 whole; clusters of 3 and of 5 to 8 leave SMs of a GPC
+// empty and took twice as long).
+struct Plan {
+    bool pair;
+    int bn, ks;
+    double cost;
+};
+Plan plan(int M, int N, int kb, int sms) {
+    Plan best{false, 256, 1, 1e300};
+    const int mt1 = (M + kRows - 1) / kRows;
+    for (int pair = 0; pair <= (M > kRows ? 1 : 0); pair++) {
+        const int mt = pair ? (mt1 + 1) / 2 : mt1, slots = pair ? sms / 2 : sms, step = pair ? 64 : 32;
+        for (int ks = 1; ks <= (pair ? 1 : std::min(kMaxSplit, kb)); ks *= 2) {
+            if (ks > 1 && mt > slots / ks) break;
+            for (int w = 1; w <= 6; w++) {
+                // the narrowest tiles that fit w rounds of the SMs
+                const long long fit = (long long)w * slots / ((long long)mt * ks);
+                int bn = fit < 1 ? kMaxBn : (int)std::min<long long>(kMaxBn, ((N + fit - 1) / fit + step - 1) / step * step);
+                const long long tiles = (long long)mt * ((N + bn - 1) / bn) * ks;
+                const long long rounds = (tiles + slots - 1) / slots;
+                if (ks > 1 && rounds > 1) continue;
+                const int blocks = (kb + ks - 1) / ks;
+                const double bytes = (std::min(M, kRows) + (pair ? bn / 2 : bn)) * (double)kBK;
+                // all weights pass from HBM once; a round's share of it
+                const double hbm = (double)N * kb * kBK / (23.0 * std::min<long long>(tiles, sms)) / ((double)rounds * blocks);
+                const double block = std::max({pair ? 600.0 + 1.5 * bn : 400.0 + 2.45 * bn, bytes / 64.0, hbm});
+                const double cost = rounds * (blocks * block + (pair ? 1500.0 : 3000.0) + (ks > 1 ? 4000.0 + 50.0 * bn : 0.0));
+                if (cost < best.cost) best = {pair != 0, bn, ks, cost};
+                if (bn <= 32) break;
+            }
+        }
+    }
+    return best;
 }
 
 }  // namespace
@@ -374,6 +916,8 @@ int launch_tile(const CUtensorMap& xm, const CUtensorMap& wm, Fp8Gemm& a, int gr
 int gemm_fp8_blocks(const uint8_t* x, int64_t ldx, const float* sx, int64_t ldsx, int x_fmt, const uint8_t* w,
                     int64_t ldw, const float* sw, int64_t ldsw, int w_fmt, int M, int N, int K, void* y, int y_type,
                     int64_t ldy, int* err, cudaStream_t st) {
+    if (M <= 16 && (int64_t)N * K <= kGemvElems[M > 8])
+        return gemv_fp8_blocks(x, ldx, sx, ldsx, x_fmt, w, ldw, sw, ldsw, w_fmt, M, N, K, y, y_type, ldy, st);
     int sms = 0;
     RENG_CUDA_TRY(current_sms(&sms));
     Fp8Gemm a{};
@@ -386,28 +930,30 @@ int gemm_fp8_blocks(const uint8_t* x, int64_t ldx, const float* sx, int64_t ldsx
     a.M = M;
     a.N = N;
     a.kb = (K + kBK - 1) / kBK;
-    a.mt = (M + kRows - 1) / kRows;
     a.mbox = std::min(kRows, (M + 7) / 8 * 8);
     a.y_f32 = y_type == RENG_TYPE_F32;
-    a.vec = ops_aligned(y, ldy * (a.y_f32 ? 4 : 2), 16);
+    a.y_vec = ops_aligned(y, ldy * (a.y_f32 ? 4 : 2), 32);
+    a.y_tma = ops_aligned(y, ldy * (a.y_f32 ? 4 : 2), 16);
+    a.sx_vec = ops_aligned(sx, ldsx * 4, 16);
     a.err = err;
+    const Plan p = plan(M, N, a.kb, sms);
+    a.bn = p.bn;
+    a.ks = p.ks;
+    const int rows = p.pair ? 2 * kRows : kRows;
+    a.mt = (M + rows - 1) / rows;
+    a.nt = (N + a.bn - 1) / a.bn;
+    a.group = std::min(a.mt, p.pair ? 8 : 16);
     // E4M3 is operand type 0, E5M2 1; f32 accumulation
-    const int BN = a.mt * ((N + 255) / 256) >= sms ? 256 : (a.mt * ((N + 127) / 128) >= sms ? 128 : 64);
     a.idesc = (1u << 4) | ((uint32_t)(x_fmt == RENG_FP8_E5M2) << 7) | ((uint32_t)(w_fmt == RENG_FP8_E5M2) << 10) |
-              ((uint32_t)(BN >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-    a.nt = (N + BN - 1) / BN;
-    a.ks = 1;
-    const long long tiles = (long long)a.mt * a.nt;
-    if (BN == 64)
-        while (a.ks < kMaxSplit && tiles * a.ks * 2 <= sms && a.ks * 2 <= a.kb) a.ks *= 2;
-    CUtensorMap xm, wm;
+              ((uint32_t)(rows >> 4) << 24);  // the kernel adds N
+    CUtensorMap xm, wm, ym{};
     int rc = codes_map(x, M, K, ldx, a.mbox, &xm);
-    if (!rc) rc = codes_map(w, N, K, ldw, BN, &wm);
+    if (!rc) rc = codes_map(w, N, K, ldw, p.pair ? a.bn / 4 : a.bn, &wm);
+    if (!rc && p.pair && a.y_tma) rc = y_map(y, a.y_f32, M, N, ldy, &ym);
     if (rc) return rc;
-    const int grid = a.ks > 1 ? (int)tiles * a.ks : (int)std::min<long long>(tiles, sms);
-    if (BN == 256) return launch_tile<256, 8, 2>(xm, wm, a, grid, st);
-    if (BN == 128) return launch_tile<128, 8, 4>(xm, wm, a, grid, st);
-    return launch_tile<64, 4, 2>(xm, wm, a, grid, st);
+    const long long tiles = (long long)a.mt * a.nt;
+    if (p.pair) return launch_tiles<true>(xm, wm, ym, a, 2 * (int)std::min<long long>(tiles, sms / 2), st);
+    return launch_tiles<false>(xm, wm, ym, a, a.ks > 1 ? (int)tiles * a.ks : (int)std::min<long long>(tiles, sms), st);
 }
 
 }  // namespace reng

@@ -7,6 +7,8 @@ namespace reng {
 
 inline int64_t ops_groups(int64_t cols) { return (cols + 127) / 128; }
 
+constexpr int64_t kOpsMaxCols = (int64_t)1 << 30;  // columns are counted in 32 bits
+
 // A row pitch that holds its row, in a matrix whose extent (and that of any
 // index formed from it) stays far inside 64 bits.
 inline bool ops_pitch_ok(int64_t rows, int64_t cols, int64_t ld) {

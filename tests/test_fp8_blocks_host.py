@@ -22,7 +22,7 @@ GOOD_Q = dict(x=4096, type=0, rows=4, cols=256, ldx=256, block_rows=1, fmt=0, co
 
 
 @pytest.mark.parametrize("change,word", [
-    (dict(rows=-1), "rows >= 0"), (dict(cols=0), "cols >= 1"), (dict(type=2), "element type"), (dict(fmt=2), "format"),
+    (dict(rows=-1), "rows >= 0"), (dict(cols=0), "cols in [1"), (dict(type=2), "element type"), (dict(fmt=2), "format"),
     (dict(block_rows=64), "block_rows"), (dict(ldx=255), "pitch"), (dict(ldc=255), "pitch"), (dict(lds=1), "pitch"),
     (dict(rows=1 << 41), "2^40"), (dict(ldx=1 << 41), "2^40"), (dict(rows=1 << 30, ldx=1 << 20), "2^40"),
     (dict(x=None), "NULL"), (dict(codes=None), "NULL"), (dict(scales=None), "NULL"), (dict(x=4097), "aligned"),
@@ -70,7 +70,7 @@ def desc(reng_lib, **change):
 
 
 @pytest.mark.parametrize("change,word", [
-    (dict(rows=-1), "rows >= 0"), (dict(cols=0), "cols >= 1"), (dict(residual_type=2), "element type"),
+    (dict(rows=-1), "rows >= 0"), (dict(cols=0), "cols in [1"), (dict(residual_type=2), "element type"),
     (dict(branch_type=-1), "element type"), (dict(gate=4096, ld_gate=256, gate_type=5), "element type"),
     (dict(out=5), "output kind"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"),
     (dict(scale=float("inf")), "scale"), (dict(branch=None, out=0), "nothing to do"),
