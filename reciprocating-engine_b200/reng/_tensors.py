@@ -62,18 +62,25 @@ def vector(t, name, n, dev):
 def codes_empty(rows, cols, like):
     """uint8 [rows, cols] in rows of 16-byte pitch (as the product reads them), and the pitch."""
     pitch = -(-cols // 16) * 16
-    t = torch.empty((rows, pitch), dtype=torch.uint8, device=like.device)
+    t = torch.empty(rows, pitch, dtype=torch.uint8, device=like.device)
     return (t if pitch == cols else t[:, :cols]), pitch
+
+
+try:  # the handle without building a Stream object around it
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+except ImportError:
+    def _raw_stream(dev):
+        return torch.cuda.current_stream(dev).cuda_stream
 
 
 def call(dev, name, *args):
     """The library call on the device's current stream, with the device current."""
     f = getattr(_lib.lib(), name)
     if dev == torch.cuda.current_device():
-        rc = f(*args, torch.cuda.current_stream(dev).cuda_stream)
+        rc = f(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
-            rc = f(*args, torch.cuda.current_stream(dev).cuda_stream)
+            rc = f(*args, _raw_stream(dev))
     if rc:
         _lib.check(rc)
 
@@ -96,7 +103,7 @@ def blocks_out(x, dev, rows, cols, scale_rows, codes, scales):
         ldc = matrix(codes, "codes", U8, dev, rows, cols)
     if scales is None:
         lds = groups(cols)
-        scales = torch.empty((scale_rows, lds), dtype=torch.float32, device=x.device)
+        scales = torch.empty(scale_rows, lds, dtype=torch.float32, device=x.device)
     else:
         lds = matrix(scales, "scales", F32, dev, scale_rows, groups(cols))
     return codes, ldc, scales, lds
@@ -142,7 +149,7 @@ def gemm_fp8_blocks(x, x_scales, w, w_scales, out, dtype, x_fmt, w_fmt):
     ldsx = matrix(x_scales, "x_scales", F32, dev, M, kb)
     ldsw = matrix(w_scales, "w_scales", F32, dev, groups(N), kb)
     if out is None:
-        out = torch.empty((M, N), dtype=dtype or torch.bfloat16, device=x.device)
+        out = torch.empty(M, N, dtype=dtype or torch.bfloat16, device=x.device)
         ldy = N
     else:
         if dtype is not None and out.dtype != dtype:

@@ -14,7 +14,7 @@ pass over the rows.
 operand of gemm.gemm_fp8_blocks.  Sums and norms are f32.  `out` may be
 `residual` itself (in place); without a branch y is `residual`, unwritten.
 """
-import ctypes as C
+import struct
 
 import torch
 
@@ -22,66 +22,66 @@ from . import _lib
 from ._tensors import TYPES, blocks_out, call, index, matrix, on_stream, vector
 
 _FP8_OUT = {_lib.RENG_FP8_E4M3: _lib.RENG_NORM_E4M3, _lib.RENG_FP8_E5M2: _lib.RENG_NORM_E5M2}
+# reng_block_norm_desc, field for field (packed at once: filling the ctypes
+# struct costs a call as much as its checks do)
+_DESC = struct.Struct("8P8q4i2f")
 
 
-def _desc(residual, branch, post_gain, gate, scale, pre_gain, eps, out):
+def _run(residual, branch, post_gain, gate, scale, pre_gain, eps, out, h_out, h, ld_h, scales, ld_scales):
+    """The checks of what is common and the call; returns y.  h, scales: tensors or None."""
     dev = index(residual)
-    d = _lib.BlockNormDesc()
-    d.ld_residual = matrix(residual, "residual", TYPES, dev)
+    ldr = matrix(residual, "residual", TYPES, dev)
     rows, cols = residual.shape
-    d.rows, d.cols = rows, cols
-    d.residual = residual.data_ptr()
-    d.residual_type = TYPES[residual.dtype]
-    d.scale, d.eps = scale, eps
-    d.post_gain = vector(post_gain, "post_gain", cols, dev)
-    d.pre_gain = vector(pre_gain, "pre_gain", cols, dev)
+    post, pre = vector(post_gain, "post_gain", cols, dev), vector(pre_gain, "pre_gain", cols, dev)
+    rtype = TYPES[residual.dtype]
+    pb = pg = py = ldb = ldg = ldy = tb = tg = 0
     if branch is None:
         if gate is not None or post_gain is not None or out is not None:
             raise ValueError("a gate, a post norm or an output residual without a branch")
-        return d, residual
-    d.ld_branch = matrix(branch, "branch", TYPES, dev, rows, cols)
-    d.branch = branch.data_ptr()
-    d.branch_type = TYPES[branch.dtype]
-    if gate is not None:
-        if gate.dim() == 1:
-            gate = gate.unsqueeze(0)
-            matrix(gate, "gate", TYPES, dev, 1, cols)
-            d.ld_gate = 0
-        else:
-            d.ld_gate = matrix(gate, "gate", TYPES, dev, rows, cols)
-        d.gate = gate.data_ptr()
-        d.gate_type = TYPES[gate.dtype]
-    if out is None:
-        out = torch.empty((rows, cols), dtype=residual.dtype, device=residual.device)
-        d.ld_y = cols
+        out = residual
     else:
-        d.ld_y = matrix(out, "out", (residual.dtype,), dev, rows, cols)
-    d.y = out.data_ptr()
-    return d, out
+        ldb = matrix(branch, "branch", TYPES, dev, rows, cols)
+        pb, tb = branch.data_ptr(), TYPES[branch.dtype]
+        if gate is not None:
+            if gate.dim() == 1:
+                matrix(gate.unsqueeze(0), "gate", TYPES, dev, 1, cols)
+            else:
+                ldg = matrix(gate, "gate", TYPES, dev, rows, cols)
+            pg, tg = gate.data_ptr(), TYPES[gate.dtype]
+        if out is None:
+            out = torch.empty(rows, cols, dtype=residual.dtype, device=residual.device)
+            ldy = cols
+        else:
+            ldy = matrix(out, "out", (residual.dtype,), dev, rows, cols)
+        py = out.data_ptr()
+    call(dev, "reng_block_norm", _DESC.pack(
+        pb, residual.data_ptr(), pg, post or 0, pre or 0, py, 0 if h is None else h.data_ptr(),
+        0 if scales is None else scales.data_ptr(), rows, cols, ldb, ldr, ldg, ldy, ld_h, ld_scales,
+        tb, rtype, tg, h_out, scale, eps))
+    return out
 
 
 def _norm(residual, branch, post_gain, gate, scale, pre_gain, eps, norm, out, h, dtype):
-    d, y = _desc(residual, branch, post_gain, gate, scale, pre_gain, eps, out)
-    dev = residual.get_device()
+    ldh, kind = 0, _lib.RENG_NORM_NONE
     if norm:
+        dev = index(residual)
         if h is None:
-            h = torch.empty((d.rows, d.cols), dtype=dtype, device=residual.device)
-        d.ld_h = matrix(h, "h", TYPES, dev, d.rows, d.cols)
-        d.h = h.data_ptr()
-        d.out = _lib.RENG_NORM_BF16 if h.dtype == torch.bfloat16 else _lib.RENG_NORM_F32
+            h = torch.empty(residual.shape, dtype=dtype, device=residual.device)
+        ldh = matrix(h, "h", TYPES, dev, *residual.shape)
+        kind = _lib.RENG_NORM_BF16 if h.dtype == torch.bfloat16 else _lib.RENG_NORM_F32
     elif h is not None or pre_gain is not None:
         raise ValueError("norm=False takes no h and no pre_gain")
-    call(dev, "reng_block_norm", C.byref(d))
+    y = _run(residual, branch, post_gain, gate, scale, pre_gain, eps, out, kind, h, ldh, None, 0)
     return y, h
 
 
 def _norm_fp8(residual, branch, post_gain, gate, scale, pre_gain, eps, fmt, out, codes, scales):
-    d, y = _desc(residual, branch, post_gain, gate, scale, pre_gain, eps, out)
-    dev = residual.get_device()
-    codes, d.ld_h, scales, d.ld_scales = blocks_out(residual, dev, d.rows, d.cols, d.rows, codes, scales)
-    d.h, d.h_scales = codes.data_ptr(), scales.data_ptr()
-    d.out = _FP8_OUT.get(fmt, -1)
-    call(dev, "reng_block_norm", C.byref(d))
+    dev = index(residual)
+    if residual.dim() != 2:
+        raise ValueError("residual has shape %s" % (tuple(residual.shape),))
+    rows, cols = residual.shape
+    codes, ldh, scales, lds = blocks_out(residual, dev, rows, cols, rows, codes, scales)
+    y = _run(residual, branch, post_gain, gate, scale, pre_gain, eps, out, _FP8_OUT.get(fmt, -1), codes, ldh, scales, lds)
     return y, codes, scales
 
 
