@@ -140,6 +140,12 @@ typedef struct reng_model reng_model;
 #define RENG_WEIGHTS_FP8_E4M3 1 /* projections quantized on the device at
                                    create time: E4M3, per-channel scales,
                                    backoff 1.0 (reng_fp8_quantize) */
+#define RENG_WEIGHTS_FP8_BLOCKS 2 /* projections quantized at create time in
+                                   128 x 128 blocks (reng_fp8_quantize_blocks)
+                                   and multiplied by 8-bit activations in
+                                   1 x 128 groups (reng_block_norm,
+                                   reng_fp8_swiglu_quantize,
+                                   reng_gemm_fp8_blocks); tp_world 1 only */
 
 typedef struct reng_model_desc {
     int32_t hidden;         /* hidden_size */

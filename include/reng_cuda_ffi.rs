@@ -8,6 +8,9 @@ pub const RENG_MEM_DEVICE: c_int = 0;
 pub const RENG_MEM_HOST: c_int = 1;
 pub const RENG_FP8_E4M3: c_int = 0;
 pub const RENG_FP8_E5M2: c_int = 1;
+pub const RENG_WEIGHTS_BF16: i32 = 0;
+pub const RENG_WEIGHTS_FP8_E4M3: i32 = 1;
+pub const RENG_WEIGHTS_FP8_BLOCKS: i32 = 2;
 pub const RENG_SCALING_PCS: c_int = 0;
 pub const RENG_SCALING_HW: c_int = 1;
 pub const RENG_SCALING_UNIT: c_int = 2;

@@ -128,6 +128,21 @@ struct QkNormArgs {
     float eps;
 };
 
+// Plain q/k/v rows [M][ld] (checkpoint order: q heads, k heads, v) to the q
+// buffer and the cache (rope_kv.cu).
+struct RopeKvArgs {
+    const uint16_t* qkv;
+    int ld;
+    const float* bias;       // [q_dim + 2 kv_dim] (q part pre-scaled) or null
+    float q_scale;           // the attention scale on q (1 when it rides elsewhere)
+    const float* rope_cos;   // [cap][hd]
+    const float* rope_sin;
+    const int* row_slot;
+    const int* row_pos;
+    uint16_t *q, *kcache, *vcache;
+    int nq, n_kv, hd, cap;
+};
+
 struct AttnArgs {
     const uint16_t* q;      // [M][q_dim]
     const uint16_t* kcache; // this layer [B][n_kv][cap][hd]
@@ -210,6 +225,7 @@ cudaError_t launch_attn(const AttnArgs& a, int chunk, bool pdl, cudaStream_t st)
 // rows x KV groups (RENG_ATTN_SLICES fixes them).
 int attn_slices(long long units);
 cudaError_t launch_embed(const EmbedArgs& a, bool pdl, cudaStream_t st);
+cudaError_t launch_rope_kv(const RopeKvArgs& a, int M, cudaStream_t st);
 cudaError_t launch_qk_norm(const QkNormArgs& a, bool pdl, cudaStream_t st);
 cudaError_t launch_pack(const PackArgs& a, cudaStream_t st);
 cudaError_t launch_pack8(const Pack8Args& a, cudaStream_t st);

@@ -12,6 +12,7 @@
 #include <vector>
 
 #include "gemm.cuh"
+#include "ops.cuh"
 
 using namespace reng;
 
@@ -31,7 +32,8 @@ struct LayerDev {
     float *g1 = nullptr, *g2 = nullptr, *bqkv = nullptr;
     float *qn = nullptr, *kn = nullptr;  // q/k norm gains [hd] (qk_norm; qn carries the attention scale)
     bool no_rope = false;                // NoPE layer: the q/k/v launch rotates with the identity table
-    // FP8 weights: per packed row scales (null for bf16)
+    // FP8 weights: per packed row scales, or per 128 x 128 block of the plain
+    // codes [rows][K] (null for bf16)
     float *sqkv = nullptr, *so = nullptr, *sgu = nullptr, *sd = nullptr;
 };
 
@@ -68,6 +70,12 @@ struct reng_model {
     int *row_slot = nullptr, *row_pos = nullptr, *pos = nullptr, *step = nullptr;
     int* err = nullptr;  // device error word of the bounded waits
     int w8 = 0;          // projections held as FP8-E4M3 codes + row scales
+    // projections held as plain FP8-E4M3 codes with 128 x 128 block scales, run
+    // on 8-bit activations (RENG_WEIGHTS_FP8_BLOCKS)
+    bool blocks = false;
+    uint8_t* codes = nullptr;   // the next product's x codes [kBlockRows][widest K]
+    float* cscale = nullptr;    // and their 1 x 128 scales
+    uint16_t *wide = nullptr, *branch = nullptr;  // q/k/v and gate/up rows; o and down rows
     uint32_t *ids_ring = nullptr, *prefill_ids = nullptr, *next_id = nullptr;
     unsigned int* am_count = nullptr;
     unsigned long long* am_key = nullptr;  // [kBlockRows] LM-head argmax keys
@@ -193,6 +201,17 @@ int pack_fp8(reng_model* m, uint8_t** out, float** out_scales, const uint16_t* s
     return RENG_OK;
 }
 
+// Quantize a staged bf16 matrix [rows][K] in 128 x 128 blocks (E4M3), in
+// place of packing it: the block-scaled product reads plain rows.
+int quantize_matrix(reng_model* m, uint8_t** out, float** out_scales, const uint16_t* staged, int rows, int K) {
+    const int64_t groups = ops_groups(K);
+    TRY(dalloc(m, out, (size_t)rows * K));
+    TRY(dalloc(m, out_scales, (size_t)ops_groups(rows) * groups));
+    TRY(reng_fp8_quantize_blocks(staged, RENG_TYPE_BF16, rows, K, K, 128, RENG_FP8_E4M3, *out, K, *out_scales, groups, m->st));
+    CU(cudaStreamSynchronize(m->st));  // the staging is reused
+    return RENG_OK;
+}
+
 std::vector<int> plain_map(int rows) {
     int tiles = (rows + kTileRows - 1) / kTileRows;
     std::vector<int> v((size_t)tiles * kTileRows, -1);
@@ -266,14 +285,17 @@ int validate(const reng_model_desc* d) {
                    "reng_model_create: head_dim must be a multiple of 16 and <= 128");
     RENG_CHECK_ARG(d->n_heads / d->n_kv_heads <= 8, "reng_model_create: more than 8 query heads per KV head");
     RENG_CHECK_ARG((d->inter / d->tp_world) % 8 == 0, "reng_model_create: intermediate per rank must be a multiple of 8");
-    RENG_CHECK_ARG(d->weights == RENG_WEIGHTS_BF16 || d->weights == RENG_WEIGHTS_FP8_E4M3,
+    RENG_CHECK_ARG(d->weights == RENG_WEIGHTS_BF16 || d->weights == RENG_WEIGHTS_FP8_E4M3 ||
+                       d->weights == RENG_WEIGHTS_FP8_BLOCKS,
                    "reng_model_create: unknown weight format");
+    if (d->weights == RENG_WEIGHTS_FP8_BLOCKS && d->tp_world > 1)
+        return fail(RENG_E_UNSUPPORTED, "reng_model_create: block-scaled FP8 weights do not shard (tp_world 1 only)");
     RENG_CHECK_ARG(std::isfinite(d->eps) && d->eps >= 0.f && std::isfinite(d->attn_scale),
                    "reng_model_create: eps / attn_scale not finite");
     RENG_CHECK_ARG(d->capacity <= (1 << 20), "reng_model_create: capacity above 1048576 positions");
     // the FP8 GEMV reads x 16 columns at a time: every K it sees (hidden,
     // q width, intermediate per rank) must be a multiple of 16
-    if (d->weights == RENG_WEIGHTS_FP8_E4M3 && (d->inter / d->tp_world) % 16 != 0)
+    if (d->weights != RENG_WEIGHTS_BF16 && (d->inter / d->tp_world) % 16 != 0)
         return fail(RENG_E_UNSUPPORTED, "reng_model_create: FP8 weights need the intermediate size per rank (" +
                                             std::to_string(d->inter / d->tp_world) + ") to be a multiple of 16");
     RENG_CHECK_ARG(d->qk_norm == 0 || d->qk_norm == 1, "reng_model_create: qk_norm must be 0 or 1");
@@ -433,8 +455,85 @@ GemvArgs qkv_args(reng_model* m, int l, int M) {
     return g;
 }
 
+// ---- the 8-bit path (RENG_WEIGHTS_FP8_BLOCKS): every projection is the
+// block-scaled product of codes that the step before it wrote ----
+
+// y[M][N] (bf16) = m->codes [M][K] times a layer's codes [N][K].
+int block_product(reng_model* m, const uint8_t* w, const float* sw, int M, int N, int K, uint16_t* y, cudaStream_t st) {
+    const int64_t groups = ops_groups(K);
+    TRY(gemm_fp8_blocks(m->codes, K, m->cscale, groups, RENG_FP8_E4M3, w, K, sw, groups, RENG_FP8_E4M3, M, N, K, y,
+                        RENG_TYPE_BF16, N, m->err, st));
+    m->launches++;
+    return RENG_OK;
+}
+
+// The residual stream takes the branch (null: none yet) and its norm with
+// `gain` goes to m->codes, or (codes false) to m->xn for the LM head.
+int block_step(reng_model* m, const uint16_t* branch, const float* gain, bool codes, int M, cudaStream_t st) {
+    reng_block_norm_desc d{};
+    d.branch = branch;
+    d.residual = d.y = m->x_res;
+    d.pre_gain = gain;
+    d.h = codes ? (void*)m->codes : (void*)m->xn;
+    d.h_scales = m->cscale;
+    d.rows = M;
+    d.cols = d.ld_branch = d.ld_residual = d.ld_y = d.ld_h = m->hidden;
+    d.ld_scales = ops_groups(m->hidden);
+    d.out = codes ? RENG_NORM_E4M3 : RENG_NORM_BF16;
+    d.scale = 1.0f;
+    d.eps = m->d.eps;
+    TRY(reng_block_norm(&d, st));
+    m->launches++;
+    return RENG_OK;
+}
+
+int block_qkv(reng_model* m, int l, int M, cudaStream_t st) {
+    const LayerDev& w = m->layers[l];
+    const int N = m->q_dim + 2 * m->kv_dim;
+    TRY(block_product(m, w.wqkv, w.sqkv, M, N, m->hidden, m->wide, st));
+    const bool id = m->qk_norm || w.no_rope;  // as qkv_args: raw q/k, rotated after the norm; NoPE: never
+    RopeKvArgs a{};
+    a.qkv = m->wide;
+    a.ld = N;
+    a.bias = w.bqkv;
+    a.q_scale = m->qk_norm ? 1.0f : m->d.attn_scale;
+    a.rope_cos = id ? m->rope_cos_id : m->rope_cos;
+    a.rope_sin = id ? m->rope_sin_id : m->rope_sin;
+    a.row_slot = m->row_slot;
+    a.row_pos = m->row_pos;
+    a.q = m->qbuf;
+    a.kcache = m->kcache + (size_t)l * m->layer_kv;
+    a.vcache = m->vcache + (size_t)l * m->layer_kv;
+    a.nq = m->nh;
+    a.n_kv = m->nkv;
+    a.hd = m->hd;
+    a.cap = m->cap;
+    CU(launch_rope_kv(a, M, st));
+    m->launches++;
+    return RENG_OK;
+}
+
+// o_proj (which 0) or down_proj (1) with the residual add and the norm that
+// follows: the MLP's, the next layer's, or the LM head's after the last.
+int block_proj(reng_model* m, int l, int M, int which, cudaStream_t st) {
+    const LayerDev& w = m->layers[l];
+    const int K = which == 0 ? m->q_dim : m->inter;
+    const int64_t groups = ops_groups(K);
+    if (which == 0)
+        TRY(reng_fp8_quantize_blocks(m->attn, RENG_TYPE_BF16, M, K, K, 1, RENG_FP8_E4M3, m->codes, K, m->cscale, groups, st));
+    else
+        TRY(reng_fp8_swiglu_quantize(m->wide, m->wide + K, RENG_TYPE_BF16, M, K, 2 * K, RENG_FP8_E4M3, m->codes, K,
+                                     m->cscale, groups, st));
+    m->launches++;
+    TRY(block_product(m, which == 0 ? w.wo : w.wd, which == 0 ? w.so : w.sd, M, m->hidden, K, m->branch, st));
+    if (which == 0) return block_step(m, m->branch, w.g2, true, M, st);
+    const bool last = l + 1 == m->L;
+    return block_step(m, m->branch, last ? m->final_gamma : m->layers[l + 1].g1, !last, M, st);
+}
+
 int k_qkv_launch(reng_model* m, int l, int M, cudaStream_t st) {
-    TRY(linear(m, qkv_args(m, l, M), EPI_QKV, 0, 0, st));
+    if (m->blocks) TRY(block_qkv(m, l, M, st));
+    else TRY(linear(m, qkv_args(m, l, M), EPI_QKV, 0, 0, st));
     if (m->qk_norm) {  // per-head RMSNorm of q and k, then RoPE (model.rs:2962-3010)
         QkNormArgs a{};
         a.q = m->qbuf;
@@ -528,6 +627,7 @@ GemvArgs proj_args(reng_model* m, int l, int M, int which) {
 }
 
 int k_proj_launch(reng_model* m, int l, int M, int which, cudaStream_t st) {
+    if (m->blocks) return block_proj(m, l, M, which, st);
     const GemvArgs o = proj_args(m, l, M, which);
     const int kind = which == 0 ? 1 : 3;
     if (m->world > 1) {
@@ -559,6 +659,8 @@ GemvArgs gateup_args(reng_model* m, int l, int M) {
 }
 
 int k_gateup_launch(reng_model* m, int l, int M, cudaStream_t st) {
+    if (m->blocks)  // SwiGLU is down_proj's quantizer
+        return block_product(m, m->layers[l].wgu, m->layers[l].sgu, M, 2 * m->inter, m->hidden, m->wide, st);
     return linear(m, gateup_args(m, l, M), EPI_SWIGLU, 2, 0, st);
 }
 
@@ -570,6 +672,10 @@ GemvArgs head_args(reng_model* m, int mode, int M, int slot, int r0, bool shard 
     GemvArgs h = norm_args(m, M, m->final_gamma);
     h.x = m->x_res + (size_t)r0 * m->hidden;
     h.ss_in = m->ss + (size_t)r0 * kSsStride;
+    if (m->blocks) {  // the last layer's step normalised the rows already
+        h.x = m->xn + (size_t)r0 * m->hidden;
+        h.ss_in = nullptr;
+    }
     h.w = m->lm;
     h.tiles = m->lm_tiles;
     if (shard) {
@@ -613,6 +719,7 @@ enum { HEAD_NONE = 0, HEAD_LAST = 1, HEAD_ALL = 2, HEAD_SHARD = 3 };
 int enqueue_step(reng_model* m, int mode, int M, int slot, int head, cudaStream_t st, int* nk) {
     const int before = m->launches;
     TRY(k_embed_launch(m, mode, M, slot, st));
+    if (m->blocks) TRY(block_step(m, nullptr, m->layers[0].g1, true, M, st));
     for (int l = 0; l < m->L; l++) {
         TRY(k_qkv_launch(m, l, M, st));
         TRY(k_attn_launch(m, l, M, mode, st));
@@ -680,6 +787,7 @@ int create(const reng_model_desc* d, const reng_layer_weights* layers, const uin
     m->rank = d->tp_rank;
     m->world = d->tp_world;
     m->w8 = d->weights == RENG_WEIGHTS_FP8_E4M3 ? 1 : 0;
+    m->blocks = d->weights == RENG_WEIGHTS_FP8_BLOCKS;
     m->qk_norm = d->qk_norm == 1;
     // the attention scale rides on wq (and bq), or on the q norm gain
     // (scaled_wq, model.rs:148-157)
@@ -753,27 +861,35 @@ int create(const reng_model_desc* d, const reng_layer_weights* layers, const uin
         TRY(copy_matrix(stage + (size_t)m->q_dim * H, s.wk + (size_t)R * m->kv_dim * H, m->kv_dim, H, H, mem, m->st));
         TRY(copy_matrix(stage + (size_t)(m->q_dim + m->kv_dim) * H, s.wv + (size_t)R * m->kv_dim * H, m->kv_dim, H, H,
                         mem, m->st));
-        if (m->w8)
+        if (m->blocks)  // the attention scale is applied to q in f32 (rope_kv.cu)
+            TRY(quantize_matrix(m, &w.wqkv, &w.sqkv, stage, m->q_dim + 2 * m->kv_dim, H));
+        else if (m->w8)
             TRY(pack_fp8(m, &w.wqkv, &w.sqkv, stage, m->q_dim + 2 * m->kv_dim, qkv_map, H, wq_scale, m->q_dim,
                          &m->qkv_tiles));
         else
             TRY(pack(m, &w.wqkv, stage, qkv_map, H, wq_scale, m->q_dim, &m->qkv_tiles));
         // o_proj column window
         TRY(copy_matrix(stage, s.wo + (size_t)R * m->q_dim, H, m->q_dim, q_full, mem, m->st));
-        if (m->w8)
+        if (m->blocks)
+            TRY(quantize_matrix(m, &w.wo, &w.so, stage, H, m->q_dim));
+        else if (m->w8)
             TRY(pack_fp8(m, &w.wo, &w.so, stage, H, plain_map(H), m->q_dim, 1.f, 0, &m->o_tiles));
         else
             TRY(pack(m, &w.wo, stage, plain_map(H), m->q_dim, 0.f, 0, &m->o_tiles));
         // gate, up row blocks
         TRY(copy_matrix(stage, s.wg + (size_t)R * m->inter * H, m->inter, H, H, mem, m->st));
         TRY(copy_matrix(stage + (size_t)m->inter * H, s.wu + (size_t)R * m->inter * H, m->inter, H, H, mem, m->st));
-        if (m->w8)
+        if (m->blocks)
+            TRY(quantize_matrix(m, &w.wgu, &w.sgu, stage, 2 * m->inter, H));
+        else if (m->w8)
             TRY(pack_fp8(m, &w.wgu, &w.sgu, stage, 2 * m->inter, gu_map, H, 1.f, 0, &m->gu_tiles));
         else
             TRY(pack(m, &w.wgu, stage, gu_map, H, 0.f, 0, &m->gu_tiles));
         // down column window
         TRY(copy_matrix(stage, s.wd + (size_t)R * m->inter, H, m->inter, d->inter, mem, m->st));
-        if (m->w8)
+        if (m->blocks)
+            TRY(quantize_matrix(m, &w.wd, &w.sd, stage, H, m->inter));
+        else if (m->w8)
             TRY(pack_fp8(m, &w.wd, &w.sd, stage, H, plain_map(H), m->inter, 1.f, 0, &m->d_tiles));
         else
             TRY(pack(m, &w.wd, stage, plain_map(H), m->inter, 0.f, 0, &m->d_tiles));
@@ -836,7 +952,15 @@ int create(const reng_model_desc* d, const reng_layer_weights* layers, const uin
     TRY(dalloc(m, &m->qbuf, (size_t)MR * m->q_dim));
     TRY(dalloc(m, &m->xn, (size_t)MR * H));
     TRY(dalloc(m, &m->attn, (size_t)MR * m->q_dim));
-    TRY(dalloc(m, &m->act, (size_t)MR * m->inter));
+    if (m->blocks) {
+        const int widest = std::max({H, m->q_dim, m->inter});
+        TRY(dalloc(m, &m->codes, (size_t)MR * widest));
+        TRY(dalloc(m, &m->cscale, (size_t)MR * ops_groups(widest)));
+        TRY(dalloc(m, &m->wide, (size_t)MR * std::max(m->q_dim + 2 * m->kv_dim, 2 * m->inter)));
+        TRY(dalloc(m, &m->branch, (size_t)MR * H));
+    } else {
+        TRY(dalloc(m, &m->act, (size_t)MR * m->inter));
+    }
     TRY(dalloc(m, &m->logits, (size_t)MR * m->vocab));
     TRY(dalloc(m, &m->ss, (size_t)kSsStride * MR));
     TRY(dalloc(m, &m->part, (size_t)MR * H));
@@ -1139,6 +1263,7 @@ extern "C" int reng_model_time_kernels_rows(reng_model* m, int rows, int iters, 
     // its current position
     if (rows > 0) TRY(sync_pos(m));
     TRY(k_embed_launch(m, mode, M, 0, m->st));
+    if (m->blocks) TRY(block_step(m, nullptr, m->layers[0].g1, true, M, m->st));
     for (int kind = 0; kind < RENG_KERNEL_KINDS; kind++) {
         // one untimed pass, then `iters` launches cycling over the layers
         for (int pass = 0; pass < 2; pass++) {

@@ -62,4 +62,11 @@ cudaError_t launch_ops(void (*k)(P...), dim3 grid, dim3 block, size_t smem, cuda
     return cudaLaunchKernelEx(&cfg, k, args...);
 }
 
+// The block-scaled product (gemm_fp8.cu) behind reng_gemm_fp8_blocks: checked
+// arguments, and the device word a wait that ran out is recorded in (null: the
+// entry point's own).
+int gemm_fp8_blocks(const uint8_t* x, int64_t ldx, const float* sx, int64_t ldsx, int x_fmt, const uint8_t* w,
+                    int64_t ldw, const float* sw, int64_t ldsw, int w_fmt, int M, int N, int K, void* y, int y_type,
+                    int64_t ldy, int* err, cudaStream_t st);
+
 }  // namespace reng

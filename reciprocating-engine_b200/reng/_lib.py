@@ -37,6 +37,7 @@ RENG_NORM_E5M2 = 4
 
 RENG_WEIGHTS_BF16 = 0
 RENG_WEIGHTS_FP8_E4M3 = 1
+RENG_WEIGHTS_FP8_BLOCKS = 2
 
 
 class RengError(RuntimeError):

@@ -24,8 +24,9 @@ no one-recipe prefill to fall back from, so `--cached` is accepted and
 changes nothing); `--decode-rows` is accepted for compatibility (decode
 always runs one row per slot); `--batch` is accepted by generate and prefill
 as well (every slot takes the prompt, as reng-tp's `--batch`); FP8 weights
-are E4M3 with per-channel scales (the engine's device format: another
-`RENG_FP8` format is refused, never run as something else), and reng-tp
+are E4M3 with per-channel scales or, with `RENG_FP8=blocks`, with 128 x 128
+block scales and 8-bit activations (another `RENG_FP8` format is refused,
+never run as something else), and reng-tp
 accepts `--fp8` because each rank quantizes its own shard on its device.
 reng-tp's `--ifname` / `--no-numa` (HCCL sideband interface, NUMA binding)
 have no counterpart: NCCL picks its transport itself.  Errors print one
@@ -116,9 +117,9 @@ def parse_fp8(args, env=FROM_ENV):
         sw = fp8_switch(env, flag)
     except ValueError as e:
         raise UsageError(str(e))
-    if sw is not None and (sw != ("e4m3", "pcs") or sw.backoff != 1.0):
+    if sw is not None and (sw not in (("e4m3", "pcs"), ("e4m3", "blocks")) or sw.backoff != 1.0):
         raise UsageError("RENG_FP8 %s: this engine's FP8 weights are e4m3 with per-channel "
-                         "scales (pcs) and backoff 1" % (sw,))
+                         "scales (pcs) or block scales (blocks) and backoff 1" % (sw,))
     return rest, sw
 
 
@@ -172,10 +173,19 @@ def load_model(model_dir):
     return cfg, w, time.perf_counter() - t0
 
 
+def plan_weights(fp8):
+    """CachePlan's name for an engine's weights (fp8: a RENG_FP8 spec or None)."""
+    if not fp8:
+        return "bf16"
+    return "fp8_blocks" if fp8[1] == "blocks" else "fp8"
+
+
 def fp8_report_line(cfg, w, fp8):
     """The reference prints its quantization report when FP8 is on
     (generate.rs:207-212); the engine itself quantizes on the device at
     create time with the same rules."""
+    if fp8[1] == "blocks":  # no per-channel report: the scales follow each block's largest value
+        return "fp8 e4m3:blocks: weights in 128 x 128 blocks, activations in 1 x 128 groups"
     from . import fp8 as f
     _, rep = f.quantize_model(w, cfg)
     return "fp8 %s:%s: %s" % (fp8[0], fp8[1], rep)
@@ -328,7 +338,7 @@ def generate_main(argv=None):
     if a["fp8"]:
         print(fp8_report_line(cfg, w, a["fp8"]))
     print("loaded weights in %.2fs" % load_s)
-    plan = CachePlan.new(cfg, batch=a["batch"], weights="fp8" if a["fp8"] else "bf16")
+    plan = CachePlan.new(cfg, batch=a["batch"], weights=plan_weights(a["fp8"]))
     cap = a["capacity"]
     if a["recompute"]:
         cap = max(cap, len(a["ids"]) + n_new)
@@ -419,7 +429,7 @@ def prefill_main(argv=None):
     if msg:
         print(msg, file=sys.stderr)
         print(msg)
-    plan = CachePlan.new(cfg, batch=a["batch"], weights="fp8" if a["fp8"] else "bf16")
+    plan = CachePlan.new(cfg, batch=a["batch"], weights=plan_weights(a["fp8"]))
     print(plan.summary(tokens))
     plan.check(tokens)
     host = 4.0 * cfg.vocab_size * tokens
@@ -496,6 +506,8 @@ def parse_fp8_quantize(argv, env=FROM_ENV):
             i += 2
         else:
             raise UsageError("unknown flag %s\n%s" % (argv[i], FP8Q_USAGE))
+    if a["fp8"][1] == "blocks":
+        raise UsageError("reng-fp8-quantize reports the per-channel schemes (pcs, hw, unit), not blocks")
     return a
 
 
@@ -603,7 +615,7 @@ def bench_main(argv=None):
         print(fp8_report_line(cfg, w, a["fp8"]))
     print("loaded weights in %.2fs" % load_s)
     B = max(a["batch"], 1)
-    plan = CachePlan.new(cfg, batch=B, weights="fp8" if a["fp8"] else "bf16")
+    plan = CachePlan.new(cfg, batch=B, weights=plan_weights(a["fp8"]))
     print(plan.summary(a["capacity"]))
     msg = cfg.context_warning(a["prompt"] + a["new"])
     if msg:
@@ -682,6 +694,8 @@ def parse_tp(argv, env=FROM_ENV):
     """tp.rs:124-240: positional model dir, n_new and ids mixed with flags;
     worker-only flags --rank / --world / --module / --dir."""
     args, fp8 = parse_fp8(list(argv), env)
+    if fp8 and fp8[1] == "blocks":
+        raise UsageError("RENG_FP8=blocks: block-scaled weights do not shard (reng-tp takes pcs)")
     o = {"fp8": fp8, "modules": [], "prompt_file": None, "ref": None, "margin": DEFAULT_MARGIN,
          "rows": DEFAULT_ROWS, "capacity": DEFAULT_CAPACITY, "batch": 1, "bench": 0, "out": None,
          "timeout": DEFAULT_TIMEOUT_S, "rank": None, "world": 0, "module": 0, "hand_dir": None}

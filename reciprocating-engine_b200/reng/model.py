@@ -57,7 +57,9 @@ def fp8_switch(value, flag=False):
     yes mean the defaults; anything else is a list of settings separated by
     ':' or ',', each a format (e4m3, e5m2), a scale scheme (pcs, hw, unit)
     or backoff=<f32> in (0, 1].  A word that is none of these raises
-    ValueError, so a typo never runs as bf16."""
+    ValueError, so a typo never runs as bf16.  Beyond the reference, the
+    scheme `blocks` asks for block-scaled weights and 8-bit activations
+    (E4M3, backoff 1 only)."""
     import re
     from .fp8 import Fp8Format, Scaling
     if value is None:
@@ -76,6 +78,8 @@ def fp8_switch(value, flag=False):
             fmt = Fp8Format.from_name(word).short_name
         elif Scaling.from_name(word) is not None:
             sch = Scaling.from_name(word).short_name
+        elif word == "blocks":
+            sch = "blocks"
         elif word.startswith("backoff="):
             try:
                 backoff = float(np.float32(word[len("backoff="):]))
@@ -86,6 +90,8 @@ def fp8_switch(value, flag=False):
         else:
             raise ValueError("RENG_FP8: %r is neither a format (e4m3, e5m2), a scale scheme "
                              "(pcs, hw, unit) nor backoff=<f32>" % word)
+    if sch == "blocks" and (fmt != "e4m3" or backoff != 1.0):
+        raise ValueError("RENG_FP8: blocks are E4M3 with backoff 1")
     return Fp8Config(fmt, sch, backoff)
 
 
@@ -166,7 +172,10 @@ class Engine:
         desc.attn_scale = cfg.attention_scale()
         desc.has_qkv_bias = 1 if with_bias else 0
         desc.qk_norm = 1 if qk else 0
-        desc.weights = _lib.RENG_WEIGHTS_BF16 if fp8 is None else _lib.RENG_WEIGHTS_FP8_E4M3
+        if fp8 is None:
+            desc.weights = _lib.RENG_WEIGHTS_BF16
+        else:  # (format, scheme): per-channel weight-only, or blocks with 8-bit activations
+            desc.weights = _lib.RENG_WEIGHTS_FP8_BLOCKS if fp8[1] == "blocks" else _lib.RENG_WEIGHTS_FP8_E4M3
         desc.batch = batch
         desc.capacity = capacity
         desc.tp_rank = tp_rank

@@ -29,6 +29,7 @@ class CachePlan:
     batch: int
     weight_bytes: int
     q_dim: int = 0       # query width (heads x head_dim); 0: the hidden size
+    eight_bit: bool = False  # 8-bit activations (fp8_blocks): their work buffers
     device_bytes: int = 183_359 * 1024 * 1024  # B200 HBM (nvidia-smi total)
     reserve_bytes: int = 2 << 30               # context, graphs, work buffers, allocator slack
 
@@ -40,13 +41,19 @@ class CachePlan:
         inter = cfg.intermediate_size // world
         per_layer = h * qd * 2 + 2 * h * nkv * hd + 3 * h * inter
         rows = qd + 2 * nkv * hd + h + 2 * inter + h
-        if weights == "fp8":
+        if weights == "fp8_blocks":  # plain codes + one f32 scale per 128 x 128 block (rounded up per matrix)
+            def block(r, c):
+                return r * c + 4 * (-(-r // 128)) * (-(-c // 128))
+            body = cfg.num_hidden_layers * (block(qd + 2 * nkv * hd, h) + block(h, qd) + block(2 * inter, h) +
+                                            block(h, inter))
+        elif weights == "fp8":
             body = cfg.num_hidden_layers * (per_layer + 4 * rows)
         else:
             body = cfg.num_hidden_layers * per_layer * 2
         emb = cfg.vocab_size * h * 2
         wbytes = body + 2 * emb  # LM head (packed) + embedding table, bf16
         p = CachePlan(cfg.num_hidden_layers, nkv, hd, h, inter, cfg.vocab_size, batch, wbytes, q_dim=qd)
+        p.eight_bit = weights == "fp8_blocks"
         if device_bytes is not None:
             p.device_bytes = device_bytes
         return p
@@ -69,6 +76,10 @@ class CachePlan:
         qd = self.q_dim or self.hidden
         per_row = (2 * self.hidden * 2 + 2 * qd * 2 + self.inter * 2 + self.vocab * 2 + self.hidden * 4
                    + SS_STRIDE * 4 + 3 * 4 + 8)
+        if self.eight_bit:  # codes, their scales, the wide and branch rows, instead of the activation
+            k = max(self.hidden, qd, self.inter)
+            wide = max(qd + 2 * self.n_kv_heads * self.head_dim, 2 * self.inter)
+            per_row += k + 4 * (-(-k // 128)) + 2 * wide + 2 * self.hidden - 2 * self.inter
         return BLOCK_ROWS * per_row + GEMM_PARTS * 4 + (capacity + 1) * self.batch * 4 + (1 << 20)
 
     def total_bytes_at(self, capacity):

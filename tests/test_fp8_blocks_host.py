@@ -118,3 +118,60 @@ def test_block_norm_desc_layout(reng_lib):
     rs = re.search(r"pub struct reng_block_norm_desc \{(.*?)\n\}", rs, re.S).group(1)
     assert re.findall(r"pub (\w+):", rs) == names
     assert C.sizeof(reng_lib.BlockNormDesc) == 8 * 8 + 8 * 8 + 6 * 4
+
+
+# ---- the engine's block-scaled weights ----
+
+def test_the_switch_knows_blocks():
+    from reng.model import fp8_switch
+    assert fp8_switch("blocks") == ("e4m3", "blocks") and fp8_switch("e4m3:blocks", True).backoff == 1.0
+    for v in ("e5m2:blocks", "blocks,backoff=0.5", "block"):
+        with pytest.raises(ValueError):
+            fp8_switch(v)
+
+
+def test_the_quantize_tool_refuses_blocks():
+    from reng.cli import UsageError, fp8_report_line, parse_fp8_quantize, plan_weights
+    for argv, env in ((["m", "--fp8", "blocks"], None), (["m"], "blocks")):
+        with pytest.raises(UsageError, match="blocks"):
+            parse_fp8_quantize(argv, env=env)
+    assert "128 x 128" in fp8_report_line(None, None, ("e4m3", "blocks"))
+    assert [plan_weights(f) for f in (None, ("e4m3", "pcs"), ("e4m3", "blocks"))] == ["bf16", "fp8", "fp8_blocks"]
+
+
+def test_the_commands_take_blocks():
+    from reng import cli
+    argv = ["m", "o", "2", "--fp8", "7"]
+    assert cli.parse_generate(argv, env="blocks")["fp8"] == ("e4m3", "blocks")
+    assert cli.parse_generate(["m", "o", "2", "7"], env="e4m3,blocks")["fp8"] == ("e4m3", "blocks")
+    with pytest.raises(cli.UsageError, match="do not shard"):
+        cli.parse_tp(["m", "8", "1", "--modules", "0,1"], env="blocks")
+
+
+def test_the_plan_counts_block_scales():
+    from reng.config import LlamaConfig
+    from reng.plan import CachePlan
+    cfg = LlamaConfig(hidden_size=256, intermediate_size=400, num_hidden_layers=2, num_attention_heads=4,
+                      num_key_value_heads=2, head_dim_=64, vocab_size=1024)
+    p = CachePlan.new(cfg, weights="fp8_blocks")
+    codes = 2 * (512 * 256 + 256 * 256 + 800 * 256 + 256 * 400)
+    scales = 2 * (4 * 2 + 2 * 2 + 7 * 2 + 2 * 4)
+    assert p.weight_bytes == codes + 4 * scales + 2 * 1024 * 256 * 2
+    q = CachePlan.new(cfg, weights="fp8")
+    rows = (p.transient_bytes_at(64) - q.transient_bytes_at(64)) / (400 + 4 * 4 + 2 * 800 + 2 * 256 - 2 * 400)
+    assert rows == int(rows) and rows >= 256
+
+
+def test_blocks_do_not_shard(reng_lib):
+    import ctypes as C
+    from reng import _lib
+    d = _lib.ModelDesc(hidden=256, inter=512, n_layers=1, n_heads=4, n_kv_heads=2, head_dim=64, vocab=256, eps=1e-5,
+                       attn_scale=0.125, weights=_lib.RENG_WEIGHTS_FP8_BLOCKS, batch=1, capacity=64, tp_world=2)
+    out, layer, one = C.c_void_p(), _lib.LayerWeights(), C.c_void_p(16)
+    with pytest.raises(Exception, match="do not shard"):
+        _lib.call("reng_model_create", C.byref(d), C.byref(layer), one, one, one, one, one, _lib.RENG_MEM_HOST,
+                  C.byref(out))
+    d.weights, d.tp_world = 3, 1
+    with pytest.raises(Exception, match="unknown weight format"):
+        _lib.call("reng_model_create", C.byref(d), C.byref(layer), one, one, one, one, one, _lib.RENG_MEM_HOST,
+                  C.byref(out))
