@@ -12,6 +12,7 @@
 // once, from f32.  Replaces, for an 8-bit path, the reference's residual add
 // and RMSNorm nodes (crates/reng-synapse/src/model.rs:738-742).
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <string>
 #include <type_traits>
@@ -36,6 +37,14 @@ struct NormArgs {
     float scale, eps, inv_n;
 };
 
+// k_block_norm's teams and their shared memory: kSlots slots a team, each one
+// row's streams.  Offsets in bytes.
+constexpr int kSlots = 2;
+struct Plan {
+    int nw, teams;             // warps of a team, teams of a CTA
+    int residual, gate, slot;  // in a slot (the branch's image at 0), and its size
+};
+
 template <int TYPE>
 constexpr int kBytes = TYPE == RENG_TYPE_BF16 ? 2 : 4;
 
@@ -43,6 +52,8 @@ template <int TYPE, typename P>
 __device__ __forceinline__ P* row_at(P* base, int64_t elems) {
     return reinterpret_cast<P*>((uintptr_t)base + elems * kBytes<TYPE>);
 }
+
+constexpr int kMaxWarps = 24;  // of a CTA (named barriers: 15 teams of more than one warp)
 
 // The warps that share a row: a CTA holds blockDim / (32 nw) such teams, each
 // on a row of its own.
@@ -54,16 +65,20 @@ struct Team {
         id = w / nw;
         warp = w - id * nw;
     }
+    __device__ __forceinline__ void wait() const {
+        if (nw == 1) __syncwarp();
+        else asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(32 * nw) : "memory");
+    }
     // Sum over the team, the same bits on every thread (warps added in order).
     // `red` alternates between two rows, so one barrier is enough: a row is
     // written again only after the barrier of the other's sum.
-    __device__ __forceinline__ float sum(float v, float (&red)[2][16]) {
+    __device__ __forceinline__ float sum(float v, float (&red)[2][kMaxWarps]) {
         v = warp_sum(v);
         if (nw == 1) return v;
         float* r = red[turn] + id * nw;
         turn ^= 1;
         if ((threadIdx.x & 31) == 0) r[warp] = v;
-        asm volatile("bar.sync %0, %1;" ::"r"(id + 1), "r"(32 * nw) : "memory");
+        wait();
         float s = 0.f;
         for (int w = 0; w < nw; w++) s += r[w];
         return s;
@@ -90,12 +105,19 @@ struct Tile {
 
 template <bool KEEP, int TYPE, int G>
 __device__ __forceinline__ void tile_load(const void* row, const Tile<G>& t, int cols, Raw16<TYPE, G>& r) {
-    raw_zero(r);
+    if constexpr (G < 4) {
+        raw_zero(r);
 #pragma unroll
-    for (int g = 0; g < G; g++) {
-        if (!t.live[g]) continue;
-        if constexpr (G < 4) raw_load<TYPE, KEEP>(static_cast<const char*>(row) + (uint32_t)(t.c[g] * kBytes<TYPE>), g, r);
-        else raw_load<TYPE, KEEP>(row, t.c[g], cols, g, r);
+        for (int g = 0; g < G; g++)
+            if (t.live[g]) raw_load<TYPE, KEEP>(static_cast<const char*>(row) + (uint32_t)(t.c[g] * kBytes<TYPE>), g, r);
+    } else if (t.c[3] + kFp8Group <= cols) {
+#pragma unroll
+        for (int g = 0; g < 4; g++) raw_load<TYPE, KEEP, true>(row, t.c[g], cols, g, r);
+    } else {
+        raw_zero(r);
+#pragma unroll
+        for (int g = 0; g < 4; g++)
+            if (t.live[g]) raw_load<TYPE, KEEP>(row, t.c[g], cols, g, r);
     }
 }
 
@@ -109,6 +131,25 @@ __device__ __forceinline__ void tile_mul(const void* row, const Tile<G>& t, int 
 #pragma unroll
     for (int i = 0; i < 8; i++) v[i] = mul_f2(v[i], w[i]);
 }
+template <int G>
+__device__ __forceinline__ void tile_gate(const NormArgs& a, const void* row, const Tile<G>& t, f2 (&v)[8]) {
+    if (a.tg == RENG_TYPE_BF16) tile_mul<RENG_TYPE_BF16>(row, t, a.cols, v);
+    else tile_mul<RENG_TYPE_F32>(row, t, a.cols, v);
+}
+
+// The vectors that every row takes, at a tile: f = post_gain * gate (where
+// the gate is one row, 1 where there is neither) and pre_gain (or 1).
+template <int G>
+struct Vectors {
+    f2 f[8], pre[8];
+    __device__ __forceinline__ Vectors(const NormArgs& a, const Tile<G>& t) {
+#pragma unroll
+        for (int i = 0; i < 8; i++) f[i] = pre[i] = make_f2(1.f);
+        if (a.post) tile_mul<RENG_TYPE_F32>(a.post, t, a.cols, f);
+        if (a.pre) tile_mul<RENG_TYPE_F32>(a.pre, t, a.cols, pre);
+        if (a.gate && !a.ldg) tile_gate(a, a.gate, t, f);
+    }
+};
 
 // y's raw form from its values, rounded to TYPE.
 template <int TYPE, int G>
@@ -142,37 +183,35 @@ __device__ __forceinline__ void tile_store(void* row, const Tile<G>& t, int cols
             }
         }
     } else {
-        const int lane = threadIdx.x & 31;
+        using E = std::conditional_t<TYPE == RENG_TYPE_BF16, uint16_t, uint32_t>;
 #pragma unroll
-        for (int e = 0; e < 16; e++) {
-            const int c = t.c[e >> 2] + 32 * (e & 3) + lane;
-            if (c < cols) {
-                if (TYPE == RENG_TYPE_BF16) static_cast<uint16_t*>(row)[c] = (uint16_t)r.w[e];
-                else static_cast<uint32_t*>(row)[c] = r.w[e];
+        for (int g = 0; g < 4; g++) {
+            const int c = t.c[g] + (threadIdx.x & 31);
+            E* p = static_cast<E*>(row) + c;
+            if (t.c[g] + kFp8Group <= cols) {
+#pragma unroll
+                for (int i = 0; i < 4; i++) p[32 * i] = (E)r.w[4 * g + i];
+            } else {
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    if (c + 32 * i < cols) p[32 * i] = (E)r.w[4 * g + i];
             }
         }
     }
 }
 
-// y of a tile, rounded, from the branch u and the residual y: norm, gain and
-// gate of the branch, then y + scale u.
+// y of a tile, rounded, from the branch u and the residual y:
+// y + (r(u) scale) (u f gate), the gate's row of this row or null.
 template <int TB, int TR, int G>
-__device__ __forceinline__ void tile_residual(const NormArgs& a, int64_t row, const Tile<G>& t, float inv,
-                                              const Raw16<TB, G>& u, Raw16<TR, G>& y) {
+__device__ __forceinline__ void tile_residual(const NormArgs& a, const Vectors<G>& x, const void* gate,
+                                              const Tile<G>& t, float inv, const Raw16<TB, G>& u, Raw16<TR, G>& y) {
     f2 v[8], w[8];
     raw_floats(u, v);
-    if (a.post) {
-        const f2 n = make_f2(inv);
 #pragma unroll
-        for (int i = 0; i < 8; i++) v[i] = mul_f2(v[i], n);
-        tile_mul<RENG_TYPE_F32>(a.post, t, a.cols, v);
-    }
-    if (a.gate) {
-        if (a.tg == RENG_TYPE_BF16) tile_mul<RENG_TYPE_BF16>(row_at<RENG_TYPE_BF16>(a.gate, row * a.ldg), t, a.cols, v);
-        else tile_mul<RENG_TYPE_F32>(row_at<RENG_TYPE_F32>(a.gate, row * a.ldg), t, a.cols, v);
-    }
+    for (int i = 0; i < 8; i++) v[i] = mul_f2(v[i], x.f[i]);
+    if (gate) tile_gate(a, gate, t, v);
     raw_floats(y, w);
-    const f2 s = make_f2(a.scale);
+    const f2 s = make_f2(inv * a.scale);
 #pragma unroll
     for (int i = 0; i < 8; i++) w[i] = fma_f2(s, v[i], w[i]);
     raw_round(w, y);
@@ -199,14 +238,13 @@ __device__ __forceinline__ void tile_emit_fp8(const NormArgs& a, int64_t row, co
 
 // h of a tile (whole warps: the FP8 groups shuffle).
 template <int TR, int G>
-__device__ __forceinline__ void tile_emit(const NormArgs& a, int64_t row, const Tile<G>& t, float inv,
-                                          const Raw16<TR, G>& y) {
+__device__ __forceinline__ void tile_emit(const NormArgs& a, const Vectors<G>& x, int64_t row, const Tile<G>& t,
+                                          float inv, const Raw16<TR, G>& y) {
     f2 h[8];
     raw_floats(y, h);
     const f2 n = make_f2(inv);
 #pragma unroll
-    for (int i = 0; i < 8; i++) h[i] = mul_f2(h[i], n);
-    if (a.pre) tile_mul<RENG_TYPE_F32>(a.pre, t, a.cols, h);
+    for (int i = 0; i < 8; i++) h[i] = mul_f2(mul_f2(h[i], n), x.pre[i]);
     if (a.out == OUT_E4M3) {
         tile_emit_fp8<RENG_FP8_E4M3, G>(a, row, t, h);
     } else if (a.out == OUT_E5M2) {
@@ -235,82 +273,122 @@ __device__ __forceinline__ float f2_sum(f2 s) {
     split_f2(s, lo, hi);
     return lo + hi;
 }
-// Raw words stay raw between the passes over them: as floats they would take
-// twice the registers, which here are loads in flight.
-template <int TYPE, int G>
-__device__ __forceinline__ void keep_raw(Raw16<TYPE, G>& r) {
-#pragma unroll
-    for (int i = 0; i < Raw16<TYPE, G>::N; i++) asm volatile("" : "+r"(r.w[i]));
+
+__device__ __forceinline__ void copy16(void* dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
+                 : "memory");
+}
+__device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void copy_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// A team per row, the row in registers: C warp tiles per warp.  The next
-// row's residual and branch are loaded before this row's two sums are formed,
-// so the memory is busy while the team waits for itself.
-template <int TB, int TR, int G, int C>
-__global__ void __launch_bounds__(C == 1 ? 256 : 512, C == 1 ? 3 : 1) k_block_norm(const NormArgs a, int nw) {
-    __shared__ float red[2][16];
-    Team team(nw);
-    const int teams = blockDim.x / (32 * nw);
-    const int64_t step = (int64_t)gridDim.x * teams;
-    int64_t row = (int64_t)blockIdx.x * teams + team.id;
-    pdl_wait();
-    pdl_launch();
-    Raw16<TR, G> r[C];
-    Raw16<TB, G> b[C];
-    auto load = [&](int64_t at) {
+// Bytes between a row's 16-byte boundary and its first element: its image in
+// shared memory keeps them, so that both sides of a copy are aligned whatever
+// the row's own alignment.
+__device__ __forceinline__ int lead(const void* row) { return (int)((uintptr_t)row & 15); }
+
+// A row's image: every 16-byte piece that holds some of its bytes (a piece
+// lies within one page, so the bytes beside the row can be read), spread over
+// n threads.
+__device__ __forceinline__ void copy_image(uint8_t* dst, const void* row, int bytes, int thread, int n) {
+    const char* src = static_cast<const char*>(row) - lead(row);
+    const int end = lead(row) + bytes;
+    for (int at = thread * 16; at < end; at += n * 16) copy16(dst + at, src + at);
+}
+
+// The same of an aligned row, each lane copying what it will read itself.
+template <int TYPE>
+__device__ __forceinline__ void copy_own(uint8_t* dst, const void* row, const Tile<2>& t) {
 #pragma unroll
-        for (int k = 0; k < C; k++) {
-            const Tile<G> t(k * nw + team.warp, a.cols);
-            tile_load<false>(row_at<TR>(a.residual, at * a.ldr), t, a.cols, r[k]);
-            if (a.branch) tile_load<false>(row_at<TB>(a.branch, at * a.ldb), t, a.cols, b[k]);
-        }
-    };
-    if (row < a.rows) load(row);
-    for (; row < a.rows; row += step) {
-        Raw16<TR, G> y[C];
-        Raw16<TB, G> u[C];
-#pragma unroll
-        for (int k = 0; k < C; k++) {
-            y[k] = r[k];
-            if (a.branch) u[k] = b[k];
-        }
-        if (row + step < a.rows) load(row + step);
-        if (a.branch) {
-            float inv = 1.f;
-            if (a.post) {
-                f2 s = 0ull;
-#pragma unroll
-                for (int k = 0; k < C; k++) {
-                    s = square_sum(u[k], s);
-                    keep_raw(u[k]);
-                }
-                inv = inv_rms(team.sum(f2_sum(s), red), a);
-            }
-#pragma unroll
-            for (int k = 0; k < C; k++) {
-                const Tile<G> t(k * nw + team.warp, a.cols);
-                tile_residual(a, row, t, inv, u[k], y[k]);
-                tile_store(row_at<TR>(a.y, row * a.ldy), t, a.cols, y[k]);
-            }
-        }
-        if (a.out == OUT_NONE) continue;
-        f2 s = 0ull;
-#pragma unroll
-        for (int k = 0; k < C; k++) {
-            s = square_sum(y[k], s);
-            keep_raw(y[k]);
-        }
-        const float inv = inv_rms(team.sum(f2_sum(s), red), a);
-#pragma unroll
-        for (int k = 0; k < C; k++) tile_emit(a, row, Tile<G>(k * nw + team.warp, a.cols), inv, y[k]);
+    for (int g = 0; g < 2; g++) {
+        if (!t.live[g]) continue;
+        const uint32_t at = (uint32_t)t.c[g] * kBytes<TYPE>;
+        const char* src = static_cast<const char*>(row) + at;
+        copy16(dst + at, src);
+        if (TYPE == RENG_TYPE_F32) copy16(dst + at + 16, src + 16);
     }
 }
 
-// Rows too long for the registers: three passes over the columns, each warp
+// A team per row, a warp per tile.  The team's next row travels to shared
+// memory (cp.async) while it works on one, and the vectors that every row
+// takes stay in registers, so HBM is busy while teams wait for their sums.
+// Held as loads in registers instead, the next row left 15 warps an SM and
+// rows of any alignment spilled: 1023 x 5120, f32 branch, gate and both norms
+// 22.5 us against 15.1 (4.2 TB/s); 8192 x 4096 to FP8 65 against 56 (bound by
+// instruction issue, the codes above all); 6599 x 578 to FP8 43 against 16.
+// A third slot costs wide rows their second team (5120 columns: 18.3 us).
+template <int TB, int TR, int G>
+__global__ void __launch_bounds__(32 * kMaxWarps, 1) k_block_norm(const NormArgs a, const Plan p) {
+    extern __shared__ __align__(16) uint8_t sm[];
+    __shared__ float red[2][kMaxWarps];
+    Team team(p.nw);
+    const Tile<G> t(team.warp, a.cols);
+    const int64_t step = (int64_t)gridDim.x * p.teams;
+    int64_t row = (int64_t)team.id * gridDim.x + blockIdx.x;
+    uint8_t* slots = sm + team.id * kSlots * p.slot;
+    const bool gated = a.gate && a.ldg;
+    auto gate_row = [&](int64_t at) -> const void* {
+        return a.tg == RENG_TYPE_BF16 ? row_at<RENG_TYPE_BF16>(a.gate, at * a.ldg)
+                                      : row_at<RENG_TYPE_F32>(a.gate, at * a.ldg);
+    };
+    auto copy = [&](int64_t at, uint8_t* slot) {
+        if (at < a.rows) {
+            const void *u = row_at<TB>(a.branch, at * a.ldb), *r = row_at<TR>(a.residual, at * a.ldr);
+            if constexpr (G == 2) {
+                copy_own<TR>(slot + p.residual, r, t);
+                if (a.branch) copy_own<TB>(slot, u, t);
+                if (gated) {
+                    if (a.tg == RENG_TYPE_BF16) copy_own<RENG_TYPE_BF16>(slot + p.gate, gate_row(at), t);
+                    else copy_own<RENG_TYPE_F32>(slot + p.gate, gate_row(at), t);
+                }
+            } else {
+                const int thread = team.warp * 32 + (threadIdx.x & 31), n = 32 * p.nw;
+                copy_image(slot + p.residual, r, a.cols * kBytes<TR>, thread, n);
+                if (a.branch) copy_image(slot, u, a.cols * kBytes<TB>, thread, n);
+                if (gated) copy_image(slot + p.gate, gate_row(at), a.cols * (a.tg == RENG_TYPE_BF16 ? 2 : 4), thread, n);
+            }
+        }
+        copy_commit();
+    };
+    pdl_wait();
+    pdl_launch();
+#pragma unroll
+    for (int i = 0; i < kSlots - 1; i++) copy(row + i * step, slots + i * p.slot);
+    const Vectors<G> x(a, t);
+    for (int i = 0; row < a.rows; row += step, i = i + 1 == kSlots ? 0 : i + 1) {
+        uint8_t *slot = slots + i * p.slot, *next = slots + (i == 0 ? kSlots - 1 : i - 1) * p.slot;
+        if constexpr (G == 2) {  // the lane's own pieces: its reads of that slot are behind it
+            copy(row + (kSlots - 1) * step, next);
+            copy_wait<kSlots - 1>();
+        } else {  // pieces of other lanes: all of this row there, all reads of the last one done
+            copy_wait<kSlots - 2>();
+            team.wait();
+            copy(row + (kSlots - 1) * step, next);
+        }
+        Raw16<TB, G> u;
+        Raw16<TR, G> y;
+        tile_load<true>(slot + p.residual + (G == 2 ? 0 : lead(row_at<TR>(a.residual, row * a.ldr))), t, a.cols, y);
+        if (a.branch) {
+            tile_load<true>(slot + (G == 2 ? 0 : lead(row_at<TB>(a.branch, row * a.ldb))), t, a.cols, u);
+            float inv = 1.f;
+            if (a.post) inv = inv_rms(team.sum(f2_sum(square_sum(u, 0ull)), red), a);
+            const void* gate = gated ? slot + p.gate + (G == 2 ? 0 : lead(gate_row(row))) : nullptr;
+            tile_residual(a, x, gate, t, inv, u, y);
+            tile_store(row_at<TR>(a.y, row * a.ldy), t, a.cols, y);
+        }
+        if (a.out == OUT_NONE) continue;
+        const float inv = inv_rms(team.sum(f2_sum(square_sum(y, 0ull)), red), a);
+        tile_emit(a, x, row, t, inv, y);
+    }
+}
+
+// Rows too long for shared memory: three passes over the columns, each warp
 // reading back only what it wrote itself.
 template <int TB, int TR, int G>
 __global__ void __launch_bounds__(512) k_block_norm_long(const NormArgs a) {
-    __shared__ float red[2][16];
+    __shared__ float red[2][kMaxWarps];
     Team team(16);
     const int tiles = (a.cols + kTileGroups * kFp8Group - 1) / (kTileGroups * kFp8Group);
     pdl_wait();
@@ -318,6 +396,9 @@ __global__ void __launch_bounds__(512) k_block_norm_long(const NormArgs a) {
     for (int64_t row = blockIdx.x; row < a.rows; row += gridDim.x) {
         const void *branch = row_at<TB>(a.branch, row * a.ldb), *residual = row_at<TR>(a.residual, row * a.ldr);
         void* out = row_at<TR>(a.y, row * a.ldy);
+        const void* gate = !a.gate || !a.ldg ? nullptr
+                           : a.tg == RENG_TYPE_BF16 ? row_at<RENG_TYPE_BF16>(a.gate, row * a.ldg)
+                                                    : row_at<RENG_TYPE_F32>(a.gate, row * a.ldg);
         float inv = 1.f;
         if (a.branch && a.post) {
             f2 s = 0ull;
@@ -336,7 +417,7 @@ __global__ void __launch_bounds__(512) k_block_norm_long(const NormArgs a) {
             if (a.branch) {
                 Raw16<TB, G> u;
                 tile_load<false>(branch, t, a.cols, u);
-                tile_residual(a, row, t, inv, u, y);
+                tile_residual(a, Vectors<G>(a, t), gate, t, inv, u, y);
                 tile_store(out, t, a.cols, y);
             }
             s = square_sum(y, s);
@@ -347,26 +428,42 @@ __global__ void __launch_bounds__(512) k_block_norm_long(const NormArgs a) {
             const Tile<G> t(i, a.cols);
             Raw16<TR, G> y;
             tile_load<false>(a.branch ? out : residual, t, a.cols, y);
-            tile_emit(a, row, t, inv, y);
+            tile_emit(a, Vectors<G>(a, t), row, t, inv, y);
         }
     }
 }
 
+// The image of a row of `cols` elements, with room for its lead.
+int64_t image(int64_t cols, int esize) { return (cols * esize + 15) / 16 * 16 + 16; }
+
+constexpr int kSmemMax = 226 * 1024;
+
 template <int TB, int TR, int G>
 cudaError_t launch_row(const NormArgs& a, int sms, cudaStream_t st) {
     constexpr int kTile = kTileGroups * kFp8Group;
-    const int tiles = (a.cols + kTile - 1) / kTile;
-    if (tiles > 32)
+    const int tiles = (int)(((int64_t)a.cols + kTile - 1) / kTile), eg = a.tg == RENG_TYPE_BF16 ? 2 : 4;
+    const int64_t residual = a.branch ? image(a.cols, kBytes<TB>) : 0, gate = residual + image(a.cols, kBytes<TR>),
+                  slot = gate + (a.gate && a.ldg ? image(a.cols, eg) : 0);
+    if (tiles > kMaxWarps || kSlots * slot > kSmemMax)
         return launch_ops(k_block_norm_long<TB, TR, G>, dim3((unsigned)std::min<int64_t>(a.rows, (int64_t)sms * 4)),
                           dim3(512), 0, st, a);
-    const int c = tiles > 8 ? 2 : 1, nw = (tiles + c - 1) / c, teams = std::max(1, 8 / nw);
-    // as many CTAs as fit the SMs (the kernels' launch bounds), every team on
-    // its next row's loads while it works on one
-    const int64_t want = (a.rows + teams - 1) / teams;
-    const int64_t fit = (int64_t)sms * (c == 1 ? 3 * std::max(1, 8 / (teams * nw)) : std::max(1, 16 / nw));
-    const dim3 grid((unsigned)std::min(want, fit)), block((unsigned)(32 * teams * nw));
-    return c == 1 ? launch_ops(k_block_norm<TB, TR, G, 1>, grid, block, 0, st, a, nw)
-                  : launch_ops(k_block_norm<TB, TR, G, 2>, grid, block, 0, st, a, nw);
+    Plan p;
+    p.nw = tiles;
+    // rows go to as many SMs as there are, then to teams of one CTA
+    p.teams = (int)std::min<int64_t>({p.nw == 1 ? kMaxWarps : 15, kMaxWarps / p.nw, kSmemMax / (kSlots * slot), (a.rows + sms - 1) / sms});
+    p.residual = (int)residual, p.gate = (int)gate, p.slot = (int)slot;
+    const size_t smem = (size_t)(p.teams * kSlots * slot);
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e != cudaSuccess) return e;
+    static std::atomic<uint64_t> ready{0};  // devices whose limit is raised
+    if (dev >= 64 || !(ready.load() >> dev & 1)) {
+        e = cudaFuncSetAttribute(k_block_norm<TB, TR, G>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemMax);
+        if (e != cudaSuccess) return e;
+        if (dev < 64) ready.fetch_or((uint64_t)1 << dev);
+    }
+    const dim3 grid((unsigned)std::min<int64_t>((a.rows + p.teams - 1) / p.teams, sms));
+    return launch_ops(k_block_norm<TB, TR, G>, grid, dim3((unsigned)(32 * p.teams * p.nw)), smem, st, a, p);
 }
 
 int launch(const NormArgs& a, int tb, int tr, bool vec, cudaStream_t st) {

@@ -10,6 +10,7 @@
 // so the activation never goes through HBM at 16 bits.
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "ops.cuh"
 #include "fp8_encode.cuh"
@@ -81,18 +82,17 @@ __device__ __forceinline__ const void* elem(const void* base, int64_t at) {
 }
 
 // 1 x 128 groups: one warp tile of 4 consecutive groups (of any rows) each,
-// codes and scales straight from registers.
+// codes and scales straight from registers.  4 CTAs an SM: with the loads'
+// latency and the exponentials 3 leave issue slots free, and 5 spill (SwiGLU of
+// 8192 x 14336 bf16: 122, 117 and 132 us).
 template <int TYPE, int FMT, int G, bool SWIGLU>
-__global__ void __launch_bounds__(256) k_fp8_groups(GroupArgs a) {
+__global__ void __launch_bounds__(256, 4) k_fp8_groups(GroupArgs a) {
     const uint32_t t0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kTileGroups;
     pdl_wait();
     pdl_launch();
     uint32_t row[G], grp[G];
     int c[G];
-    bool live[G];
-    Raw16<TYPE, G> x, u;
-    raw_zero(x);
-    if (SWIGLU) raw_zero(u);
+    bool live[G], whole = G == 4;  // every group inside its row, for the whole warp
 #pragma unroll
     for (int g = 0; g < G; g++) {
         const uint32_t t = t0 + lane_group<G>(g);
@@ -100,16 +100,30 @@ __global__ void __launch_bounds__(256) k_fp8_groups(GroupArgs a) {
         grp[g] = t - row[g] * a.per_row.d;
         c[g] = (int)(grp[g] * kFp8Group) + lane_col<G>();
         live[g] = t < a.blocks && c[g] < a.cols;
-        if (live[g]) {
+        whole = whole && live[g] && c[g] + kFp8Group <= a.cols;
+    }
+    Raw16<TYPE, G> x, u;
+    auto load = [&](auto all) {
+        constexpr bool kAll = decltype(all)::value;
+#pragma unroll
+        for (int g = 0; g < G; g++) {
+            if (!kAll && !live[g]) continue;
             const int64_t at = row[g] * a.ldx;
             if constexpr (G < 4) {
                 raw_load<TYPE>(elem<TYPE>(a.x, at + c[g]), g, x);
                 if (SWIGLU) raw_load<TYPE>(elem<TYPE>(a.up, at + c[g]), g, u);
             } else {
-                raw_load<TYPE>(elem<TYPE>(a.x, at), c[g], a.cols, g, x);
-                if (SWIGLU) raw_load<TYPE>(elem<TYPE>(a.up, at), c[g], a.cols, g, u);
+                raw_load<TYPE, false, kAll>(elem<TYPE>(a.x, at), c[g], a.cols, g, x);
+                if (SWIGLU) raw_load<TYPE, false, kAll>(elem<TYPE>(a.up, at), c[g], a.cols, g, u);
             }
         }
+    };
+    if (whole) {
+        load(std::true_type());
+    } else {
+        raw_zero(x);
+        if (SWIGLU) raw_zero(u);
+        load(std::false_type());
     }
     f2 v[8];
     raw_floats(x, v);
@@ -146,18 +160,22 @@ __global__ void __launch_bounds__(256) k_fp8_blocks(GroupArgs a) {
     pdl_wait();
     pdl_launch();
     Raw16<TYPE, G> x[4];
+    auto load = [&](auto all) {
+        constexpr bool kAll = decltype(all)::value;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        raw_zero(x[i]);
+        for (int i = 0; i < 4; i++) {
+            if (!kAll) raw_zero(x[i]);
 #pragma unroll
-        for (int g = 0; g < G; g++) {
-            const int64_t row = row_of(i, g);
-            if (row < a.rows && c < a.cols) {
+            for (int g = 0; g < G; g++) {
+                const int64_t row = row_of(i, g);
+                if (!kAll && (row >= a.rows || c >= a.cols)) continue;
                 if constexpr (G < 4) raw_load<TYPE>(elem<TYPE>(a.x, row * a.ldx + c), g, x[i]);
-                else raw_load<TYPE>(elem<TYPE>(a.x, row * a.ldx), c, a.cols, g, x[i]);
+                else raw_load<TYPE, false, kAll>(elem<TYPE>(a.x, row * a.ldx), c, a.cols, g, x[i]);
             }
         }
-    }
+    };
+    if ((int64_t)(rb + 1) * kFp8Group <= a.rows && (int)(grp + 1) * kFp8Group <= a.cols) load(std::true_type());
+    else load(std::false_type());
     float top = 0.f;
     bool odd = false;
 #pragma unroll
@@ -215,10 +233,12 @@ cudaError_t launch_blocks(const GroupArgs& a, int block_rows, bool swiglu, cudaS
 template <int TYPE, int FMT>
 cudaError_t pick_vec(const GroupArgs& a, int block_rows, bool swiglu, cudaStream_t st) {
     const int esz = TYPE == RENG_TYPE_BF16 ? 2 : 4;
-    const bool vec = a.cols % 16 == 0 && ops_aligned(a.x, a.ldx * esz, 16) &&
-                     (!swiglu || ops_aligned(a.up, a.ldx * esz, 16)) && ops_aligned(a.codes, a.ldc, 16);
-    return vec ? launch_blocks<TYPE, FMT, 1>(a, block_rows, swiglu, st)
-               : launch_blocks<TYPE, FMT, 4>(a, block_rows, swiglu, st);
+    // whole 16-column pieces on 16 bytes, whole 8-column pieces, or any row
+    // (333 x 5000 f32: 2.7 us in pieces of 8, 3.7 by elements)
+    const bool rows = ops_aligned(a.x, a.ldx * esz, 16) && (!swiglu || ops_aligned(a.up, a.ldx * esz, 16));
+    if (rows && a.cols % 16 == 0 && ops_aligned(a.codes, a.ldc, 16)) return launch_blocks<TYPE, FMT, 1>(a, block_rows, swiglu, st);
+    if (rows && a.cols % 8 == 0 && ops_aligned(a.codes, a.ldc, 8)) return launch_blocks<TYPE, FMT, 2>(a, block_rows, swiglu, st);
+    return launch_blocks<TYPE, FMT, 4>(a, block_rows, swiglu, st);
 }
 
 int quantize(const char* who, const GroupArgs& a, int type, int block_rows, int fmt, bool swiglu, cudaStream_t st) {

@@ -2,6 +2,8 @@
 // gives the rules and why the hardware converters meet them) and the block
 // quantizers (fp8_blocks.cu, block_norm.cu).
 #pragma once
+#include <type_traits>
+
 #include "common.cuh"
 #include "fp8_product.h"
 
@@ -65,13 +67,15 @@ __device__ __forceinline__ float fp8_block_scale(float absmax) {
 //        scales and shuffles, 32 bytes of a bf16 row a lane (the quantizers);
 //   G 2  columns 8 (l % 16) .. + 7 of groups l / 16 and 2 + l / 16:
 //        consecutive lanes on consecutive 16 bytes of a bf16 row and 32 of an
-//        f32 one (the norm, whose gains are f32 and come from L1);
+//        f32 one (the norm, whose shared memory takes no bank conflicts then,
+//        and quantizers of rows of whole 8-column pieces);
 //   G 4  columns l, 32 + l, 64 + l and 96 + l of every group: one element per
 //        access, consecutive lanes on consecutive elements, for any pitch,
 //        alignment and width.
-// Columns are below 2^31.  G 1 and 2 need rows on 16 bytes and whole 16- or 8-column chunks.  A group's
-// (row pointer, first column) is the caller's; columns at or past `cols` read
-// as 0, which no absmax or sum notices, and are not written.
+// Columns are below 2^31.  G 1 and 2 need rows on 16 bytes and whole 16- or
+// 8-column pieces.  A group's (row pointer, first column) is the caller's;
+// columns at or past `cols` read as 0, which no absmax or sum notices, and are
+// not written.
 constexpr int kTileGroups = 4;
 // This lane's group of index g among the tile's 4, and its first column there.
 template <int G>
@@ -122,17 +126,18 @@ __device__ __forceinline__ void raw_load(const void* p, int g, Raw16<TYPE, G>& r
     }
 }
 
-// G 4: group g's 4 values of this lane, from column c0 of `row`.
-template <int TYPE, bool KEEP = false>
+// G 4: group g's 4 values of this lane, from column c0 of `row`.  WHOLE: the
+// group lies inside the row, no element is tested (a whole warp's case, half
+// the instructions; callers take all loads of a warp one way or the other, so
+// that none waits behind a branch).
+template <int TYPE, bool KEEP = false, bool WHOLE = false>
 __device__ __forceinline__ void raw_load(const void* row, int c0, int cols, int g, Raw16<TYPE, 4>& r) {
-    const int lane = threadIdx.x & 31;
+    using E = std::conditional_t<TYPE == RENG_TYPE_BF16, uint16_t, uint32_t>;
+    const int c = c0 + (threadIdx.x & 31);
+    const E* p = static_cast<const E*>(row) + c;
 #pragma unroll
-    for (int i = 0; i < 4; i++) {
-        const int c = c0 + 32 * i + lane;
-        if (c < cols)
-            r.w[4 * g + i] = TYPE == RENG_TYPE_BF16 ? (uint32_t)ld_elem<KEEP>(static_cast<const uint16_t*>(row) + c)
-                                                    : ld_elem<KEEP>(static_cast<const uint32_t*>(row) + c);
-    }
+    for (int i = 0; i < 4; i++)
+        if (WHOLE || c + 32 * i < cols) r.w[4 * g + i] = (uint32_t)ld_elem<KEEP>(p + 32 * i);
 }
 
 // A lane's values are handled two at a time: one instruction on a register
@@ -300,11 +305,14 @@ __device__ __forceinline__ void tile_store_codes(uint8_t* row, int c, int cols, 
     } else if (G == 2) {
         *reinterpret_cast<uint2*>(row + c) = make_uint2(w[(2 * g) & 3], w[(2 * g + 1) & 3]);
     } else {
-        const int lane = threadIdx.x & 31;
+        uint8_t* p = row + c + (threadIdx.x & 31);
+        if (c + kFp8Group <= cols) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int at = c + 32 * i + lane;
-            if (at < cols) row[at] = (uint8_t)(w[g] >> (8 * i));
+            for (int i = 0; i < 4; i++) p[32 * i] = (uint8_t)(w[g] >> (8 * i));
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if (c + 32 * i + (int)(threadIdx.x & 31) < cols) p[32 * i] = (uint8_t)(w[g] >> (8 * i));
         }
     }
 }
