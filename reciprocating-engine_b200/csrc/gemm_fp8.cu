@@ -25,7 +25,10 @@
 //   * Many rows (PAIR): two CTAs of a cluster multiply one 256-row tile with
 //     tcgen05 cta_group::2; each loads its own 128 token rows and half of the
 //     weight rows, so the bytes an SM takes from L2 per block drop from 48 to
-//     32 KB at bn = 256.
+//     32 KB at bn = 256.  8192 x 28672 x 4096 takes 800 us (2.4 PFLOP/s): the
+//     power limit, the tensor cores busy for 512 of a block's 684 cycles.
+//     (The two halves of the columns as MMAs of their own read the token rows
+//     twice from shared memory: 8192 x 4096 x 14336 440 us against 390.)
 //   * Few tiles (decode): K is split over the CTAs of a cluster, each leaves
 //     its f32 partial in its own shared memory and all of them add a share of
 //     the columns in rank order over distributed shared memory, so the result
@@ -68,8 +71,9 @@ constexpr int kPartRows = 132;   // a split's partial: rows of a column, padded
 constexpr int kThreads = 384;    // a warpgroup of roles, two of accumulators
 constexpr int kAccWarps = 8;
 // an accumulator warp's staging for its output: 32 rows of 16 columns, 17
-// apart, or (PAIR) as many swizzled 32 x 32 boxes as fit 8 KB
-constexpr int kStageOut = 32 * 17 * 4, kStageOutPair = 8192;
+// apart, or (PAIR) as many swizzled 32 x 32 boxes as fit 4 KB: one of f32 or
+// two of bf16 (twice that costs the pipeline a stage: 400 us against 380)
+constexpr int kStageOut = 32 * 17 * 4, kStageOutPair = 4096;
 constexpr int kScaleSlots = 4;   // scales in flight, 4 blocks a slot:
 constexpr int kScaleSlot = kRows * 16 + 64;  // [128 rows][4] of x, [3 weight blocks][4] of w
 // registers per thread after the hand-over: 128 x 40 + 256 x 232 = 384 x 168,
@@ -274,15 +278,14 @@ __device__ __forceinline__ TileAt tile_at(const Fp8Gemm& a, long long t) {
     return {first + in % rows, in / rows};
 }
 
-// The barriers of a CTA: operand stages filled and free, halves of TMEM
-// buffers filled and free ([buffer][half]), scale slots filled and free, the
-// last MMA done.
+// The barriers of a CTA: operand stages, TMEM buffers and scale slots, each
+// filled and free; the last MMA done.
 enum : int {
     B_FULL = 0,
     B_EMPTY = B_FULL + kMaxStages,
     B_TFULL = B_EMPTY + kMaxStages,
-    B_TEMPTY = B_TFULL + 4,
-    B_SFULL = B_TEMPTY + 4,
+    B_TEMPTY = B_TFULL + 2,
+    B_SFULL = B_TEMPTY + 2,
     B_SEMPTY = B_SFULL + kScaleSlots,
     B_DRAIN = B_SEMPTY + kScaleSlots,
     kBars
@@ -294,7 +297,6 @@ enum : int {
 // only keeps the barriers' count.
 struct AccState {
     uint32_t tmem, bar0;     // this warp's TMEM lanes and columns; the barriers
-    int half;                // its half of the columns
     uint32_t sx, sw;         // scales in slot 0: this lane's row, this warp's weight block
     int lane, d, slot;       // the TMEM buffer and the scale slot of the next block
     uint32_t dph, sph;       // their phases
@@ -312,8 +314,8 @@ __device__ __forceinline__ void add_blocks(AccState& st, int k0, int k1, int edg
     }
     for (int b = k0; b < k1; b++) {
         const float s0 = x * w0, s1 = x * w1;
-        const uint32_t src = st.tmem + st.d * kMaxBn, tempty = st.bar0 + 8u * (B_TEMPTY + 2 * st.d + st.half);
-        wait(td, st.bar0 + 8u * (B_TFULL + 2 * st.d + st.half), st.dph, st.bad);
+        const uint32_t src = st.tmem + st.d * kMaxBn, tempty = st.bar0 + 8u * (B_TEMPTY + st.d);
+        wait(td, st.bar0 + 8u * (B_TFULL + st.d), st.dph, st.bad);
         if ((st.d ^= 1) == 0) st.dph ^= 1u;
         __syncwarp();
         asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -330,7 +332,7 @@ __device__ __forceinline__ void add_blocks(AccState& st, int k0, int k1, int edg
                 asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                 __syncwarp();
                 lane0_arrive<PAIR>(tempty, st.lane);
-                td = early(st.bar0 + 8u * (B_TFULL + 2 * st.d + st.half), st.dph);
+                td = early(st.bar0 + 8u * (B_TFULL + st.d), st.dph);
                 const int q = (b - k0) & 3;
                 if (q == 2) {
                     const int next = st.slot + 1 == kScaleSlots ? 0 : st.slot + 1;
@@ -447,9 +449,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             bar_init(bar(B_FULL, s), 1);
             bar_init(bar(B_EMPTY, s), 1);
         }
-        for (int s = 0; s < 4; s++) {
+        for (int s = 0; s < 2; s++) {
             bar_init(bar(B_TFULL, s), 1);
-            bar_init(bar(B_TEMPTY, s), kAccWarps);  // a pair's: half the warps of two CTAs
+            bar_init(bar(B_TEMPTY, s), PAIR ? 2 * kAccWarps : kAccWarps);
         }
         for (int s = 0; s < kScaleSlots; s++) {
             bar_init(bar(B_SFULL, s), 32);
@@ -494,7 +496,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (long long t = first; t < tiles && !bad; t += tstep) {
                 const TileAt at = tile_at(a, t);
                 const int m0 = at.mi * kTileRows_ + (PAIR ? rank * kRows : 0);
-                const int n0 = at.ni * a.bn + (PAIR ? rank * (int)brows / 2 : 0);
+                const int n0 = at.ni * a.bn + (PAIR ? rank * (int)brows : 0);
                 for (int b = k0; b < k1; b++) {
                     if (issued >= a.stages) {
                         wait(bar(B_EMPTY, s), ph ^ 1u, bad);
@@ -507,9 +509,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                             if (rank == 0) bar_expect_tx(bar(B_FULL, s), 2 * (abytes + bbytes));
                             const uint32_t fb = map_cta(bar(B_FULL, s), 0);
                             pair_g2s(xs, &xmap, b * kBK, m0, fb);
-                            // each half of the columns: this CTA's half of its rows
                             pair_g2s(ws, &wmap, b * kBK, n0, fb);
-                            pair_g2s(ws + bbytes / 2, &wmap, b * kBK, n0 + a.bn / 2, fb);
                         } else {
                             bar_expect_tx(bar(B_FULL, s), abytes + bbytes);
                             tensor_g2s(xs, &xmap, b * kBK, m0, bar(B_FULL, s));
@@ -532,45 +532,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                 }
             }
         } else if (warp == 1 && (!PAIR || rank == 0)) {
-            // ---- MMAs; a pair's in two halves of the columns, so that one
-            // half's sum is taken out while the other's runs ----
+            // ---- MMAs ----
             int s = 0, d = 0, used = 0;
-            uint32_t ph = 0, dph = 0, af = 0, ae[2] = {0, 0};  // early answers: the stage, the buffer's halves
+            uint32_t ph = 0, dph = 0, af = 0, ae = 0;  // early answers: the stage, the buffer
             const uint32_t alo0 = kDescLo | sA >> 4, blo0 = kDescLo | sB >> 4;
-            const uint32_t idesc = a.idesc | (uint32_t)((PAIR ? a.bn / 2 : a.bn) >> 3) << 17;
+            const uint32_t idesc = a.idesc | (uint32_t)(a.bn >> 3) << 17;
             for (long long t = first; t < tiles; t += tstep) {
                 for (int b = k0; b < k1; b++) {
                     const uint32_t alo = alo0 + ((uint32_t)s * abytes >> 4), blo = blo0 + ((uint32_t)s * bbytes >> 4);
-                    const uint32_t dst = tmem + d * kMaxBn, done = bar(B_TFULL, 2 * d), gone = bar(B_EMPTY, s);
-                    const uint32_t free0 = bar(B_TEMPTY, 2 * d), fph = dph ^ 1u;
+                    const uint32_t dst = tmem + d * kMaxBn, done = bar(B_TFULL, d), gone = bar(B_EMPTY, s);
                     wait(af, bar(B_FULL, s), ph, bad);
-                    if (used >= 2) wait(ae[0], free0, fph, bad);
+                    if (used >= 2) wait(ae, bar(B_TEMPTY, d), dph ^ 1u, bad);
                     __syncwarp();
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     if (leader && !bad) {
 #pragma unroll
                         for (int kk = 0; kk < 4; kk++) umma_f8<PAIR>(dst, alo + 2 * kk, blo + 2 * kk, idesc, kk != 0);
                         commit<PAIR>(done);
-                        if (!PAIR) commit<PAIR>(gone);
+                        commit<PAIR>(gone);
                     }
                     if (++s == a.stages) s = 0, ph ^= 1u;
                     if ((d ^= 1) == 0) dph ^= 1u;
-                    if (PAIR) {
-                        if (used >= 2) wait(ae[1], free0 + 8u, fph, bad);
-                        __syncwarp();
-                        asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                        ae[1] = early(bar(B_TEMPTY, 2 * d + 1), dph ^ 1u);
-                    }
                     af = early(bar(B_FULL, s), ph);
-                    ae[0] = early(bar(B_TEMPTY, 2 * d), dph ^ 1u);
+                    ae = early(bar(B_TEMPTY, d), dph ^ 1u);
                     used = used < 2 ? used + 1 : used;
-                    if (PAIR && leader && !bad) {
-#pragma unroll
-                        for (int kk = 0; kk < 4; kk++)
-                            umma_f8<PAIR>(dst + h0, alo + 2 * kk, blo + (bbytes / 2 >> 4) + 2 * kk, idesc, kk != 0);
-                        commit<PAIR>(done + 8u);
-                        commit<PAIR>(gone);
-                    }
                 }
             }
             // every MMA issued has completed before TMEM is freed
@@ -643,7 +628,6 @@ __global__ void __launch_bounds__(kThreads, 1)
         AccState st;
         st.tmem = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + c0;
         st.bar0 = bar0;
-        st.half = PAIR ? half : 0;  // without a pair the buffer is filled and freed whole
         st.sx = sScale + 16 * r;
         st.lane = lane;
         st.d = st.slot = 0;
@@ -682,10 +666,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int g = 0; g < 4; g++) {
                     if (32 * g >= cw || n0 + 32 * g >= a.N) break;
                     const unsigned long long* q = acc + 16 * g;
-                    if (a.y_f32) {  // 128-byte rows, two boxes
-                        const uint32_t buf = out0 + box * 4096u;
-                        box = (box + 1) & 1;
-                        if (lane == 0) s2g_wait_read<1>();
+                    if (a.y_f32) {  // 128-byte rows, one box
+                        const uint32_t buf = out0;
+                        if (lane == 0) s2g_wait_read<0>();
                         __syncwarp();
 #pragma unroll
                         for (int ch = 0; ch < 8; ch++) {
@@ -698,10 +681,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) tensor_s2g(&ymap, n0 + 32 * g, mw, buf);
-                    } else {  // 64-byte rows, four boxes
+                    } else {  // 64-byte rows, two boxes
                         const uint32_t buf = out0 + box * 2048u;
-                        box = (box + 1) & 3;
-                        if (lane == 0) s2g_wait_read<3>();
+                        box ^= 1;
+                        if (lane == 0) s2g_wait_read<1>();
                         __syncwarp();
 #pragma unroll
                         for (int ch = 0; ch < 4; ch++) {
@@ -871,13 +854,14 @@ int launch_tiles(const CUtensorMap& xm, const CUtensorMap& wm, const CUtensorMap
     return RENG_OK;
 }
 
-// Cycles that a plan's busiest SM takes, from what launches took on B200 (bf16
-// output, 2048 x 18944 x 4096 and x 16384): a block costs about 400 + 2.45 bn
-// cycles in one CTA and 600 + 1.5 bn in a pair, and no less than its bytes at
-// 64 a cycle from L2 and 23 from HBM when all SMs stream; a tile has a fixed
-// cost, and a split's exchange 4000 + 50 bn (64 rows x 4096 x 14336: 20.4 us
-// split by 4 against 34 whole; clusters of 3 and of 5 to 8 leave SMs of a GPC
-// empty and took twice as long).
+// Cycles that a plan's busiest SM takes, from what launches of one round took
+// on B200 (1024 rows x 18 bn x 4096 and 16384, at 1.9 GHz): a block costs about
+// 357 + 2.1 bn cycles in one CTA and 315 + 2.13 bn in a pair, bn rounded up to
+// 64 (the MMAs' own 2 bn and the issuing warp's waits, which they do not
+// cover), and no less than its bytes at 64 a cycle from L2 and 23 from HBM
+// when all SMs stream; a tile has a fixed cost, and a split's exchange 4000 +
+// 50 bn (64 rows x 4096 x 14336: 20.4 us split by 4 against 34 whole; clusters
+// of 3 and of 5 to 8 leave SMs of a GPC empty and took twice as long).
 struct Plan {
     bool pair;
     int bn, ks;
@@ -901,7 +885,8 @@ Plan plan(int M, int N, int kb, int sms) {
                 const double bytes = (std::min(M, kRows) + (pair ? bn / 2 : bn)) * (double)kBK;
                 // all weights pass from HBM once; a round's share of it
                 const double hbm = (double)N * kb * kBK / (23.0 * std::min<long long>(tiles, sms)) / ((double)rounds * blocks);
-                const double block = std::max({pair ? 600.0 + 1.5 * bn : 400.0 + 2.45 * bn, bytes / 64.0, hbm});
+                const int wide = (bn + 63) / 64 * 64;
+                const double block = std::max({pair ? 315.0 + 2.13 * wide : 357.0 + 2.1 * wide, bytes / 64.0, hbm});
                 const double cost = rounds * (blocks * block + (pair ? 1500.0 : 3000.0) + (ks > 1 ? 4000.0 + 50.0 * bn : 0.0));
                 if (cost < best.cost) best = {pair != 0, bn, ks, cost};
                 if (bn <= 32) break;
@@ -948,7 +933,7 @@ int gemm_fp8_blocks(const uint8_t* x, int64_t ldx, const float* sx, int64_t ldsx
               ((uint32_t)(rows >> 4) << 24);  // the kernel adds N
     CUtensorMap xm, wm, ym{};
     int rc = codes_map(x, M, K, ldx, a.mbox, &xm);
-    if (!rc) rc = codes_map(w, N, K, ldw, p.pair ? a.bn / 4 : a.bn, &wm);
+    if (!rc) rc = codes_map(w, N, K, ldw, p.pair ? a.bn / 2 : a.bn, &wm);
     if (!rc && p.pair && a.y_tma) rc = y_map(y, a.y_f32, M, N, ldy, &ym);
     if (rc) return rc;
     const long long tiles = (long long)a.mt * a.nt;
