@@ -29,6 +29,9 @@
 //     power limit, the tensor cores busy for 512 of a block's 684 cycles.
 //     (The two halves of the columns as MMAs of their own read the token rows
 //     twice from shared memory: 8192 x 4096 x 14336 440 us against 390.)
+//   * The last round of tiles over the SMs is rarely full: it takes narrower
+//     tiles than the rounds before it (1001 x 5120 x 27648: 166 us in tiles of
+//     192 columns, 154 in 18 of 256 and 8 of 64; 5789 x 909 x 4011 64 and 50).
 //   * Few tiles (decode): K is split over the CTAs of a cluster, each leaves
 //     its f32 partial in its own shared memory and all of them add a share of
 //     the columns in rank order over distributed shared memory, so the result
@@ -87,7 +90,8 @@ struct Fp8Gemm {
     void* y;
     int64_t ldsx, ldsw, ldy;
     int M, N, kb;      // rows, columns, 128-k blocks
-    int mt, nt, bn;    // tiles and their width
+    int mt, nt, bn;    // row and column tiles, their width
+    int nt1, bn2;      // column tiles of that width; those behind them are bn2 wide
     int group;         // row tiles walked before the next column tile
     int ks;            // K splits (CTAs of a cluster; 1 with PAIR)
     int stages, mbox;  // pipeline stages, token rows of an x copy
@@ -267,15 +271,19 @@ __device__ __forceinline__ void st_global32(void* p, const uint32_t (&w)[8]) {
 }
 
 // The tile of index t: row tiles fastest within groups of `group`, so the
-// CTAs at work together share a few row and column tiles in L2.
+// CTAs at work together share a few row and column tiles in L2; the wide
+// tiles first.
 struct TileAt {
-    int mi, ni;
+    int mi, n0, bn;
 };
 __device__ __forceinline__ TileAt tile_at(const Fp8Gemm& a, long long t) {
-    const long long per = (long long)a.group * a.nt;
+    const long long wide = (long long)a.mt * a.nt1;
+    const bool second = t >= wide;
+    if (second) t -= wide;
+    const long long per = (long long)a.group * (second ? a.nt - a.nt1 : a.nt1);
     const int g = (int)(t / per), first = g * a.group, rows = min(a.group, a.mt - first);
-    const int in = (int)(t - g * per);
-    return {first + in % rows, in / rows};
+    const int in = (int)(t - g * per), ni = in / rows;
+    return {first + in % rows, second ? a.nt1 * a.bn + ni * a.bn2 : ni * a.bn, second ? a.bn2 : a.bn};
 }
 
 // The barriers of a CTA: operand stages, TMEM buffers and scale slots, each
@@ -424,7 +432,7 @@ __device__ __forceinline__ void add_partials(const Fp8Gemm& a, float* part, int 
 template <bool PAIR>
 __global__ void __launch_bounds__(kThreads, 1)
     k_gemm_fp8(const __grid_constant__ CUtensorMap xmap, const __grid_constant__ CUtensorMap wmap,
-               const __grid_constant__ CUtensorMap ymap, const Fp8Gemm a) {
+               const __grid_constant__ CUtensorMap wmap2, const __grid_constant__ CUtensorMap ymap, const Fp8Gemm a) {
     namespace cg = cooperative_groups;
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     __shared__ __align__(8) unsigned long long bars[kBars];
@@ -479,7 +487,6 @@ __global__ void __launch_bounds__(kThreads, 1)
     pdl_wait();
     pdl_launch();
 
-    const int h0 = (a.bn / 2 + 31) / 32 * 32;  // columns of the first half
     const int split = PAIR ? 0 : rank, span = PAIR ? 2 : a.ks;  // CTAs per tile
     const int k0 = (int)((long long)split * a.kb / a.ks), k1 = (int)((long long)(split + 1) * a.kb / a.ks);
     const long long tiles = (long long)a.mt * a.nt, first = blockIdx.x / span, tstep = gridDim.x / span;
@@ -496,7 +503,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (long long t = first; t < tiles && !bad; t += tstep) {
                 const TileAt at = tile_at(a, t);
                 const int m0 = at.mi * kTileRows_ + (PAIR ? rank * kRows : 0);
-                const int n0 = at.ni * a.bn + (PAIR ? rank * (int)brows : 0);
+                const uint32_t nrows = PAIR ? (uint32_t)at.bn / 2 : (uint32_t)at.bn, bytes = abytes + nrows * kBK;
+                const int n0 = at.n0 + (PAIR ? rank * (int)nrows : 0);
+                const CUtensorMap* wm = at.bn == a.bn ? &wmap : &wmap2;
                 for (int b = k0; b < k1; b++) {
                     if (issued >= a.stages) {
                         wait(bar(B_EMPTY, s), ph ^ 1u, bad);
@@ -506,14 +515,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (leader) {
                         if (PAIR) {
                             // the leader CTA's barrier counts the bytes of both
-                            if (rank == 0) bar_expect_tx(bar(B_FULL, s), 2 * (abytes + bbytes));
+                            if (rank == 0) bar_expect_tx(bar(B_FULL, s), 2 * bytes);
                             const uint32_t fb = map_cta(bar(B_FULL, s), 0);
                             pair_g2s(xs, &xmap, b * kBK, m0, fb);
-                            pair_g2s(ws, &wmap, b * kBK, n0, fb);
+                            pair_g2s(ws, wm, b * kBK, n0, fb);
                         } else {
-                            bar_expect_tx(bar(B_FULL, s), abytes + bbytes);
+                            bar_expect_tx(bar(B_FULL, s), bytes);
                             tensor_g2s(xs, &xmap, b * kBK, m0, bar(B_FULL, s));
-                            tensor_g2s(ws, &wmap, b * kBK, n0, bar(B_FULL, s));
+                            tensor_g2s(ws, wm, b * kBK, n0, bar(B_FULL, s));
                         }
                     }
                     issued = issued < a.stages ? issued + 1 : issued;
@@ -536,8 +545,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             int s = 0, d = 0, used = 0;
             uint32_t ph = 0, dph = 0, af = 0, ae = 0;  // early answers: the stage, the buffer
             const uint32_t alo0 = kDescLo | sA >> 4, blo0 = kDescLo | sB >> 4;
-            const uint32_t idesc = a.idesc | (uint32_t)(a.bn >> 3) << 17;
             for (long long t = first; t < tiles; t += tstep) {
+                const uint32_t idesc = a.idesc | (uint32_t)(tile_at(a, t).bn >> 3) << 17;
                 for (int b = k0; b < k1; b++) {
                     const uint32_t alo = alo0 + ((uint32_t)s * abytes >> 4), blo = blo0 + ((uint32_t)s * bbytes >> 4);
                     const uint32_t dst = tmem + d * kMaxBn, done = bar(B_TFULL, d), gone = bar(B_EMPTY, s);
@@ -578,7 +587,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             for (long long t = first; t < tiles; t += tstep) {
                 const TileAt at = tile_at(a, t);
                 const int m0 = at.mi * kTileRows_ + (PAIR ? rank * kRows : 0);
-                const int wb = min(at.ni * a.bn / kBK + (lane >> 2), (a.N - 1) / kBK);
+                const int wb = min(at.n0 / kBK + (lane >> 2), (a.N - 1) / kBK);
                 for (int b = k0; b < k1; b += 4) {
                     if (used >= kScaleSlots) wait(bar(B_SEMPTY, slot), ph ^ 1u, bad);
                     const uint32_t dst = sScale + slot * kScaleSlot;
@@ -621,12 +630,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsAcc));
         const int half = (warp - 4) >> 2;
         const int r = 32 * (warp & 3) + lane;
-        // this warp's columns of a tile (multiples of 32)
-        const int c0 = half ? h0 : 0, cw = half ? a.bn - h0 : h0;
         const uint32_t out0 = sOut + (uint32_t)(warp - 4) * (PAIR ? kStageOutPair : kStageOut);
         uint32_t box = 0;  // staging box of the next output copy
         AccState st;
-        st.tmem = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + c0;
         st.bar0 = bar0;
         st.sx = sScale + 16 * r;
         st.lane = lane;
@@ -636,14 +642,17 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (long long t = first; t < tiles; t += tstep) {
             const TileAt at = tile_at(a, t);
             const int mw = at.mi * kTileRows_ + (PAIR ? rank * kRows : 0) + 32 * (warp & 3), m = mw + lane;
-            const int n0 = at.ni * a.bn + c0;
+            // this warp's columns of the tile (multiples of 32)
+            const int h0 = (at.bn / 2 + 31) / 32 * 32, c0 = half ? h0 : 0, cw = half ? at.bn - h0 : h0;
+            const int n0 = at.n0 + c0;
+            st.tmem = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + c0;
             const bool any = mw < a.M && n0 < a.N && cw > 0;  // the warp has outputs in this tile
             unsigned long long acc[64];
 #pragma unroll
             for (int c = 0; c < 64; c++) acc[c] = 0ull;
             // its columns touch at most two weight blocks; the second starts at column `edge`
             const int edge = (n0 / kBK + 1) * kBK - n0;
-            st.sw = sScale + kRows * 16 + 16 * (n0 / kBK - at.ni * a.bn / kBK);
+            st.sw = sScale + kRows * 16 + 16 * (n0 / kBK - at.n0 / kBK);
             add_tile<PAIR>(st, any ? cw / 32 : 0, edge < cw, k0, k1, edge, acc);
             if (!any) continue;
             if (!PAIR && a.ks > 1) {
@@ -758,7 +767,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             cg::this_cluster().sync();
             const TileAt at = tile_at(a, first);
             add_partials(a, reinterpret_cast<float*>(smem_raw + (smem0 - (uint32_t)__cvta_generic_to_shared(smem_raw))),
-                         at.mi * kRows, at.ni * a.bn, rank);
+                         at.mi * kRows, at.n0, rank);
             cg::this_cluster().sync();  // this CTA's partial stays until its peers have read it
         }
     }
@@ -815,8 +824,8 @@ int y_map(void* y, bool f32, int64_t M, int64_t N, int64_t ldy, CUtensorMap* out
 constexpr size_t kSmemMax = 227 * 1024 - 1024;  // dynamic shared memory of a CTA, beside its barriers
 
 template <bool PAIR>
-int launch_tiles(const CUtensorMap& xm, const CUtensorMap& wm, const CUtensorMap& ym, Fp8Gemm& a, int grid,
-                 cudaStream_t st) {
+int launch_tiles(const CUtensorMap& xm, const CUtensorMap& wm, const CUtensorMap& wm2, const CUtensorMap& ym, Fp8Gemm& a,
+                 int grid, cudaStream_t st) {
     const int brows = PAIR ? a.bn / 2 : a.bn;
     const size_t stage = (size_t)(a.mbox + brows) * kBK, out = (size_t)kAccWarps * (PAIR ? kStageOutPair : kStageOut) + kScaleSlots * kScaleSlot;
     const int steps = (int)(((long long)a.mt * a.nt * (PAIR ? 2 : a.ks) + grid - 1) / grid) * ((a.kb + a.ks - 1) / a.ks);
@@ -850,7 +859,7 @@ int launch_tiles(const CUtensorMap& xm, const CUtensorMap& wm, const CUtensorMap
     attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
     cfg.numAttrs = PAIR || a.ks > 1 ? 2 : 1;
-    RENG_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm_fp8<PAIR>, xm, wm, ym, a));
+    RENG_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_gemm_fp8<PAIR>, xm, wm, wm2, ym, a));
     return RENG_OK;
 }
 
@@ -865,13 +874,23 @@ int launch_tiles(const CUtensorMap& xm, const CUtensorMap& wm, const CUtensorMap
 struct Plan {
     bool pair;
     int bn, ks;
+    int nt1, bn2;  // bn2 > 0: nt1 column tiles of bn, the others of bn2
     double cost;
 };
 Plan plan(int M, int N, int kb, int sms) {
-    Plan best{false, 256, 1, 1e300};
+    Plan best{false, 256, 1, 0, 0, 1e300};
     const int mt1 = (M + kRows - 1) / kRows;
     for (int pair = 0; pair <= (M > kRows ? 1 : 0); pair++) {
         const int mt = pair ? (mt1 + 1) / 2 : mt1, slots = pair ? sms / 2 : sms, step = pair ? 64 : 32;
+        // a block's cost in a launch of `rounds` rounds of `tiles` tiles, `blocks` blocks each
+        auto block = [&](int bn, long long tiles, long long rounds, int blocks) {
+            const int wide = (bn + 63) / 64 * 64;
+            const double bytes = (std::min(M, kRows) + (pair ? bn / 2 : bn)) * (double)kBK;
+            // all weights pass from HBM once; a round's share of it
+            const double hbm = (double)N * kb * kBK / (23.0 * std::min<long long>(tiles, sms)) / ((double)rounds * blocks);
+            return std::max({pair ? 315.0 + 2.13 * wide : 357.0 + 2.1 * wide, bytes / 64.0, hbm});
+        };
+        const double fixed = pair ? 1500.0 : 3000.0;
         for (int ks = 1; ks <= (pair ? 1 : std::min(kMaxSplit, kb)); ks *= 2) {
             if (ks > 1 && mt > slots / ks) break;
             for (int w = 1; w <= 6; w++) {
@@ -882,14 +901,22 @@ Plan plan(int M, int N, int kb, int sms) {
                 const long long rounds = (tiles + slots - 1) / slots;
                 if (ks > 1 && rounds > 1) continue;
                 const int blocks = (kb + ks - 1) / ks;
-                const double bytes = (std::min(M, kRows) + (pair ? bn / 2 : bn)) * (double)kBK;
-                // all weights pass from HBM once; a round's share of it
-                const double hbm = (double)N * kb * kBK / (23.0 * std::min<long long>(tiles, sms)) / ((double)rounds * blocks);
-                const int wide = (bn + 63) / 64 * 64;
-                const double block = std::max({pair ? 315.0 + 2.13 * wide : 357.0 + 2.1 * wide, bytes / 64.0, hbm});
-                const double cost = rounds * (blocks * block + (pair ? 1500.0 : 3000.0) + (ks > 1 ? 4000.0 + 50.0 * bn : 0.0));
-                if (cost < best.cost) best = {pair != 0, bn, ks, cost};
+                const double cost = rounds * (blocks * block(bn, tiles, rounds, blocks) + fixed + (ks > 1 ? 4000.0 + 50.0 * bn : 0.0));
+                if (cost < best.cost) best = {pair != 0, bn, ks, 0, 0, cost};
                 if (bn <= 32) break;
+            }
+        }
+        // wide tiles in all rounds but the last, which narrower ones fill
+        for (int w = 2; w <= 6; w++) {
+            for (int bn = kMaxBn; bn > step; bn -= step) {
+                const int nt1 = (int)std::min<long long>((long long)(w - 1) * slots / mt, N / bn), left = N - nt1 * bn;
+                const int fit = (int)(((long long)w * slots - (long long)mt * nt1) / mt);
+                if (nt1 < 1 || fit < 1 || left < 1) continue;
+                const int bn2 = ((left + fit - 1) / fit + step - 1) / step * step;
+                if (bn2 >= bn) break;
+                const long long tiles = (long long)mt * (nt1 + (left + bn2 - 1) / bn2);
+                const double cost = kb * ((w - 1) * block(bn, tiles, w, kb) + block(bn2, tiles, w, kb)) + w * fixed;
+                if (cost < best.cost) best = {pair != 0, bn, 1, nt1, bn2, cost};
             }
         }
     }
@@ -926,19 +953,23 @@ int gemm_fp8_blocks(const uint8_t* x, int64_t ldx, const float* sx, int64_t ldsx
     a.ks = p.ks;
     const int rows = p.pair ? 2 * kRows : kRows;
     a.mt = (M + rows - 1) / rows;
-    a.nt = (N + a.bn - 1) / a.bn;
+    a.nt1 = p.bn2 ? p.nt1 : (N + a.bn - 1) / a.bn;
+    a.bn2 = p.bn2;
+    a.nt = a.nt1 + (p.bn2 ? (N - a.nt1 * a.bn + p.bn2 - 1) / p.bn2 : 0);
     a.group = std::min(a.mt, p.pair ? 8 : 16);
     // E4M3 is operand type 0, E5M2 1; f32 accumulation
     a.idesc = (1u << 4) | ((uint32_t)(x_fmt == RENG_FP8_E5M2) << 7) | ((uint32_t)(w_fmt == RENG_FP8_E5M2) << 10) |
               ((uint32_t)(rows >> 4) << 24);  // the kernel adds N
-    CUtensorMap xm, wm, ym{};
+    CUtensorMap xm, wm, wm2, ym{};
     int rc = codes_map(x, M, K, ldx, a.mbox, &xm);
     if (!rc) rc = codes_map(w, N, K, ldw, p.pair ? a.bn / 2 : a.bn, &wm);
+    wm2 = wm;
+    if (!rc && p.bn2) rc = codes_map(w, N, K, ldw, p.pair ? p.bn2 / 2 : p.bn2, &wm2);
     if (!rc && p.pair && a.y_tma) rc = y_map(y, a.y_f32, M, N, ldy, &ym);
     if (rc) return rc;
     const long long tiles = (long long)a.mt * a.nt;
-    if (p.pair) return launch_tiles<true>(xm, wm, ym, a, 2 * (int)std::min<long long>(tiles, sms / 2), st);
-    return launch_tiles<false>(xm, wm, ym, a, a.ks > 1 ? (int)tiles * a.ks : (int)std::min<long long>(tiles, sms), st);
+    if (p.pair) return launch_tiles<true>(xm, wm, wm2, ym, a, 2 * (int)std::min<long long>(tiles, sms / 2), st);
+    return launch_tiles<false>(xm, wm, wm2, ym, a, a.ks > 1 ? (int)tiles * a.ks : (int)std::min<long long>(tiles, sms), st);
 }
 
 }  // namespace reng

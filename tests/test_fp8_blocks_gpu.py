@@ -142,6 +142,21 @@ def test_product(m, n, k, dtype):
     check_product(gemm.gemm_fp8_blocks(*ops, dtype=dtype), *ops)
 
 
+@pytest.mark.parametrize("m,n,k", [
+    (1001, 5120, 384), (1001, 5123, 300), (2048, 6144, 128), (3000, 4100, 256), (5789, 909, 261),  # pairs
+    (100, 40000, 200), (60, 40333, 128)])
+def test_product_in_tiles_of_two_widths(m, n, k):
+    """Sizes whose last round of tiles is narrower than the others."""
+    from reng import gemm
+    ops = operands(m + n + k, m, n, k)
+    check_product(gemm.gemm_fp8_blocks(*ops, dtype=BF16), *ops)
+    y, store = pitched(m, n, n + 3, F32, 1, fill=-3.0)  # by elements instead of whole boxes
+    gemm.gemm_fp8_blocks(*ops, out=y)
+    check_product(y, *ops)
+    y.fill_(-3.0)
+    assert bool((store == -3.0).all())
+
+
 @pytest.mark.parametrize("xf,wf", [(0, 1), (1, 0), (1, 1)])
 @pytest.mark.parametrize("m,n,k", [(5, 200, 700), (300, 2000, 300), (1024, 6144, 256)])
 def test_product_formats(m, n, k, xf, wf):
@@ -335,6 +350,45 @@ def test_block_norm_pitches_leave_the_rest():
             assert bool(((got.float() - w.float()).abs() <= steps * 2.02 * U_BF16 * w.float().abs() + 1e-30).all())
         y.fill_(9.0), h.fill_(9.0)
         assert bool((ys == 9.0).all()) and bool((hs == 9.0).all())
+
+
+@pytest.mark.parametrize("rows,cols", [(8000, 75), (4000, 300), (1200, 1407), (700, 6200), (310, 8200)])
+def test_block_norm_rows_of_any_alignment(rows, cols):
+    """Several rows per team, each stream with a pitch and an offset of its own."""
+    from reng import norm
+    c = norm_case(rows, cols, F32, BF16, True, "full", cols)
+    for i, k in enumerate(("residual", "branch", "gate")):
+        moved, _ = pitched(rows, cols, cols + 3 + i, c[k].dtype, 1 + 2 * i, fill=float("nan"))
+        moved.copy_(c[k])
+        c[k] = moved
+    for k in ("post_gain", "pre_gain"):
+        moved = torch.empty(cols + 1, device="cuda")[1:]
+        c[k] = moved.copy_(c[k])
+    y, ys = pitched(rows, cols, cols + 2, BF16, 7, fill=9.0)
+    h, hs = pitched(rows, cols, cols + 1, BF16, 2, fill=9.0)
+    norm.block_norm(**c, scale=0.5, out=y, h=h)
+    check_y(y, c, 0.5, 1e-5)
+    want = want_h(y, c["pre_gain"], 1e-5)
+    assert bool(((h.double() - want).abs() <= (NORM_REL + U_BF16 * (1 + NORM_REL)) * want.abs()).all())
+    codes, cs = pitched(rows, cols, cols + 5, torch.uint8, 3, fill=0xA5)
+    groups = (cols + 127) // 128
+    scales, ss = pitched(rows, groups, groups + 1, F32, 1, fill=7.5)
+    y2, _, _ = norm.block_norm_fp8(**c, scale=0.5, codes=codes, scales=scales)
+    assert torch.equal(y2, y)
+    check_groups(codes, scales, want_h(y2, c["pre_gain"], 1e-5), 0, NORM_REL)
+    for t, store, fill in ((y, ys, 9.0), (h, hs, 9.0), (codes, cs, 0xA5), (scales, ss, 7.5)):
+        t.fill_(fill)
+        assert bool((store == fill).all())
+
+
+@pytest.mark.parametrize("rows,cols", [(3000, 576), (3000, 577), (1001, 5120)])
+def test_block_norm_in_place_over_many_rows(rows, cols):
+    from reng import norm
+    c = norm_case(rows, cols, BF16, BF16, True, "none", 5)
+    y, h = norm.block_norm(**c)
+    r = c["residual"].clone()
+    y2, h2 = norm.block_norm(**{**c, "residual": r}, out=r)
+    assert y2 is r and torch.equal(r, y) and torch.equal(h, h2)
 
 
 def test_block_norm_rows_of_zeros():
