@@ -48,7 +48,7 @@ __device__ __forceinline__ void swiglu(f2 (&v)[8], const f2 (&u)[8]) {
         const f2 g = v[i];
         float g0, g1, e0, e1, d0, d1;
         split_f2(g, g0, g1);
-        top = absmax_nan(absmax_nan(top, g0), g1);
+        top = absmax_nan(top, g0, g1);
         const f2 hi = mul_f2(g, make_f2(-1.44269504f));
         const f2 neg = mul_f2(hi, make_f2(-1.0f));
         const f2 lo = fma_f2(g, make_f2(-1.33497580e-8f), mul_f2(fma_f2(g, make_f2(-1.44269504f), neg), make_f2(0.693147181f)));

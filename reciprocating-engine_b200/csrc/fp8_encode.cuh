@@ -186,10 +186,10 @@ __device__ __forceinline__ uint32_t bf16x2(float lo, float hi) {
     return r;
 }
 
-// max(m, |x|), NaN if x is.
-__device__ __forceinline__ float absmax_nan(float m, float x) {
+// max(m, |x|, |y|), NaN if x or y is.
+__device__ __forceinline__ float absmax_nan(float m, float x, float y) {
     float r;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(m), "f"(fabsf(x)));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(m), "f"(fabsf(x)), "f"(fabsf(y)));
     return r;
 }
 
@@ -233,9 +233,9 @@ __device__ __forceinline__ void tile_absmax(const f2 (&v)[8], float (&m)[G], boo
         for (int i = 0; i < P; i++) {
             float a, b;
             split_f2(v[P * g + i], a, b);
-            m[g] = absmax_nan(absmax_nan(m[g], a), b);
+            m[g] = absmax_nan(m[g], a, b);
         }
-        top = absmax_nan(top, m[g]);
+        top = G == 1 ? m[g] : absmax_nan(top, m[g], 0.f);
     }
     odd = __any_sync(0xffffffffu, !(top < __int_as_float(0x7f800000)));
     if (odd) {
@@ -257,7 +257,7 @@ __device__ __forceinline__ void tile_absmax(const f2 (&v)[8], float (&m)[G], boo
 // a rounding, which the converter brings back to max_finite, so nothing is
 // clamped and no NaN is looked for; scales of at least 2^-60 take
 // fp8_product.h's correction of x * RN(1 / s) (the correctly rounded
-// quotient, with the sign of x put on a zero), smaller ones the division.
+// quotient), smaller ones the division.
 template <int FMT, int G>
 __device__ __forceinline__ void tile_codes(const f2 (&v)[8], const float (&s)[G], const float (&rs)[G], bool odd,
                                            uint32_t (&w)[4]) {
@@ -265,9 +265,11 @@ __device__ __forceinline__ void tile_codes(const f2 (&v)[8], const float (&s)[G]
 #pragma unroll
     for (int g = 0; g < G; g++) product = product && s[g] >= 8.6736174e-19f;
     if (product) {
-        f2 r[G], n[G];
+        // -x / s, so that a zero comes out with its sign: the residual of
+        // x = -0 would be +0, and take the sign of the quotient with it
+        f2 r[G], p[G];
 #pragma unroll
-        for (int g = 0; g < G; g++) r[g] = make_f2(rs[g]), n[g] = make_f2(-s[g]);
+        for (int g = 0; g < G; g++) r[g] = make_f2(-rs[g]), p[g] = make_f2(s[g]);
 #pragma unroll
         for (int i = 0; i < 4; i++) {
             const int g = i * G / 4;
@@ -275,15 +277,11 @@ __device__ __forceinline__ void tile_codes(const f2 (&v)[8], const float (&s)[G]
 #pragma unroll
             for (int h = 0; h < 2; h++) {
                 const f2 x = v[2 * i + h], y = mul_f2(x, r[g]);
-                const f2 q = fma_f2(fma_f2(y, n[g], x), r[g], y);
-                float q0, q1, x0, x1;
-                split_f2(q, q0, q1);
-                split_f2(x, x0, x1);
-                q0 = __uint_as_float(__float_as_uint(q0) | (__float_as_uint(x0) & 0x80000000u));
-                q1 = __uint_as_float(__float_as_uint(q1) | (__float_as_uint(x1) & 0x80000000u));
+                float q0, q1;
+                split_f2(fma_f2(fma_f2(y, p[g], x), r[g], y), q0, q1);
                 c[h] = FMT == RENG_FP8_E4M3 ? cvt_e4m3x2(q0, q1) : cvt_e5m2x2(q0, q1);
             }
-            w[i] = __byte_perm(c[0], c[1], 0x5410);
+            w[i] = __byte_perm(c[0], c[1], 0x5410) ^ 0x80808080u;
         }
     } else {
 #pragma unroll

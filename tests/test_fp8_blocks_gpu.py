@@ -157,6 +157,23 @@ def test_product_in_tiles_of_two_widths(m, n, k):
     assert bool((store == -3.0).all())
 
 
+@pytest.mark.parametrize("block_rows", [1, 128])
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("cols", [128, 131, 136])
+def test_zeros_and_small_values_keep_their_sign(cols, fmt, block_rows):
+    """-0 and negative values that round to zero take the code 0x80, positive ones 0, as the division gives them."""
+    from reng import fp8
+    for dtype in (BF16, F32):
+        x = torch.zeros(128, cols, device="cuda", dtype=dtype)
+        x[:, 1::2] = -0.0
+        x[:, 0] = 3.0           # a scale
+        x[:, 2], x[:, 3] = 1e-30, -1e-30
+        codes, _ = fp8.quantize_blocks(x, block_rows, fmt)
+        neg = torch.zeros_like(codes)
+        neg[:, 1::2] = 0x80
+        assert torch.equal(codes[:, 1:128], neg[:, 1:128]) and bool((codes[:, 128:] & 0x7F == 0).all())
+
+
 @pytest.mark.parametrize("xf,wf", [(0, 1), (1, 0), (1, 1)])
 @pytest.mark.parametrize("m,n,k", [(5, 200, 700), (300, 2000, 300), (1024, 6144, 256)])
 def test_product_formats(m, n, k, xf, wf):
