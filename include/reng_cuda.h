@@ -320,9 +320,11 @@ int reng_gemm_bf16(const uint16_t *w, int rows, int K, const uint16_t *x, int M,
  * [rows, ceil(cols / 128)]; block_rows 128: per 128 x 128 block (weights),
  * scales [ceil(rows / 128), ceil(cols / 128)].  A block's scale is its absmax
  * / max_finite (1.0 for a block of zeros, never below the smallest normal
- * f32; NaN is never the absmax) and its codes encode(x / scale) by the rules of reng_fp8_quantize: an infinity
- * makes its own block's scale infinite, and itself and NaN code to NaN.  Any
- * cols, pitch and element alignment; 16-byte aligned rows are read wide.
+ * f32; NaN is never the absmax) and its codes encode(x / scale) by the rules
+ * of reng_fp8_quantize: an infinity makes its own block's scale infinite, and
+ * itself and NaN code to NaN.  Any cols up to 2^30 with fewer than 2^31
+ * groups in all, any pitch and element alignment; 16-byte aligned rows are
+ * read wide.
  */
 int reng_fp8_quantize_blocks(const void *x, int type, int64_t rows, int64_t cols, int64_t ldx,
                              int block_rows, int fmt, uint8_t *codes, int64_t ldc, float *scales,

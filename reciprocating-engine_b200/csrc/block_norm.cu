@@ -201,19 +201,19 @@ __device__ __forceinline__ void tile_store(void* row, const Tile<G>& t, int cols
 }
 
 // y of a tile, rounded, from the branch u and the residual y:
-// y + (r(u) scale) (u f gate), the gate's row of this row or null.
+// y + (u (r(u) scale) gate) f, the gate's row of this row or null.
 template <int TB, int TR, int G>
 __device__ __forceinline__ void tile_residual(const NormArgs& a, const Vectors<G>& x, const void* gate,
                                               const Tile<G>& t, float inv, const Raw16<TB, G>& u, Raw16<TR, G>& y) {
     f2 v[8], w[8];
     raw_floats(u, v);
-#pragma unroll
-    for (int i = 0; i < 8; i++) v[i] = mul_f2(v[i], x.f[i]);
-    if (gate) tile_gate(a, gate, t, v);
-    raw_floats(y, w);
     const f2 s = make_f2(inv * a.scale);
 #pragma unroll
-    for (int i = 0; i < 8; i++) w[i] = fma_f2(s, v[i], w[i]);
+    for (int i = 0; i < 8; i++) v[i] = mul_f2(v[i], s);
+    if (gate) tile_gate(a, gate, t, v);
+    raw_floats(y, w);
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = fma_f2(v[i], x.f[i], w[i]);
     raw_round(w, y);
 }
 
