@@ -2,7 +2,8 @@
 (fp8.quantize_blocks, fp8.swiglu_quantize, gemm.gemm_fp8_blocks, norm.*).
 
 Misuse that is visible on the host raises ValueError before the call; what
-the library refuses raises _lib.RengError.
+the library refuses raises _lib.RengError.  Inference only: what they return
+carries no gradient.
 """
 import torch
 

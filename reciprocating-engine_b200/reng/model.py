@@ -172,6 +172,8 @@ class Engine:
         desc.attn_scale = cfg.attention_scale()
         desc.has_qkv_bias = 1 if with_bias else 0
         desc.qk_norm = 1 if qk else 0
+        if fp8 is not None and fp8[1] == "blocks" and fp8[0] != "e4m3":
+            raise ValueError("block-scaled weights are e4m3, not %s" % fp8[0])
         if fp8 is None:
             desc.weights = _lib.RENG_WEIGHTS_BF16
         else:  # (format, scheme): per-channel weight-only, or blocks with 8-bit activations

@@ -29,9 +29,9 @@ class CachePlan:
     batch: int
     weight_bytes: int
     q_dim: int = 0       # query width (heads x head_dim); 0: the hidden size
-    eight_bit: bool = False  # 8-bit activations (fp8_blocks): their work buffers
     device_bytes: int = 183_359 * 1024 * 1024  # B200 HBM (nvidia-smi total)
     reserve_bytes: int = 2 << 30               # context, graphs, work buffers, allocator slack
+    eight_bit: bool = False                    # 8-bit activations (fp8_blocks): their work buffers
 
     @staticmethod
     def new(cfg, batch=1, weights="bf16", device_bytes=None, world=1):

@@ -155,7 +155,7 @@ def attention_oracle(cfg, w, ids, qk_norm, dev="cuda"):
         def n(t, g):
             return t / (t.square().mean(-1, keepdim=True) + cfg.rms_norm_eps).sqrt() * f32(lw[g], dev).double()
         q, k = n(q, "qn"), n(k, "kn")
-    sin, cos = (f32(t, dev).double().reshape(-1, hd)[:T] for t in rope_caches_for(cfg, 512))
+    sin, cos = (f32(t, dev).double().reshape(-1, hd)[:T] for t in rope_caches_for(cfg, T))
 
     def rot(t):
         return t * cos + torch.cat([-t[..., hd // 2:], t[..., :hd // 2]], -1) * sin
@@ -198,8 +198,8 @@ CASES = {
 }
 
 
-@pytest.mark.parametrize("T", [2, 9, 70, 300])
-@pytest.mark.parametrize("case", ["gqa", "wide", "small", "bias", "qk_norm"])
+@pytest.mark.parametrize("case,T", [(c, T) for c in ("gqa", "wide", "small", "bias", "qk_norm")
+                                    for T in (2, 9, 70, 300)] + [("gqa", 1100)])  # 1100: two blocks of rows
 def test_positions_and_attention(reng_lib, case, T):
     """A prompt's every row, and its last token as a decode step after the
     others, in a slot of its own among others."""
@@ -221,7 +221,7 @@ def test_positions_and_attention(reng_lib, case, T):
         err = (got - want[rows]).abs()
         assert bool((err <= bound[rows]).all()), "%d values off, worst %.3g of the bound" % (
             int((err > bound[rows]).sum()), float((err / bound[rows]).max()))
-    e = Engine(cfg, w, batch=3, capacity=512, fp8=BLOCKS)
+    e = Engine(cfg, w, batch=3, capacity=max(512, T + 1), fp8=BLOCKS)
     check(e.prefill(1, ids, all_logits=True)[2], slice(None))
     e.reset()
     short = max(1, T // 3)

@@ -476,5 +476,78 @@ def test_captured_replayed_and_on_another_stream(m):
         assert all(torch.equal(p, q) for p, q in zip(want2, out))
 
 
+def test_products_of_every_kind_at_once():
+    """Pairs of CTAs, K split over clusters, whole tiles and the few-row kernel
+    on streams of their own, beside norms that fill shared memory."""
+    from reng import gemm, norm
+    sizes = [(1001, 5120, 1024), (64, 4096, 2048), (100, 6144, 512), (8, 2048, 4096), (300, 2000, 700)]
+    sets = [operands(i, *mnk) for i, mnk in enumerate(sizes)]
+    x = activations(3, 500, 4096, BF16)
+    work = [lambda o=o: (gemm.gemm_fp8_blocks(*o, dtype=BF16),) for o in sets] + [lambda: norm.block_norm_fp8(x, x)]
+    want = [w() for w in work]
+    streams = [torch.cuda.Stream() for _ in work]
+    torch.cuda.synchronize()
+    got = [[] for _ in work]
+    for _ in range(10):
+        for i, (w, st) in enumerate(zip(work, streams)):
+            with torch.cuda.stream(st):
+                got[i].append(w())
+    torch.cuda.synchronize()
+    for ref, runs in zip(want, got):
+        assert all(torch.equal(a, b) for run in runs for a, b in zip(ref, run))
+
+
+def test_offsets_past_32_bits():
+    """Rows 2^30 and more elements apart."""
+    from reng import fp8, gemm, norm
+    pitch = (1 << 30) + 16
+    x = activations(1, 5, 1000, BF16)
+    far = torch.empty(4 * pitch + 1000, dtype=BF16, device="cuda").as_strided((5, 1000), (pitch, 1))
+    far.copy_(x)
+    for rows in (1, 128):
+        for a, b in zip(fp8.quantize_blocks(far, rows), fp8.quantize_blocks(x, rows)):
+            assert torch.equal(a, b)
+    both = far[:, :512]
+    for a, b in zip(fp8.swiglu_quantize(both), fp8.swiglu_quantize(x[:, :512].contiguous())):
+        assert torch.equal(a, b)
+    for n in (1000, 999):  # in pieces and by elements
+        for a, b in zip(norm.block_norm(far[:, :n], x[:, :n], gate=far[:, :n]),
+                        norm.block_norm(x[:, :n], x[:, :n], gate=x[:, :n])):
+            assert torch.equal(a, b)
+    del far, both
+    for m in (5, 40):  # the few-row kernel and the tensor core's
+        o = operands(2, m, 300, 256)
+        p = (1 << 31) // (m - 1) // 16 * 16 + 4096
+        c = torch.empty((m - 1) * p + 256, dtype=torch.uint8, device="cuda").as_strided((m, 256), (p, 1))
+        c.copy_(o[0])
+        y = torch.empty((m - 1) * p + 300, dtype=F32, device="cuda").as_strided((m, 300), (p, 1))
+        gemm.gemm_fp8_blocks(c, *o[1:], out=y)
+        assert torch.equal(y, gemm.gemm_fp8_blocks(*o, dtype=F32))
+        del c, y
+
+
+def test_python_refuses_wrong_device_matrices():
+    from reng import fp8, gemm, norm
+    x, sx, w, sw = operands(3, 4, 200, 256)
+    b = torch.zeros(4, 256, dtype=BF16, device="cuda")
+    bad = [
+        lambda: gemm.gemm_fp8_blocks(x, sx, w[:, :128], sw), lambda: gemm.gemm_fp8_blocks(x, sx[:, :1], w, sw),
+        lambda: gemm.gemm_fp8_blocks(x, sx, w, sw[:1]), lambda: gemm.gemm_fp8_blocks(x, sx.double(), w, sw),
+        lambda: gemm.gemm_fp8_blocks(x.view(torch.int8), sx, w, sw), lambda: gemm.gemm_fp8_blocks(x, sx, w.t(), sw),
+        lambda: gemm.gemm_fp8_blocks(x, sx, w, sw, dtype=torch.float16),
+        lambda: gemm.gemm_fp8_blocks(x, sx, w, sw, out=b), lambda: gemm.gemm_fp8_blocks(x.cpu(), sx, w, sw),
+        lambda: fp8.quantize_blocks(b, 64), lambda: fp8.quantize_blocks(b.half()), lambda: fp8.quantize_blocks(b.t()),
+        lambda: fp8.quantize_blocks(b, codes=x[:2]), lambda: fp8.swiglu_quantize(b[:, :255]),
+        lambda: fp8.quantize_blocks(b.expand(2, 4, 256)), lambda: fp8.quantize_blocks(b[:1].expand(4, 256)),
+        lambda: norm.block_norm(b, b[:2]), lambda: norm.block_norm(b, b, post_gain=torch.ones(255, device="cuda")),
+        lambda: norm.block_norm(b, b, gate=b[:, :255]), lambda: norm.block_norm(b, gate=b),
+        lambda: norm.block_norm(b, b, pre_gain=torch.ones(256)), lambda: norm.block_norm(b, b.half()),
+        lambda: norm.block_norm(b, b, out=b.float())]
+    for i, call in enumerate(bad):
+        with pytest.raises(ValueError):
+            call()
+            print("call %d was not refused" % i)
+
+
 def test_no_wait_ran_out(reng_lib):
     reng_lib.call("reng_gemm_fp8_blocks_status")

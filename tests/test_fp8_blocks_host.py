@@ -139,6 +139,16 @@ def test_the_quantize_tool_refuses_blocks():
     assert [plan_weights(f) for f in (None, ("e4m3", "pcs"), ("e4m3", "blocks"))] == ["bf16", "fp8", "fp8_blocks"]
 
 
+def test_blocks_of_another_format_are_refused():
+    from reng.config import LlamaConfig
+    from reng.model import Engine
+    from reng.weights import random_weights
+    cfg = LlamaConfig(hidden_size=64, intermediate_size=64, num_hidden_layers=1, num_attention_heads=4,
+                      num_key_value_heads=2, head_dim_=16, vocab_size=64)
+    with pytest.raises(ValueError, match="e4m3"):
+        Engine(cfg, random_weights(cfg), fp8=("e5m2", "blocks"))
+
+
 def test_the_commands_take_blocks():
     from reng import cli
     argv = ["m", "o", "2", "--fp8", "7"]
