@@ -60,16 +60,22 @@ def vector(t, name, n, dev):
     return t.data_ptr()
 
 
-def codes_empty(rows, cols, like):
+_empty = torch.empty
+
+
+def codes_empty(rows, cols, device):
     """uint8 [rows, cols] in rows of 16-byte pitch (as the product reads them), and the pitch."""
-    pitch = -(-cols // 16) * 16
-    t = torch.empty(rows, pitch, dtype=torch.uint8, device=like.device)
-    return (t if pitch == cols else t[:, :cols]), pitch
+    pitch = cols + 15 & -16
+    if pitch == cols:
+        return _empty(rows, cols, dtype=torch.uint8, device=device), cols
+    return _empty(rows, pitch, dtype=torch.uint8, device=device)[:, :cols], pitch
 
 
-try:  # the handle without building a Stream object around it
-    from torch._C import _cuda_getCurrentRawStream as _raw_stream
+try:  # the handle without building a Stream object around it, the device without an initialisation check
+    from torch._C import _cuda_getCurrentRawStream as _raw_stream, _cuda_getDevice as _current
 except ImportError:
+    _current = torch.cuda.current_device
+
     def _raw_stream(dev):
         return torch.cuda.current_stream(dev).cuda_stream
 
@@ -77,7 +83,7 @@ except ImportError:
 def call(dev, name, *args):
     """The library call on the device's current stream, with the device current."""
     f = getattr(_lib.lib(), name)
-    if dev == torch.cuda.current_device():
+    if dev == _current():
         rc = f(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
@@ -98,13 +104,14 @@ def on_stream(stream, like, run, *args):
 
 def blocks_out(x, dev, rows, cols, scale_rows, codes, scales):
     """Codes and scales of a block quantizer with their pitches, new where not given."""
+    device = x.device
     if codes is None:
-        codes, ldc = codes_empty(rows, cols, x)
+        codes, ldc = codes_empty(rows, cols, device)
     else:
         ldc = matrix(codes, "codes", U8, dev, rows, cols)
     if scales is None:
         lds = groups(cols)
-        scales = torch.empty(scale_rows, lds, dtype=torch.float32, device=x.device)
+        scales = _empty(scale_rows, lds, dtype=torch.float32, device=device)
     else:
         lds = matrix(scales, "scales", F32, dev, scale_rows, groups(cols))
     return codes, ldc, scales, lds
@@ -150,7 +157,7 @@ def gemm_fp8_blocks(x, x_scales, w, w_scales, out, dtype, x_fmt, w_fmt):
     ldsx = matrix(x_scales, "x_scales", F32, dev, M, kb)
     ldsw = matrix(w_scales, "w_scales", F32, dev, groups(N), kb)
     if out is None:
-        out = torch.empty(M, N, dtype=dtype or torch.bfloat16, device=x.device)
+        out = _empty(M, N, dtype=dtype or torch.bfloat16, device=x.device)
         ldy = N
     else:
         if dtype is not None and out.dtype != dtype:

@@ -271,6 +271,17 @@ def quantize_device(w, rows, cols, fmt, scaling, backoff=DEFAULT_BACKOFF, codes=
     return codes, scales, int(bias.value)
 
 
+_impl = None  # ._tensors, bound on first use (it needs torch; an import statement costs 0.6 us a call)
+
+
+def _tensors():
+    global _impl
+    if _impl is None:
+        from . import _tensors as m
+        _impl = m
+    return _impl
+
+
 def quantize_blocks(x, block_rows=1, fmt=Fp8Format.E4M3, codes=None, scales=None, stream=None):
     """Quantize a torch CUDA matrix [rows, cols] (bf16 or f32) to FP8 codes
     with one f32 scale per 1 x 128 group of a row (block_rows=1, activations)
@@ -280,20 +291,20 @@ def quantize_blocks(x, block_rows=1, fmt=Fp8Format.E4M3, codes=None, scales=None
     [ceil(rows / block_rows), ceil(cols / 128)]), the operands of
     gemm.gemm_fp8_blocks.  A block's scale is absmax / max_finite (1 for
     zeros) and its codes encode(x / scale) by the rules of quantize_with."""
-    from ._tensors import on_stream, quantize_blocks as run
+    t = _impl or _tensors()
     if stream is not None:
-        return on_stream(stream, x, run, x, block_rows, fmt, codes, scales)
-    return run(x, block_rows, fmt, codes, scales)
+        return t.on_stream(stream, x, t.quantize_blocks, x, block_rows, fmt, codes, scales)
+    return t.quantize_blocks(x, block_rows, fmt, codes, scales)
 
 
 def swiglu_quantize(gate_up, fmt=Fp8Format.E4M3, codes=None, scales=None, stream=None):
     """quantize_blocks of h = silu(gate) * up in 1 x 128 groups, h in f32:
     gate_up [rows, 2 * cols] (bf16 or f32) holds the gate columns, then the
     up columns.  Returns (codes uint8 [rows, cols], scales)."""
-    from ._tensors import on_stream, swiglu_quantize as run
+    t = _impl or _tensors()
     if stream is not None:
-        return on_stream(stream, gate_up, run, gate_up, fmt, codes, scales)
-    return run(gate_up, fmt, codes, scales)
+        return t.on_stream(stream, gate_up, t.swiglu_quantize, gate_up, fmt, codes, scales)
+    return t.swiglu_quantize(gate_up, fmt, codes, scales)
 
 
 # Rows per matrix the model-level pass measures its error on (FP8_ERROR_ROWS,

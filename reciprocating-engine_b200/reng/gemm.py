@@ -19,6 +19,16 @@ import numpy as np
 
 from . import _lib
 
+_impl = None  # ._tensors, bound on first use (it needs torch; an import statement costs 0.6 us a call)
+
+
+def _tensors():
+    global _impl
+    if _impl is None:
+        from . import _tensors as m
+        _impl = m
+    return _impl
+
 
 def gemm_bf16(w_bits, x_bits, splits=0, iters=0):
     w = np.ascontiguousarray(w_bits, dtype=np.uint16)
@@ -42,7 +52,7 @@ def gemm_fp8_blocks(x, x_scales, w, w_scales, out=None, dtype=None, x_fmt=_lib.R
     with scales [ceil(N / 128), ceil(K / 128)]; rows start on 16 bytes
     (fp8.quantize_blocks lays them out so).  y [M, N] is `out`, or a new
     tensor of `dtype` (bf16 by default, or f32)."""
-    from ._tensors import gemm_fp8_blocks as run, on_stream
+    t = _impl or _tensors()
     if stream is not None:
-        return on_stream(stream, x, run, x, x_scales, w, w_scales, out, dtype, x_fmt, w_fmt)
-    return run(x, x_scales, w, w_scales, out, dtype, x_fmt, w_fmt)
+        return t.on_stream(stream, x, t.gemm_fp8_blocks, x, x_scales, w, w_scales, out, dtype, x_fmt, w_fmt)
+    return t.gemm_fp8_blocks(x, x_scales, w, w_scales, out, dtype, x_fmt, w_fmt)
