@@ -32,10 +32,11 @@
 //   * The last round of tiles over the SMs is rarely full: it takes narrower
 //     tiles than the rounds before it (1001 x 5120 x 27648: 166 us in tiles of
 //     192 columns, 154 in 18 of 256 and 8 of 64; 5789 x 909 x 4011 64 and 50).
-//   * Few tiles (decode): K is split over the CTAs of a cluster, each leaves
-//     its f32 partial in its own shared memory and all of them add a share of
-//     the columns in rank order over distributed shared memory, so the result
-//     does not depend on arrival order and no workspace is needed.
+//   * Few tiles (decode): K is split over the CTAs of a cluster.  Each CTA owns
+//     a share of the columns; all of them write their f32 partials of it into
+//     its shared memory (stores to a peer do not wait, loads from one take a
+//     microsecond), and it adds them in rank order, so the result does not
+//     depend on arrival order and no workspace is needed.
 // Every wait is bounded (tc.cuh); one that runs out records RENG_E_TIMEOUT in
 // a device word, and the call's results are invalid.
 #include <cooperative_groups.h>
@@ -70,7 +71,6 @@ constexpr int kBK = 128;         // k of a block: one swizzled row of 8-bit code
 constexpr int kMaxBn = 256;      // TMEM columns of a buffer; two buffers fill TMEM
 constexpr int kMaxStages = 12;
 constexpr int kMaxSplit = 4;     // K splits of a tile (CTAs of a cluster): 1, 2 or 4
-constexpr int kPartRows = 132;   // a split's partial: rows of a column, padded
 constexpr int kThreads = 384;    // a warpgroup of roles, two of accumulators
 constexpr int kAccWarps = 8;
 // an accumulator warp's staging for its output: 32 rows of 16 columns, 17
@@ -388,42 +388,69 @@ __device__ __forceinline__ void cta_end() {
     else __syncthreads();
 }
 
-// The sum of a cluster's partials of one tile, in rank order: CTA `rank` adds
-// the columns from rank * share on.  An accumulator thread takes 4 rows of one
-// column at a time, two such items and all ranks' reads in flight, since a
-// read of a peer's shared memory takes about a microsecond.
-__device__ __forceinline__ void add_partials(const Fp8Gemm& a, float* part, int m0, int n0, int rank) {
-    cooperative_groups::cluster_group cluster = cooperative_groups::this_cluster();
-    const int rows = min(kRows, a.M - m0), cols = min(a.bn, a.N - n0);
-    const int share = (cols + a.ks - 1) / a.ks, c0 = rank * share, nc = min(share, cols - c0);
-    const int items = nc > 0 ? (rows + 3) / 4 * nc : 0;
-    for (int i = threadIdx.x - (kThreads - 32 * kAccWarps); i < items; i += 2 * 32 * kAccWarps) {
-        float4 v[2][kMaxSplit];
-        int c[2], row[2];
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
+
+// Partials of a K split: [rank of the writer][column of the owner][row].  A
+// warp's 32 rows lie together, so a store to a peer is one piece of 128 bytes
+// (as 32 pieces of 8 bytes a split by 4 took 9 us); a column is mbox + 1 long,
+// so 32 columns of one row are read from as many banks.
+//
+// A thread's accumulators (row r of the tile, columns c0 .. c0 + cw - 1) into
+// the shared memory of the CTAs that own the columns.
+__device__ __forceinline__ void push_partials(const Fp8Gemm& a, uint32_t part, int rank, int r, int c0, int cw,
+                                              const unsigned long long (&acc)[64]) {
+    const int share = a.bn / a.ks, first = c0 / share;
+    const uint32_t pitch = 4u * (uint32_t)(a.mbox + 1), mine = part + (uint32_t)(rank * share) * pitch + 4u * (uint32_t)r;
+    int q = first, left = share - (c0 - first * share);
+    uint32_t to = (q == rank ? mine : map_cta(mine, q)) + (uint32_t)(share - left) * pitch;
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            const int j = i + u * 32 * kAccWarps;
-            row[u] = j < items ? j / nc * 4 : rows;
-            c[u] = c0 + j % nc;
-#pragma unroll
-            for (int q = 0; q < kMaxSplit; q++)
-                if (q < a.ks && j < items)
-                    v[u][q] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&part[c[u] * kPartRows + row[u]], q));
+    for (int i = 0; i < 64; i++) {
+        if (2 * i >= cw) break;
+        float lo, hi;
+        unpair2(acc[i], lo, hi);
+        if (q == rank) {  // its own share
+            sts_f(to, lo);
+            sts_f(to + pitch, hi);
+        } else {
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to), "f"(lo) : "memory");
+            asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(to + pitch), "f"(hi) : "memory");
         }
+        to += 2 * pitch, left -= 2;
+        if (left == 0) {
+            q = min(q + 1, a.ks - 1), left = share;
+            to = q == rank ? mine : map_cta(mine, q);
+        }
+    }
+}
+
+// This CTA's share of a tile from the partials that all CTAs wrote here, in
+// rank order: a warp a row, a lane a column, four rows in flight.
+template <int KS>
+__device__ __forceinline__ void add_partials(const Fp8Gemm& a, uint32_t part, int m0, int n0, int rank) {
+    constexpr int kAcross = 4;
+    const int share = a.bn / KS, rows = min(kRows, a.M - m0), cols = min(share, a.N - n0 - rank * share);
+    const int warp = (int)(threadIdx.x >> 5) - (kThreads / 32 - kAccWarps);
+    const uint32_t pitch = 4u * (uint32_t)(a.mbox + 1), step = (uint32_t)share * pitch;
+    for (int c = threadIdx.x & 31; c < cols; c += 32) {
+        const uint32_t from = part + (uint32_t)c * pitch;
+        for (int r0 = warp; r0 < rows; r0 += kAcross * kAccWarps) {
+            float v[kAcross][KS];
 #pragma unroll
-        for (int u = 0; u < 2; u++) {
-            float s[4] = {0.f, 0.f, 0.f, 0.f};
-            if (row[u] < rows) {
+            for (int i = 0; i < kAcross; i++)
 #pragma unroll
-                for (int q = 0; q < kMaxSplit; q++)
-                    if (q < a.ks) s[0] += v[u][q].x, s[1] += v[u][q].y, s[2] += v[u][q].z, s[3] += v[u][q].w;
-            }
+                for (int q = 0; q < KS; q++)  // past the last row: the last one's again, not written
+                    v[i][q] = lds_f(from + q * step + 4u * (uint32_t)min(r0 + i * kAccWarps, rows - 1));
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                if (row[u] + e >= rows) break;
-                const size_t to = (size_t)(m0 + row[u] + e) * a.ldy + n0 + c[u];
-                if (a.y_f32) static_cast<float*>(a.y)[to] = s[e];
-                else static_cast<uint16_t*>(a.y)[to] = (uint16_t)bf16x2(s[e], 0.f);
+            for (int i = 0; i < kAcross; i++) {
+                const int row = r0 + i * kAccWarps;
+                if (row >= rows) break;
+                float sum = v[i][0];
+#pragma unroll
+                for (int q = 1; q < KS; q++) sum += v[i][q];
+                const size_t to = (size_t)(m0 + row) * a.ldy + n0 + rank * share + c;
+                if (a.y_f32) static_cast<float*>(a.y)[to] = sum;
+                else static_cast<uint16_t*>(a.y)[to] = (uint16_t)bf16x2(sum, 0.f);
             }
         }
     }
@@ -445,12 +472,14 @@ __global__ void __launch_bounds__(kThreads, 1)
     // x stages first: the MMA reads 128 rows from each, past a shorter box
     // into what follows, and the lanes of those rows are never used
     const uint32_t sA = smem0, sB = sA + (uint32_t)a.stages * abytes, sOut = sB + (uint32_t)a.stages * bbytes,
-                   sScale = sOut + kAccWarps * (PAIR ? kStageOutPair : kStageOut);  // 16-byte aligned
+                   sScale = sOut + kAccWarps * (PAIR ? kStageOutPair : kStageOut),  // 16-byte aligned
+                   sPart = sScale + kScaleSlots * kScaleSlot;
     const uint32_t bar0 = (uint32_t)__cvta_generic_to_shared(bars);
     auto bar = [bar0](int first, int i = 0) { return bar0 + 8u * (uint32_t)(first + i); };
     const bool clustered = PAIR || a.ks > 1;
     const int rank = clustered ? (int)cg::this_cluster().block_rank() : 0;
     int* const err = a.err ? a.err : &g_fp8_gemm_err;
+    if (!PAIR && a.ks > 1) cluster_arrive();  // this CTA runs: its shared memory can be written
 
     if (threadIdx.x == 0) {
         for (int s = 0; s < a.stages; s++) {
@@ -614,6 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         }
         // the end of the CTA, said by each side of the register hand-over for
         // itself: no code after it is shared
+        if (!PAIR && a.ks > 1) cluster_wait();
         cta_end<PAIR>();
         if (warp == 1) {
             asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
@@ -622,9 +652,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             else
                 asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem) : "memory");
         }
-        if (!PAIR && a.ks > 1) {
-            cg::this_cluster().sync();  // the partials are complete (TMEM is already free: a CTA
-            cg::this_cluster().sync();  // that waits for its peers here holds none), and read
+        if (!PAIR && a.ks > 1) {  // TMEM is already free: a CTA that waits for its peers here holds none
+            cluster_arrive();
+            cluster_wait();
         }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kRegsAcc));
@@ -632,6 +662,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int r = 32 * (warp & 3) + lane;
         const uint32_t out0 = sOut + (uint32_t)(warp - 4) * (PAIR ? kStageOutPair : kStageOut);
         uint32_t box = 0;  // staging box of the next output copy
+        bool pushed = false;
         AccState st;
         st.bar0 = bar0;
         st.sx = sScale + 16 * r;
@@ -656,18 +687,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             add_tile<PAIR>(st, any ? cw / 32 : 0, edge < cw, k0, k1, edge, acc);
             if (!any) continue;
             if (!PAIR && a.ks > 1) {
-                // partial[column][row], columns kPartRows apart: conflict-free
-                // both ways, and 4 rows of a column are one 16-byte read
-                float* part = reinterpret_cast<float*>(smem_raw + (smem0 - (uint32_t)__cvta_generic_to_shared(smem_raw)));
-#pragma unroll
-                for (int c = 0; c < 64; c++) {
-                    float lo, hi;
-                    unpair2(acc[c], lo, hi);
-                    if (2 * c < cw) {
-                        part[(c0 + 2 * c) * kPartRows + r] = lo;
-                        part[(c0 + 2 * c + 1) * kPartRows + r] = hi;
-                    }
-                }
+                pushed = true;
+                cluster_wait();  // all CTAs of the cluster run
+                if (r < a.M - at.mi * kRows) push_partials(a, sPart, rank, r, c0, cw, acc);
             } else if (PAIR && a.y_tma) {
                 // 32 rows x 32 columns at a time through this warp's staging
                 // in the copy's swizzle; the copies run on behind the next tile
@@ -762,13 +784,14 @@ __global__ void __launch_bounds__(kThreads, 1)
         // the staging is read before the CTA's shared memory goes away
         if (PAIR && lane == 0) s2g_wait_read<0>();
         __syncwarp();
+        if (!PAIR && a.ks > 1 && !pushed) cluster_wait();
         cta_end<PAIR>();
         if (!PAIR && a.ks > 1) {
-            cg::this_cluster().sync();
+            cluster_arrive();
+            cluster_wait();  // all partials are here
             const TileAt at = tile_at(a, first);
-            add_partials(a, reinterpret_cast<float*>(smem_raw + (smem0 - (uint32_t)__cvta_generic_to_shared(smem_raw))),
-                         at.mi * kRows, at.n0, rank);
-            cg::this_cluster().sync();  // this CTA's partial stays until its peers have read it
+            if (a.ks == 2) add_partials<2>(a, sPart, at.mi * kRows, at.n0, rank);
+            else add_partials<4>(a, sPart, at.mi * kRows, at.n0, rank);
         }
     }
 }
@@ -823,17 +846,23 @@ int y_map(void* y, bool f32, int64_t M, int64_t N, int64_t ldy, CUtensorMap* out
 
 constexpr size_t kSmemMax = 227 * 1024 - 1024;  // dynamic shared memory of a CTA, beside its barriers
 
+// Shared memory beside the pipeline's stages: the output's staging, the scales
+// and (ks > 1) the partials.
+size_t smem_beside(bool pair, int mbox, int bn, int ks) {
+    return (size_t)kAccWarps * (pair ? kStageOutPair : kStageOut) + kScaleSlots * kScaleSlot +
+           (ks > 1 ? (size_t)bn * (mbox + 1) * 4 : 0);
+}
+
 template <bool PAIR>
 int launch_tiles(const CUtensorMap& xm, const CUtensorMap& wm, const CUtensorMap& wm2, const CUtensorMap& ym, Fp8Gemm& a,
                  int grid, cudaStream_t st) {
     const int brows = PAIR ? a.bn / 2 : a.bn;
-    const size_t stage = (size_t)(a.mbox + brows) * kBK, out = (size_t)kAccWarps * (PAIR ? kStageOutPair : kStageOut) + kScaleSlots * kScaleSlot;
+    const size_t stage = (size_t)(a.mbox + brows) * kBK, out = smem_beside(PAIR, a.mbox, a.bn, a.ks);
     const int steps = (int)(((long long)a.mt * a.nt * (PAIR ? 2 : a.ks) + grid - 1) / grid) * ((a.kb + a.ks - 1) / a.ks);
     a.stages = (int)std::min<size_t>({(size_t)kMaxStages, (kSmemMax - 1024 - out) / stage, (size_t)std::max(steps, 2)});
     size_t smem = 1024 + a.stages * stage + out;
-    // the last x stage is read 128 rows deep; a split leaves its partial
+    // the last x stage is read 128 rows deep
     smem = std::max(smem, (size_t)1024 + (size_t)(a.stages - 1) * a.mbox * kBK + kRows * kBK);
-    if (a.ks > 1) smem = std::max(smem, (size_t)1024 + (size_t)a.bn * kPartRows * 4);
     // a pair holds TMEM on two SMs while its CTAs wait for one another: it
     // takes all of their shared memory, so that no CTA of another launch that
     // does the same can sit beside one of them and wait the other way round
@@ -868,9 +897,11 @@ int launch_tiles(const CUtensorMap& xm, const CUtensorMap& wm, const CUtensorMap
 // 357 + 2.1 bn cycles in one CTA and 315 + 2.13 bn in a pair, bn rounded up to
 // 64 (the MMAs' own 2 bn and the issuing warp's waits, which they do not
 // cover), and no less than its bytes at 64 a cycle from L2 and 23 from HBM
-// when all SMs stream; a tile has a fixed cost, and a split's exchange 4000 +
-// 50 bn (64 rows x 4096 x 14336: 20.4 us split by 4 against 34 whole; clusters
-// of 3 and of 5 to 8 leave SMs of a GPC empty and took twice as long).
+// when all SMs stream; a tile has a fixed cost, and a split 6000 (its barriers
+// and additions, and what its clusters cost the launches around them) and a
+// cycle for each 8 of the bytes that go to peers (64 rows x 4096 x 14336: 18.2
+// us split by 4 against 34 whole; clusters of 3 and of 5 to 8 leave SMs of a
+// GPC empty and took twice as long).
 struct Plan {
     bool pair;
     int bn, ks;
@@ -900,8 +931,11 @@ Plan plan(int M, int N, int kb, int sms) {
                 const long long tiles = (long long)mt * ((N + bn - 1) / bn) * ks;
                 const long long rounds = (tiles + slots - 1) / slots;
                 if (ks > 1 && rounds > 1) continue;
+                const int mbox = std::min(kRows, (M + 7) / 8 * 8);
+                if (ks > 1 && smem_beside(false, mbox, bn, ks) + 3 * (size_t)(mbox + bn) * kBK > kSmemMax - 1024) continue;
                 const int blocks = (kb + ks - 1) / ks;
-                const double cost = rounds * (blocks * block(bn, tiles, rounds, blocks) + fixed + (ks > 1 ? 4000.0 + 50.0 * bn : 0.0));
+                const double exchange = ks > 1 ? 6000.0 + 0.5 * std::min(M, kRows) * bn * (ks - 1) / ks : 0.0;
+                const double cost = rounds * (blocks * block(bn, tiles, rounds, blocks) + fixed + exchange);
                 if (cost < best.cost) best = {pair != 0, bn, ks, 0, 0, cost};
                 if (bn <= 32) break;
             }
