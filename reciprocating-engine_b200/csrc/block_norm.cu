@@ -85,8 +85,14 @@ struct Team {
     }
 };
 
-// 1 / sqrt(sum / n + eps): the hardware's root is within 2 steps.
-__device__ __forceinline__ float inv_rms(float sum, const NormArgs& a) { return rsqrtf(fmaf(sum, a.inv_n, a.eps)); }
+// 1 / sqrt(sum / n + eps).  The hardware's root is within 2 steps, which would
+// move a whole row of y over its bf16 borders; one Newton step r + r (1 - x r^2) / 2
+// with the residual formed exactly leaves half a step.
+__device__ __forceinline__ float inv_rms(float sum, const NormArgs& a) {
+    const float x = fmaf(sum, a.inv_n, a.eps), r = rsqrtf(x), t = x * r;
+    const float e = fmaf(-fmaf(x, r, -t), r, fmaf(-t, r, 1.f)), n = fmaf(0.5f * r, e, r);
+    return n == n ? n : r;  // x of 0 or infinity: the limits
+}
 
 // The 4 groups of a warp tile of one row: the first column of the lane's
 // values in each of its groups.

@@ -8,7 +8,7 @@
 // (g, q) takes 16 consecutive bytes of row g at 16 q and hands them to the
 // MMAs as the k its fragments name; the token rows are read the same way.
 // That makes every load 16 bytes wide with no staging, no barrier and no TMEM
-// round trip per block (which costs the tcgen05 form some 600 cycles a block,
+// round trip per block (which costs the tcgen05 form some 470 cycles a block,
 // whatever its width).
 // One CTA owns 16 weight rows; its 8 warps split K and add their partials in
 // warp order through shared memory, so the result is deterministic.  A warp
