@@ -62,8 +62,9 @@ namespace {
 
 // Weight elements up to which gemv_fp8.cu runs calls of at most 8, and of 9 to
 // 16, token rows.  Measured on B200 (us, that kernel against this one): 8 rows
-// 6144 x 4096 7.1 / 12.3, 4096 x 14336 13.0 / 17.2, 28672 x 4096 27.2 / 22.9;
-// 16 rows 6144 x 4096 11.6 / 13.2, 28672 x 4096 44.7 / 23.2.
+// 6144 x 4096 7.2 / 11.3, 4096 x 14336 13.5 / 17.9, 28672 x 4096 27.2 / 22.9;
+// 16 rows 4096 x 4096 7.5 / 9.5, 6144 x 4096 10.7 / 11.3, 28672 x 4096 44.7 /
+// 23.2 (8192 x 2048 9.2 / 7.9: the shape counts too, by less).
 constexpr int64_t kGemvElems[2] = {(int64_t)1 << 26, (int64_t)1 << 25};
 
 constexpr int kRows = 128;       // token rows of a CTA (one TMEM lane each)
