@@ -228,8 +228,7 @@ __device__ __forceinline__ void tile_emit_fp8(const NormArgs& a, int64_t row, co
     float m[G], s[G], r[G];
     bool odd;
     tile_absmax(h, m, odd);
-    group_max(m);
-    tile_scales<FMT>(m, s, r);
+    tile_scales<FMT>(group_max(m), s, r);
     uint32_t w[4];
     tile_codes<FMT>(h, s, r, odd, w);
     uint8_t* dst = static_cast<uint8_t*>(a.h) + row * a.ldh;

@@ -135,8 +135,7 @@ __global__ void __launch_bounds__(256, 4) k_fp8_groups(GroupArgs a) {
     float m[G], s[G], r[G];
     bool odd;
     tile_absmax(v, m, odd);
-    group_max(m);
-    tile_scales<FMT>(m, s, r);
+    tile_scales<FMT>(group_max(m), s, r);
     uint32_t w[4];
     tile_codes<FMT>(v, s, r, odd, w);
 #pragma unroll

@@ -193,24 +193,29 @@ __device__ __forceinline__ float absmax_nan(float m, float x, float y) {
     return r;
 }
 
-// Maximum over a group's lanes (8 G of them) of each group's value.
+// Maximum over a group's lanes (8 G of them): a lane's is that of its group
+// lane % G.  Where a lane holds several groups it hands away half of them at a
+// step, so four groups take 6 shuffles and not 20.
 template <int G>
-__device__ __forceinline__ void group_max(float (&m)[G]) {
+__device__ __forceinline__ float group_max(const float (&m)[G]) {
+    const bool b0 = threadIdx.x & 1, b1 = threadIdx.x & 2;
+    auto merge = [](bool upper, float lo, float hi, int o) {
+        return fmaxf(upper ? hi : lo, __shfl_xor_sync(0xffffffffu, upper ? lo : hi, o));
+    };
+    float v = m[0];
+    if constexpr (G == 2) v = merge(b0, m[0], m[1], 1);
+    if constexpr (G == 4) v = merge(b1, merge(b0, m[0], m[1], 1), merge(b0, m[2], m[3], 1), 2);
 #pragma unroll
-    for (int o = 4 * G; o > 0; o >>= 1)
-#pragma unroll
-        for (int g = 0; g < G; g++) m[g] = fmaxf(m[g], __shfl_xor_sync(0xffffffffu, m[g], o));
+    for (int o = 4 * G; o >= G; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
+    return v;
 }
 
-// The scales of a lane's groups and their reciprocals, rounded to nearest.
-// The lanes of a group share the work: each forms one of their G (a division
-// and a reciprocal take some 30 instructions).
+// The scales of a lane's groups and their reciprocals, rounded to nearest,
+// from group_max's answer: each lane forms those of one group (a division and
+// a reciprocal take some 30 instructions).
 template <int FMT, int G>
-__device__ __forceinline__ void tile_scales(const float (&m)[G], float (&s)[G], float (&r)[G]) {
-    const int lane = threadIdx.x & 31, mine = lane & (G - 1);
-    float own = m[0];
-#pragma unroll
-    for (int g = 1; g < G; g++) own = mine == g ? m[g] : own;
+__device__ __forceinline__ void tile_scales(float own, float (&s)[G], float (&r)[G]) {
+    const int lane = threadIdx.x & 31;
     const float sc = fp8_block_scale<FMT>(own), rc = __frcp_rn(sc);
 #pragma unroll
     for (int g = 0; g < G; g++) {
