@@ -10,9 +10,13 @@
 // That makes every load 16 bytes wide with no staging, no barrier and no TMEM
 // round trip per block (which costs the tcgen05 form some 470 cycles a block,
 // whatever its width).
-// One CTA owns 16 weight rows; its 8 warps split K and add their partials in
-// warp order through shared memory, so the result is deterministic.  A warp
-// keeps three blocks (6 KB) in flight, two CTAs an SM.
+// One CTA owns 16 weight rows; its warps split K and add their partials in
+// warp order through shared memory, so the result is deterministic.  8 warps
+// with three blocks (6 KB) each in flight, two CTAs an SM (one above 8 token
+// rows); or 4 warps with four blocks, three (two) CTAs, where those hold all
+// CTAs of a launch at once and the former do not (us, 8 and 4 warps: 1 row
+// 6144 x 4096 8.1 / 6.9, 5120 x 5120 9.0 / 7.9, but 4096 x 4096 5.4 / 6.2, 8192
+// x 4096 9.6 / 10.8; 16 rows 4096 x 4096 8.8 / 7.9, but 5120 x 5120 13.6 / 14.5).
 #include <algorithm>
 #include <string>
 
@@ -23,8 +27,9 @@ namespace reng {
 namespace {
 
 constexpr int kTile = 16;   // weight rows of a CTA
-constexpr int kWarps = 8;   // K splits of a CTA
-constexpr int kAhead = 3;   // blocks of a warp in flight
+// K splits of a CTA (its warps: 8 or 4), a warp's blocks in flight, CTAs of an SM
+constexpr int ahead(int warps) { return warps == 8 ? 3 : 4; }
+constexpr int ctas(int warps, int mt) { return (warps == 8 ? 2 : 3) - (mt == 1 ? 0 : 1); }
 
 struct Gemv8Args {
     const uint8_t *x, *w;
@@ -75,8 +80,9 @@ struct Block {
     float sw, sx[MT][2];
 };
 
-template <int MT, int XF, int WF, bool RAGGED>
-__global__ void __launch_bounds__(32 * kWarps, MT == 1 ? 2 : 1) k_gemv_fp8(const Gemv8Args a) {
+template <int MT, int XF, int WF, bool RAGGED, int kWarps>
+__global__ void __launch_bounds__(32 * kWarps, ctas(kWarps, MT)) k_gemv_fp8(const Gemv8Args a) {
+    constexpr int kAhead = ahead(kWarps);
     __shared__ float red[kWarps][MT * 8][kTile + 1];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, q = lane & 3;
     const int n0 = blockIdx.x * kTile;
@@ -161,15 +167,26 @@ __global__ void __launch_bounds__(32 * kWarps, MT == 1 ? 2 : 1) k_gemv_fp8(const
     }
 }
 
-template <int MT, bool RAGGED>
-cudaError_t launch(const Gemv8Args& a, int x_fmt, int w_fmt, cudaStream_t st) {
-    const dim3 grid((unsigned)((a.N + kTile - 1) / kTile)), block(32 * kWarps);
+template <int MT, bool RAGGED, int W>
+cudaError_t launch_warps(const Gemv8Args& a, unsigned tiles, int x_fmt, int w_fmt, cudaStream_t st) {
+    const dim3 grid(tiles), block(32 * W);
     constexpr int E4 = RENG_FP8_E4M3, E5 = RENG_FP8_E5M2;
     if (w_fmt == E4)
-        return x_fmt == E4 ? launch_ops(k_gemv_fp8<MT, E4, E4, RAGGED>, grid, block, 0, st, a)
-                           : launch_ops(k_gemv_fp8<MT, E5, E4, RAGGED>, grid, block, 0, st, a);
-    return x_fmt == E4 ? launch_ops(k_gemv_fp8<MT, E4, E5, RAGGED>, grid, block, 0, st, a)
-                       : launch_ops(k_gemv_fp8<MT, E5, E5, RAGGED>, grid, block, 0, st, a);
+        return x_fmt == E4 ? launch_ops(k_gemv_fp8<MT, E4, E4, RAGGED, W>, grid, block, 0, st, a)
+                           : launch_ops(k_gemv_fp8<MT, E5, E4, RAGGED, W>, grid, block, 0, st, a);
+    return x_fmt == E4 ? launch_ops(k_gemv_fp8<MT, E4, E5, RAGGED, W>, grid, block, 0, st, a)
+                       : launch_ops(k_gemv_fp8<MT, E5, E5, RAGGED, W>, grid, block, 0, st, a);
+}
+
+template <int MT, bool RAGGED>
+cudaError_t launch(const Gemv8Args& a, int x_fmt, int w_fmt, cudaStream_t st) {
+    int sms = 0;
+    const cudaError_t e = current_sms(&sms);
+    if (e != cudaSuccess) return e;
+    const int tiles = (a.N + kTile - 1) / kTile;
+    return tiles > ctas(8, MT) * sms && tiles <= ctas(4, MT) * sms
+               ? launch_warps<MT, RAGGED, 4>(a, (unsigned)tiles, x_fmt, w_fmt, st)
+               : launch_warps<MT, RAGGED, 8>(a, (unsigned)tiles, x_fmt, w_fmt, st);
 }
 
 }  // namespace

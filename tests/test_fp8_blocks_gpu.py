@@ -174,6 +174,15 @@ def test_zeros_and_small_values_keep_their_sign(cols, fmt, block_rows):
         assert torch.equal(codes[:, 1:128], neg[:, 1:128]) and bool((codes[:, 128:] & 0x7F == 0).all())
 
 
+@pytest.mark.parametrize("m,n,k", [(1, 6144, 512), (8, 5120, 777), (3, 4737, 384), (16, 4096, 640), (11, 2370, 200)])
+def test_product_of_few_rows_in_small_ctas(m, n, k):
+    """Widths between two sizes of a launch, which 4 warps a CTA hold at once."""
+    from reng import gemm
+    ops = operands(m + n + k, m, n, k)
+    for dtype in (BF16, F32):
+        check_product(gemm.gemm_fp8_blocks(*ops, dtype=dtype), *ops)
+
+
 @pytest.mark.parametrize("xf,wf", [(0, 1), (1, 0), (1, 1)])
 @pytest.mark.parametrize("m,n,k", [(5, 200, 700), (300, 2000, 300), (1024, 6144, 256)])
 def test_product_formats(m, n, k, xf, wf):
