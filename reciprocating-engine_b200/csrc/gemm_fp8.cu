@@ -49,6 +49,7 @@
 
 #include "fp8_encode.cuh"
 #include "ops.cuh"
+#include "ring.h"
 #include "tc.cuh"
 
 namespace reng {
@@ -528,8 +529,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         bool bad = false;
         if (warp == 0) {
             // ---- copies of the operands' codes ----
-            int s = 0, issued = 0;
-            uint32_t ph = 0;
+            Ring ring(a.stages);
             for (long long t = first; t < tiles && !bad; t += tstep) {
                 const TileAt at = tile_at(a, t);
                 const int m0 = at.mi * kTileRows_ + (PAIR ? rank * kRows : 0);
@@ -537,8 +537,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const int n0 = at.n0 + (PAIR ? rank * (int)nrows : 0);
                 const CUtensorMap* wm = at.bn == a.bn ? &wmap : &wmap2;
                 for (int b = k0; b < k1; b++) {
-                    if (issued >= a.stages) {
-                        wait(bar(B_EMPTY, s), ph ^ 1u, bad);
+                    const int s = ring.stage;
+                    if (ring.full()) {
+                        wait(bar(B_EMPTY, s), ring.phase ^ 1u, bad);
                         if (__any_sync(0xffffffffu, bad)) break;
                     }
                     const uint32_t xs = sA + (uint32_t)s * abytes, ws = sB + (uint32_t)s * bbytes;
@@ -555,21 +556,28 @@ __global__ void __launch_bounds__(kThreads, 1)
                             tensor_g2s(ws, wm, b * kBK, n0, bar(B_FULL, s));
                         }
                     }
-                    issued = issued < a.stages ? issued + 1 : issued;
-                    if (++s == a.stages) s = 0, ph ^= 1u;
+                    ring.fill();
                 }
                 bad = __any_sync(0xffffffffu, bad);
             }
-            if (bad) {
-                if (leader) atomicExch(err, RENG_E_TIMEOUT);
-                // the last copy into each stage lands before the CTA may exit
-                // (a pair's follower is kept by the cluster barrier at the end)
-                for (int i = 0; i < issued && (!PAIR || rank == 0); i++) {
-                    if (s == 0) s = a.stages, ph ^= 1u;
-                    s--;
-                    if (!__all_sync(0xffffffffu, bar_wait(bar(B_FULL, s), ph))) break;
-                }
-            }
+            // The last fills' arrivals of this kind, newest first, until one gives up.
+            auto landed = [&](int kind) {
+                Ring last = ring;
+                while (last.back())
+                    if (!__all_sync(0xffffffffu, bar_wait(bar(kind, last.stage), last.phase))) return false;
+                return true;
+            };
+            // After a wait that ran out the last copy into each stage lands
+            // before the CTA may exit (a pair's follower is kept by the
+            // cluster barrier at the end).
+            if (bad && (!PAIR || rank == 0)) landed(B_FULL);
+            // The last arrivals at EMPTY, which no refill waits for, come from
+            // the tensor core on its own time (in a pair's follower, from the
+            // leader's): they land before this shared memory may have another
+            // owner.  Hidden behind the last block's additions (64 x 4096 x
+            // 4096 10.0 us, 1001 x 5120 x 27648 148, as without it).
+            bad = !landed(B_EMPTY) || bad;
+            if (bad && leader) atomicExch(err, RENG_E_TIMEOUT);
         } else if (warp == 1 && (!PAIR || rank == 0)) {
             // ---- MMAs ----
             int s = 0, d = 0, used = 0;

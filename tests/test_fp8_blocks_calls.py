@@ -1,0 +1,31 @@
+"""The 8-bit block operators' host side and index arithmetic beyond the
+refusals of test_fp8_blocks_host.py (CPU only)."""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+from conftest import ROOT
+
+HERE = os.path.dirname(os.path.abspath(__file__))
+
+
+def run_check(tmp_path, name):
+    """Compile and run a harness over one of the kernels' headers."""
+    if shutil.which("g++") is None:
+        pytest.skip("no C++ compiler")
+    exe = str(tmp_path / name)
+    subprocess.run(["g++", "-O2", "-std=c++17", "-I", os.path.join(ROOT, "reciprocating-engine_b200", "csrc"),
+                    os.path.join(HERE, name + ".cc"), "-o", exe], check=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, r.stdout + r.stderr
+    return r.stdout
+
+
+def test_a_product_waits_for_the_last_arrivals_of_its_stages(tmp_path):
+    """The copy warp's closing waits name every used stage's last fill."""
+    assert " bad 0" in run_check(tmp_path, "ring_check")
+    src = open(os.path.join(ROOT, "reciprocating-engine_b200", "csrc", "gemm_fp8.cu")).read()
+    # both CTAs of a pair take the wait, before the barrier that ends them
+    assert 0 < src.index("landed(B_EMPTY)") < src.index("cta_end<PAIR>();")
