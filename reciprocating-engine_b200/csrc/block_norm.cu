@@ -19,6 +19,7 @@
 
 #include "fp8_encode.cuh"
 #include "ops.cuh"
+#include "row_image.h"
 
 namespace reng {
 namespace {
@@ -283,24 +284,36 @@ __device__ __forceinline__ void copy16(void* dst, const void* src) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src)
                  : "memory");
 }
+// The first `size` of N bytes; the others are zeros.
+template <int N>
+__device__ __forceinline__ void copy_part(void* dst, const void* src, int size) {
+    if (N == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+                     "r"(size)
+                     : "memory");
+    else
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"((uint32_t)__cvta_generic_to_shared(dst)), "l"(src),
+                     "r"(size)
+                     : "memory");
+}
 __device__ __forceinline__ void copy_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N>
 __device__ __forceinline__ void copy_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
 }
 
-// Bytes between a row's 16-byte boundary and its first element: its image in
-// shared memory keeps them, so that both sides of a copy are aligned whatever
-// the row's own alignment.
-__device__ __forceinline__ int lead(const void* row) { return (int)((uintptr_t)row & 15); }
-
-// A row's image: every 16-byte piece that holds some of its bytes (a piece
-// lies within one page, so the bytes beside the row can be read), spread over
-// n threads.
-__device__ __forceinline__ void copy_image(uint8_t* dst, const void* row, int bytes, int thread, int n) {
-    const char* src = static_cast<const char*>(row) - lead(row);
-    const int end = lead(row) + bytes;
-    for (int at = thread * 16; at < end; at += n * 16) copy16(dst + at, src + at);
+// A row's image (row_image.h): its whole pieces, spread over n threads, and
+// (one warp) its edges, but for an odd first element.
+__device__ __forceinline__ void copy_whole(uint8_t* dst, const void* row, int bytes, int thread, int n) {
+    const int lead = row_lead(row);
+    const char* src = static_cast<const char*>(row) - lead;
+    for (int at = 16 + thread * 16; at < row_whole(lead, bytes); at += n * 16) copy16(dst + at, src + at);
+}
+__device__ __forceinline__ void copy_edges(uint8_t* dst, const void* row, int bytes) {
+    const int lead = row_lead(row), lane = threadIdx.x & 31;
+    const char* src = static_cast<const char*>(row) - lead;
+    if (lane < 4) row_word(lead, bytes, lane, [&](int o, int size) { copy_part<4>(dst + o, src + o, size); });
+    if (lane == 4) row_rest(lead, bytes, [&](int o, int size) { copy_part<16>(dst + o, src + o, size); });
 }
 
 // The same of an aligned row, each lane copying what it will read itself.
@@ -338,6 +351,16 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 1) k_block_norm(const NormArgs
         return a.tg == RENG_TYPE_BF16 ? row_at<RENG_TYPE_BF16>(a.gate, at * a.ldg)
                                       : row_at<RENG_TYPE_F32>(a.gate, at * a.ldg);
     };
+    // By elements, the team's last warp (the one with the fewest columns) takes
+    // the edges of the rows; its lanes 0, 1 and 2 the odd first elements of the
+    // residual, the branch and the gate.
+    const int lane = threadIdx.x & 31;
+    const bool edges = team.warp == p.nw - 1;
+    auto stream = [&](int64_t at) -> const void* {
+        if (lane == 0) return row_at<TR>(a.residual, at * a.ldr);
+        if (lane == 1 && a.branch) return row_at<TB>(a.branch, at * a.ldb);
+        return lane == 2 && gated ? gate_row(at) : nullptr;
+    };
     auto copy = [&](int64_t at, uint8_t* slot) {
         if (at < a.rows) {
             const void *u = row_at<TB>(a.branch, at * a.ldb), *r = row_at<TR>(a.residual, at * a.ldr);
@@ -349,10 +372,14 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 1) k_block_norm(const NormArgs
                     else copy_own<RENG_TYPE_F32>(slot + p.gate, gate_row(at), t);
                 }
             } else {
-                const int thread = team.warp * 32 + (threadIdx.x & 31), n = 32 * p.nw;
-                copy_image(slot + p.residual, r, a.cols * kBytes<TR>, thread, n);
-                if (a.branch) copy_image(slot, u, a.cols * kBytes<TB>, thread, n);
-                if (gated) copy_image(slot + p.gate, gate_row(at), a.cols * (a.tg == RENG_TYPE_BF16 ? 2 : 4), thread, n);
+                const int thread = team.warp * 32 + lane, n = 32 * p.nw;
+                auto image = [&](int offset, const void* from, int bytes) {
+                    copy_whole(slot + offset, from, bytes, thread, n);
+                    if (edges) copy_edges(slot + offset, from, bytes);
+                };
+                image(p.residual, r, a.cols * kBytes<TR>);
+                if (a.branch) image(0, u, a.cols * kBytes<TB>);
+                if (gated) image(p.gate, gate_row(at), a.cols * (a.tg == RENG_TYPE_BF16 ? 2 : 4));
             }
         }
         copy_commit();
@@ -369,17 +396,26 @@ __global__ void __launch_bounds__(32 * kMaxWarps, 1) k_block_norm(const NormArgs
             copy_wait<kSlots - 1>();
         } else {  // pieces of other lanes: all of this row there, all reads of the last one done
             copy_wait<kSlots - 2>();
+            // an odd first element, whose sector is in L2 with the copies
+            // (carried in a register from the copies on it spilled)
+            if (edges) {
+                const void* from = stream(row);
+                const int lead = row_lead(from);
+                if (row_odd(lead))
+                    *reinterpret_cast<unsigned short*>(slot + (lane == 0 ? p.residual : lane == 1 ? 0 : p.gate) + lead) =
+                        *static_cast<const unsigned short*>(from);
+            }
             team.wait();
             copy(row + (kSlots - 1) * step, next);
         }
         Raw16<TB, G> u;
         Raw16<TR, G> y;
-        tile_load<true>(slot + p.residual + (G == 2 ? 0 : lead(row_at<TR>(a.residual, row * a.ldr))), t, a.cols, y);
+        tile_load<true>(slot + p.residual + (G == 2 ? 0 : row_lead(row_at<TR>(a.residual, row * a.ldr))), t, a.cols, y);
         if (a.branch) {
-            tile_load<true>(slot + (G == 2 ? 0 : lead(row_at<TB>(a.branch, row * a.ldb))), t, a.cols, u);
+            tile_load<true>(slot + (G == 2 ? 0 : row_lead(row_at<TB>(a.branch, row * a.ldb))), t, a.cols, u);
             float inv = 1.f;
             if (a.post) inv = inv_rms(team.sum(f2_sum(square_sum(u, 0ull)), red), a);
-            const void* gate = gated ? slot + p.gate + (G == 2 ? 0 : lead(gate_row(row))) : nullptr;
+            const void* gate = gated ? slot + p.gate + (G == 2 ? 0 : row_lead(gate_row(row))) : nullptr;
             tile_residual(a, x, gate, t, inv, u, y);
             tile_store(row_at<TR>(a.y, row * a.ldy), t, a.cols, y);
         }

@@ -29,3 +29,8 @@ def test_a_product_waits_for_the_last_arrivals_of_its_stages(tmp_path):
     src = open(os.path.join(ROOT, "reciprocating-engine_b200", "csrc", "gemm_fp8.cu")).read()
     # both CTAs of a pair take the wait, before the barrier that ends them
     assert 0 < src.index("landed(B_EMPTY)") < src.index("cta_end<PAIR>();")
+
+
+def test_a_norm_row_of_any_alignment_is_read_alone(tmp_path):
+    """Nothing beside a row is read, where another row may be written meanwhile or memory end."""
+    assert " bad 0" in run_check(tmp_path, "row_image_check")
