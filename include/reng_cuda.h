@@ -332,7 +332,9 @@ int reng_fp8_quantize_blocks(const void *x, int type, int64_t rows, int64_t cols
 
 /*
  * The same, in 1 x 128 groups, of h = gate / (1 + exp(-gate)) * up, computed
- * in f32 and rounded once, to the codes: the input of a down projection.
+ * in f32 and rounded once, to the codes: the input of a down projection.  h is
+ * formed as one value: where exp(-gate) leaves the f32 range and h does not,
+ * h is what counts.  A gate of -inf gives NaN.
  * gate and up are [rows, cols] with one row pitch ldx (the two halves of a
  * gate/up projection's output rows: up = gate + cols, ldx = 2 cols).
  */

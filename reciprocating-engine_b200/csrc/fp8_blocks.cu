@@ -31,45 +31,69 @@ struct GroupArgs {
     FastDiv per_row;  // of one row (of blocks)
 };
 
-// silu(g) u = g / (1 + exp(-g)) u for g whose exponential is out of the sum's
-// reach: g u, or the zero of the limit (NaN for g = -inf, which has none).
-__device__ __forceinline__ float swiglu_far(float g, float u) { return (g > 0.f ? g : g * 0.f) * u; }
+// exp(-g), or exp(g) 2^208 (FAR), by the hardware's ex2: 2^t with t = g log2(e)
+// in two parts, so that the rounding of t (which |g| magnifies) does not reach
+// the result: 2^(hi + lo) = 2^hi (1 + lo ln 2).
+template <bool FAR>
+__device__ __forceinline__ f2 exp_f2(f2 g) {
+    constexpr float s = FAR ? 1.f : -1.f;
+    const f2 hi = mul_f2(g, make_f2(s * 1.44269504f)), neg = mul_f2(hi, make_f2(-1.0f));
+    const f2 lo =
+        fma_f2(g, make_f2(s * 1.33497580e-8f), mul_f2(fma_f2(g, make_f2(s * 1.44269504f), neg), make_f2(0.693147181f)));
+    float e0, e1;
+    split_f2(FAR ? add_f2(hi, make_f2(208.f)) : hi, e0, e1);
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(e0));
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(e1));
+    const f2 e = make_f2(e0, e1);
+    return fma_f2(e, lo, e);
+}
 
-// v[i] = silu(v[i]) u[i].  exp(-g) is 2^t by the hardware's ex2, t = -g log2(e)
-// in two parts so that the rounding of t (which |g| magnifies) does not reach
-// the result: 2^(hi + lo) = 2^hi (1 + lo ln 2).  The quotient is rcp's,
-// corrected by its residual.  About 6 roundings in all.
+// silu(g) u where exp(-|g|) is nothing beside 1: g u, or g exp(g) u, which a
+// large u brings back into the f32 range though exp(g) has left it.  exp(g) is
+// taken 2^208 too large (the shift of hi is exact, and exp(-200) 2^208 still
+// normal; under -200 every product is below f32's smallest), half of that given
+// back by u first, so that nothing overflows, or loses bits that count, on the
+// way.  -inf, which has no limit, gives NaN.
+__device__ __forceinline__ f2 swiglu_far(f2 g, f2 u) {
+    float g0, g1, p0, p1, r0, r1;
+    split_f2(g, g0, g1);
+    const f2 w = mul_f2(g, exp_f2<true>(make_f2(fmaxf(g0, -300.f), fmaxf(g1, -300.f)))), half = make_f2(4.93038066e-32f);  // 2^-104
+    split_f2(mul_f2(g, u), p0, p1);
+    split_f2(mul_f2(mul_f2(mul_f2(u, half), w), half), r0, r1);
+    return make_f2(g0 < 0.f ? r0 : p0, g1 < 0.f ? r1 : p1);
+}
+
+// v[i] = silu(v[i]) u[i].  The quotient is rcp's, corrected by its residual.
+// About 6 roundings in all.  Where 1 + exp(-g) nears the end of the f32 range
+// (g from about -86.9 down, and infinities and NaN), a pair that some lane has
+// there is formed again by swiglu_far; activations have such gates in single
+// columns (a test for each pair, then: SwiGLU of 8192 x 14336 bf16 with a gate
+// of 87 in a quarter of its warp tiles 119 us, all pairs again 127, and 114
+// with the far products taken as zeros).
 __device__ __forceinline__ void swiglu(f2 (&v)[8], const f2 (&u)[8]) {
-    constexpr float kFar = 87.0f;  // 2^t stays normal below
     float top = 0.f;
     f2 h[8];
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const f2 g = v[i];
-        float g0, g1, e0, e1, d0, d1;
-        split_f2(g, g0, g1);
-        top = absmax_nan(top, g0, g1);
-        const f2 hi = mul_f2(g, make_f2(-1.44269504f));
-        const f2 neg = mul_f2(hi, make_f2(-1.0f));
-        const f2 lo = fma_f2(g, make_f2(-1.33497580e-8f), mul_f2(fma_f2(g, make_f2(-1.44269504f), neg), make_f2(0.693147181f)));
-        split_f2(hi, e0, e1);
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e0) : "f"(e0));
-        asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(e1) : "f"(e1));
-        const f2 e = make_f2(e0, e1), d = add_f2(fma_f2(e, lo, e), make_f2(1.0f));
+        const f2 g = v[i], d = add_f2(exp_f2<false>(g), make_f2(1.0f));
+        float d0, d1;
         split_f2(d, d0, d1);
+        top = absmax_nan(top, d0, d1);
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d0) : "f"(d0));
         asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(d1) : "f"(d1));
         const f2 r = make_f2(d0, d1), y = mul_f2(g, r), ny = mul_f2(y, make_f2(-1.0f));
         h[i] = mul_f2(fma_f2(fma_f2(ny, d, g), r, y), u[i]);
     }
-    if (!(top < kFar)) {
+    if (__any_sync(0xffffffffu, !(top < 5.5e37f))) {
 #pragma unroll
         for (int i = 0; i < 8; i++) {
-            float g0, g1, u0, u1, h0, h1;
+            float g0, g1, f0, f1, h0, h1;
             split_f2(v[i], g0, g1);
-            split_f2(u[i], u0, u1);
+            const bool far0 = !(g0 > -86.5f && g0 < 1e30f), far1 = !(g1 > -86.5f && g1 < 1e30f);
+            if (!__any_sync(0xffffffffu, far0 || far1)) continue;
+            split_f2(swiglu_far(v[i], u[i]), f0, f1);
             split_f2(h[i], h0, h1);
-            h[i] = make_f2(fabsf(g0) < kFar ? h0 : swiglu_far(g0, u0), fabsf(g1) < kFar ? h1 : swiglu_far(g1, u1));
+            h[i] = make_f2(far0 ? f0 : h0, far1 ? f1 : h1);
         }
     }
 #pragma unroll

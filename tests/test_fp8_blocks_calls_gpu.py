@@ -1,0 +1,60 @@
+"""Calls of the 8-bit block operators at the ends of their ranges, and around
+other streams (see test_fp8_blocks_gpu.py for their values)."""
+import pytest
+import torch
+
+from fp8_block_ref import MAX, U32, step, values
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _lib_ready(reng_lib):
+    reng_lib.lib()
+
+
+# As test_fp8_blocks_gpu.py counts the near range, 12 roundings: the far one takes
+# the exponential of a fraction (4), its correction (2) and two products (2).
+SWIGLU_REL = 12 * U32
+
+
+@pytest.mark.parametrize("fmt", [0, 1])
+@pytest.mark.parametrize("cols", [1, 8, 128, 130])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_swiglu_of_far_gates(dtype, cols, fmt):
+    """Rows of one gate each, from -80 to -210, with up values that bring the product back into the f32 range."""
+    from reng import fp8
+    gate = torch.tensor([-80.0, -86.9, -87.0, -87.5, -88.0, -88.5, -89.0, -90.25, -95.0, -103.0, -110.5, -125.0, -150.0, -173.0,
+                         -174.0, -180.0, -199.0, -201.0, -210.0])
+    up = torch.tensor([1e-3, 1.0, 1e10, -3e20, 1e30, -3e38])
+    g, u = (t.reshape(-1, 1).to(dtype).cuda() for t in torch.meshgrid(gate, up, indexing="ij"))
+    both = torch.cat([g.expand(-1, cols), u.expand(-1, cols)], 1).contiguous()
+    codes, scales = fp8.swiglu_quantize(both, fmt)
+    g, u = g.double(), u.double()
+    h = g / (1 + torch.exp(-g)) * u
+    # in f32: below half its smallest step a zero (scale 1, code 0), and scales no lower than its smallest normal;
+    # rows within a factor of 4 of that half step may go either way
+    edge = 2.0 ** -150
+    zero, alive = (h.abs() < edge / 4).flatten(), (h.abs() > edge * 4).flatten()
+    assert int(zero.sum()) > 10 and int(alive.sum()) > 10
+    got = values(fmt, "cuda")[codes.long()]
+    assert bool((got[zero] == 0).all()) and bool((scales[zero] == 1).all())
+    # a group of equal values: its scale is their size over max_finite, its codes max_finite with h's sign
+    s = (h.abs() / MAX[fmt]).clamp(min=2.0 ** -126)
+    tiny = 2.0 ** -149 / MAX[fmt]  # a subnormal h is off by half a step of 2^-149, and so its quotient
+    assert bool(((scales.double() - s).abs() <= s * (SWIGLU_REL + 2 * U32) + tiny)[alive].all())
+    v = (h / s).expand(-1, cols)
+    bound = 0.5 * torch.maximum(step(v, fmt), step(got, fmt)) + (SWIGLU_REL + 2 * U32) * v.abs() + 2.0 ** -149 / s
+    assert bool(((got - v).abs() <= bound)[alive].all())
+
+
+def test_swiglu_of_infinite_gates():
+    from reng import fp8
+    inf = float("inf")
+    both = torch.tensor([[inf, 2.0], [-inf, 2.0], [-300.0, 5.0], [300.0, -5.0], [float("nan"), 1.0]], device="cuda")
+    codes, scales = fp8.swiglu_quantize(both)
+    assert scales[0, 0] == inf and int(codes[0, 0]) & 0x7F == 0x7F       # inf / inf
+    assert int(codes[1, 0]) & 0x7F == 0x7F and scales[1, 0] == 1         # -inf / inf: NaN, never the absmax
+    assert int(codes[2, 0]) == 0x80 and scales[2, 0] == 1                # the zero of the limit, with its sign
+    assert values(0)[int(codes[3, 0])] == -240 and abs(float(scales[3, 0]) - 6.25) <= 6.25 * 2 * U32
+    assert int(codes[4, 0]) & 0x7F == 0x7F and scales[4, 0] == 1
