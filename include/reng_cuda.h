@@ -362,8 +362,14 @@ int reng_gemm_fp8_blocks(const uint8_t *x, int64_t ldx, const float *x_scales, i
 
 /* Whether a product of reng_gemm_fp8_blocks on the current device gave up on
  * a bounded device wait since the last call of this function: RENG_E_TIMEOUT
- * (its results are invalid), else RENG_OK.  Synchronises with the device. */
+ * (its results are invalid), else RENG_OK.  Waits for all work of the device,
+ * whatever its stream; not for use during stream capture. */
 int reng_gemm_fp8_blocks_status(void);
+
+/* One warp that waits, as a product's do, for an arrival that never comes, and
+ * gives up after the bound (2 s): reng_gemm_fp8_blocks_status must report it.
+ * Asynchronous on `stream`; for tests. */
+int reng_gemm_fp8_blocks_wait_check(void *stream);
 
 /* What h is written as. */
 #define RENG_NORM_NONE 0 /* y only */

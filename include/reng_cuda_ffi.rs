@@ -118,5 +118,6 @@ extern "C" {
                                 m: i64, n: i64, k: i64, y: *mut c_void, y_type: c_int, ldy: i64,
                                 stream: *mut c_void) -> c_int;
     pub fn reng_gemm_fp8_blocks_status() -> c_int;
+    pub fn reng_gemm_fp8_blocks_wait_check(stream: *mut c_void) -> c_int;
     pub fn reng_block_norm(desc: *const reng_block_norm_desc, stream: *mut c_void) -> c_int;
 }

@@ -85,7 +85,12 @@ constexpr int kScaleSlot = kRows * 16 + 64;  // [128 rows][4] of x, [3 weight bl
 // the registers that the block is launched with
 constexpr int kRegsRole = 40, kRegsAcc = 232;
 
-__device__ int g_fp8_gemm_err;   // set by a product whose waits ran out
+__device__ int g_fp8_gemm_err;    // set by a product whose waits ran out
+__device__ int g_fp8_gemm_taken;  // the value that a status call took from it
+
+// Read and clear in one step: a product of another stream may set the word
+// meanwhile, and is told of by the next call.
+__global__ void k_take_err() { g_fp8_gemm_taken = atomicExch(&g_fp8_gemm_err, 0); }
 
 struct Fp8Gemm {
     const float *sx, *sw;
@@ -219,6 +224,16 @@ __device__ __forceinline__ void wait(uint32_t bar, uint32_t parity, bool& bad) {
         : "r"(bar), "r"(parity)
         : "memory");
     if (!ok && !bad) bad = !bar_wait(bar, parity);
+}
+// A product's wait for an arrival that never comes.
+__global__ void k_wait_check() {
+    __shared__ __align__(8) unsigned long long never;
+    const uint32_t bar = (uint32_t)__cvta_generic_to_shared(&never);
+    if (threadIdx.x == 0) bar_init(bar, 1);
+    __syncwarp();
+    bool bad = false;
+    wait(bar, 0, bad);
+    if (bad) atomicExch(&g_fp8_gemm_err, RENG_E_TIMEOUT);
 }
 // The answer to a wait takes over 100 cycles even when the phase is complete,
 // so the loops ask for their next one ahead of the work between (`early`,
@@ -1050,10 +1065,19 @@ extern "C" int reng_gemm_fp8_blocks(const uint8_t *x, int64_t ldx, const float *
 }
 
 extern "C" int reng_gemm_fp8_blocks_status(void) {
+    static std::mutex mu;  // calls share g_fp8_gemm_taken
+    std::lock_guard<std::mutex> lock(mu);
+    RENG_CUDA_TRY(cudaDeviceSynchronize());  // non-blocking streams too
+    k_take_err<<<1, 1>>>();
+    RENG_CUDA_TRY(cudaGetLastError());
     int v = 0;
-    RENG_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_fp8_gemm_err, sizeof(v)));
+    RENG_CUDA_TRY(cudaMemcpyFromSymbol(&v, g_fp8_gemm_taken, sizeof(v)));
     if (v == 0) return RENG_OK;
-    const int zero = 0;
-    RENG_CUDA_TRY(cudaMemcpyToSymbol(g_fp8_gemm_err, &zero, sizeof(zero)));
     return fail(v, "reng_gemm_fp8_blocks: a product gave up on a bounded wait; its results are invalid");
+}
+
+extern "C" int reng_gemm_fp8_blocks_wait_check(void *stream) {
+    k_wait_check<<<1, 32, 0, (cudaStream_t)stream>>>();
+    RENG_CUDA_TRY(cudaGetLastError());
+    return RENG_OK;
 }

@@ -122,6 +122,7 @@ SIGNATURES = {
     "reng_gemm_fp8_blocks": ([_P, C.c_int64, _P, C.c_int64, C.c_int, _P, C.c_int64, _P, C.c_int64, C.c_int,
                               C.c_int64, C.c_int64, C.c_int64, _P, C.c_int, C.c_int64, _P], C.c_int),
     "reng_gemm_fp8_blocks_status": ([], C.c_int),
+    "reng_gemm_fp8_blocks_wait_check": ([_P], C.c_int),
     "reng_block_norm": ([_P, _P], C.c_int),
     "reng_tp_unique_id": ([_P], C.c_int),
     "reng_gemm_bf16": ([_P, C.c_int, C.c_int, _P, C.c_int, _P, C.c_int, C.c_int, _P, C.c_int], C.c_int),

@@ -12,6 +12,7 @@ And the block-scaled FP8 product on torch CUDA tensors:
 
 with x from fp8.quantize_blocks(.., 1) / fp8.swiglu_quantize /
 norm.block_norm_fp8 and w from fp8.quantize_blocks(.., 128).
+gemm_fp8_blocks_status() tells whether all products so far came to their end.
 """
 import ctypes as C
 
@@ -51,8 +52,22 @@ def gemm_fp8_blocks(x, x_scales, w, w_scales, out=None, dtype=None, x_fmt=_lib.R
     x uint8 codes [M, K] with scales [M, ceil(K / 128)], w uint8 codes [N, K]
     with scales [ceil(N / 128), ceil(K / 128)]; rows start on 16 bytes
     (fp8.quantize_blocks lays them out so).  y [M, N] is `out`, or a new
-    tensor of `dtype` (bf16 by default, or f32)."""
+    tensor of `dtype` (bf16 by default, or f32).  Should a device wait of the
+    product run out (a fault of the device or of this library), y is invalid
+    and gemm_fp8_blocks_status raises."""
     t = _impl or _tensors()
     if stream is not None:
         return t.on_stream(stream, x, t.gemm_fp8_blocks, x, x_scales, w, w_scales, out, dtype, x_fmt, w_fmt)
     return t.gemm_fp8_blocks(x, x_scales, w, w_scales, out, dtype, x_fmt, w_fmt)
+
+
+def gemm_fp8_blocks_status(device=None):
+    """Raise RengError (code RENG_E_TIMEOUT) if a product on the device (the
+    current one by default) gave up on a bounded wait since the last call: its
+    results are invalid.  Waits for all work of the device."""
+    if device is None:
+        _lib.call("reng_gemm_fp8_blocks_status")
+    else:
+        import torch
+        with torch.cuda.device(device):
+            _lib.call("reng_gemm_fp8_blocks_status")

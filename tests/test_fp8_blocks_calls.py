@@ -34,3 +34,20 @@ def test_a_product_waits_for_the_last_arrivals_of_its_stages(tmp_path):
 def test_a_norm_row_of_any_alignment_is_read_alone(tmp_path):
     """Nothing beside a row is read, where another row may be written meanwhile or memory end."""
     assert " bad 0" in run_check(tmp_path, "row_image_check")
+
+
+def test_python_raises_what_the_status_tells(monkeypatch, reng_lib):
+    from reng import gemm
+    codes = [reng_lib.RENG_E_TIMEOUT, reng_lib.RENG_OK]
+
+    class Fake:
+        def reng_gemm_fp8_blocks_status(self):
+            return codes.pop(0)
+
+        def reng_last_error(self):
+            return b"gave up"
+    monkeypatch.setattr(reng_lib, "lib", Fake)
+    with pytest.raises(reng_lib.RengError, match="gave up"):
+        gemm.gemm_fp8_blocks_status()
+    gemm.gemm_fp8_blocks_status()
+    assert not codes

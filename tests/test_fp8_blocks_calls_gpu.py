@@ -58,3 +58,17 @@ def test_swiglu_of_infinite_gates():
     assert int(codes[2, 0]) == 0x80 and scales[2, 0] == 1                # the zero of the limit, with its sign
     assert values(0)[int(codes[3, 0])] == -240 and abs(float(scales[3, 0]) - 6.25) <= 6.25 * 2 * U32
     assert int(codes[4, 0]) & 0x7F == 0x7F and scales[4, 0] == 1
+
+
+# ------------------------------------------------- a product that gave up --
+def test_a_wait_that_ran_out_on_another_stream_is_told(reng_lib):
+    """The status waits for work of every stream (torch's do not block the legacy one), tells once, and clears."""
+    from reng import gemm
+    gemm.gemm_fp8_blocks_status()
+    side = torch.cuda.Stream()
+    reng_lib.call("reng_gemm_fp8_blocks_wait_check", side.cuda_stream)  # 2 s, still running below
+    with pytest.raises(reng_lib.RengError, match="gave up") as e:
+        gemm.gemm_fp8_blocks_status()
+    assert e.value.code == reng_lib.RENG_E_TIMEOUT and side.query()
+    gemm.gemm_fp8_blocks_status()
+    gemm.gemm_fp8_blocks_status(torch.cuda.current_device())
