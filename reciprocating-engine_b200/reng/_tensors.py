@@ -94,12 +94,20 @@ def call(dev, name, *args):
 
 def on_stream(stream, like, run, *args):
     """run(*args) on `stream` (a torch stream or a raw handle of the tensor's
-    device): what it allocates belongs to that stream too.  As with any work
-    on a side stream, the caller orders it after its inputs."""
+    device): what it allocates belongs to that stream.  As with any work on a
+    side stream, the caller orders it after its inputs.  The tensors among
+    `args` are held until a torch stream is done with them; a raw handle may be
+    gone by then, so its caller keeps them alive."""
+    external = torch.cuda.ExternalStream
     if not isinstance(stream, torch.cuda.Stream):
-        stream = torch.cuda.ExternalStream(stream, device=like.device)
+        stream = external(stream, device=like.device)
     with torch.cuda.stream(stream):
-        return run(*args)
+        out = run(*args)
+    if not isinstance(stream, external):
+        for t in args:
+            if isinstance(t, torch.Tensor):
+                t.record_stream(stream)
+    return out
 
 
 def blocks_out(x, dev, rows, cols, scale_rows, codes, scales):

@@ -290,7 +290,11 @@ def quantize_blocks(x, block_rows=1, fmt=Fp8Format.E4M3, codes=None, scales=None
     Returns (codes uint8 [rows, cols] in rows of 16-byte pitch, scales f32
     [ceil(rows / block_rows), ceil(cols / 128)]), the operands of
     gemm.gemm_fp8_blocks.  A block's scale is absmax / max_finite (1 for
-    zeros) and its codes encode(x / scale) by the rules of quantize_with."""
+    zeros) and its codes encode(x / scale) by the rules of quantize_with.
+
+    `stream`: a torch stream of x's device to run on, or a raw handle (the
+    current stream by default).  The caller orders it after x, and with a raw
+    handle keeps x alive; a torch stream holds x until it is done."""
     t = _impl or _tensors()
     if stream is not None:
         return t.on_stream(stream, x, t.quantize_blocks, x, block_rows, fmt, codes, scales)
@@ -300,7 +304,8 @@ def quantize_blocks(x, block_rows=1, fmt=Fp8Format.E4M3, codes=None, scales=None
 def swiglu_quantize(gate_up, fmt=Fp8Format.E4M3, codes=None, scales=None, stream=None):
     """quantize_blocks of h = silu(gate) * up in 1 x 128 groups, h in f32:
     gate_up [rows, 2 * cols] (bf16 or f32) holds the gate columns, then the
-    up columns.  Returns (codes uint8 [rows, cols], scales)."""
+    up columns.  Returns (codes uint8 [rows, cols], scales).  `stream` as for
+    quantize_blocks."""
     t = _impl or _tensors()
     if stream is not None:
         return t.on_stream(stream, gate_up, t.swiglu_quantize, gate_up, fmt, codes, scales)

@@ -54,7 +54,7 @@ def gemm_fp8_blocks(x, x_scales, w, w_scales, out=None, dtype=None, x_fmt=_lib.R
     (fp8.quantize_blocks lays them out so).  y [M, N] is `out`, or a new
     tensor of `dtype` (bf16 by default, or f32).  Should a device wait of the
     product run out (a fault of the device or of this library), y is invalid
-    and gemm_fp8_blocks_status raises."""
+    and gemm_fp8_blocks_status raises.  `stream` as for fp8.quantize_blocks."""
     t = _impl or _tensors()
     if stream is not None:
         return t.on_stream(stream, x, t.gemm_fp8_blocks, x, x_scales, w, w_scales, out, dtype, x_fmt, w_fmt)

@@ -13,6 +13,7 @@ pass over the rows.
 (y, codes, scales), h as FP8 codes with one f32 scale per 1 x 128 group, the
 operand of gemm.gemm_fp8_blocks.  Sums and norms are f32.  `out` may be
 `residual` itself (in place); without a branch y is `residual`, unwritten.
+`stream` as for fp8.quantize_blocks.
 """
 import struct
 

@@ -72,3 +72,43 @@ def test_a_wait_that_ran_out_on_another_stream_is_told(reng_lib):
     assert e.value.code == reng_lib.RENG_E_TIMEOUT and side.query()
     gemm.gemm_fp8_blocks_status()
     gemm.gemm_fp8_blocks_status(torch.cuda.current_device())
+
+
+# ------------------------------------------------------------ side streams --
+@pytest.mark.parametrize("what", ["quantize", "swiglu", "product", "norm", "norm_fp8"])
+def test_a_side_stream_holds_its_inputs(what):
+    """Inputs dropped right after a call on a busy stream, and their memory taken by others."""
+    from reng import fp8, gemm, norm
+    g = torch.Generator(device="cuda").manual_seed(3)
+
+    def inputs():
+        g.manual_seed(3)
+        x = torch.randn(512, 4096, generator=g, device="cuda")
+        if what == "product":
+            return fp8.quantize_blocks(x) + fp8.quantize_blocks(torch.randn(512, 4096, generator=g, device="cuda"), 128)
+        return (x, x + 1) if what.startswith("norm") else (x,)
+    call = {"quantize": fp8.quantize_blocks, "swiglu": fp8.swiglu_quantize, "product": gemm.gemm_fp8_blocks,
+            "norm": norm.block_norm, "norm_fp8": norm.block_norm_fp8}[what]
+
+    def outputs(r):
+        return [r] if torch.is_tensor(r) else [t for t in r if t is not None]
+    want = [t.clone() for t in outputs(call(*inputs()))]
+    side = torch.cuda.Stream()
+    args = inputs()
+    sizes = [(t.untyped_storage().nbytes(),) for t in args]
+    keep = [torch.full(n, 7, dtype=torch.uint8, device="cuda") for n in sizes]  # the kernel that writes below is loaded
+    torch.cuda.synchronize()
+    with torch.cuda.stream(side):
+        torch.cuda._sleep(int(1e9))  # half a second
+    got = outputs(call(*args, stream=side))
+    assert not side.query()
+    del args
+    keep += [torch.full(n, 7, dtype=torch.uint8, device="cuda") for n in sizes for _ in range(2)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    # and on a raw handle, whose caller keeps the inputs
+    args = inputs()
+    side.wait_stream(torch.cuda.current_stream())
+    got = outputs(call(*args, stream=side.cuda_stream))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
