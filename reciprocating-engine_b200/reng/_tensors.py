@@ -98,9 +98,12 @@ def on_stream(stream, like, run, *args):
     side stream, the caller orders it after its inputs.  The tensors among
     `args` are held until a torch stream is done with them; a raw handle may be
     gone by then, so its caller keeps them alive."""
+    index(like)
     external = torch.cuda.ExternalStream
     if not isinstance(stream, torch.cuda.Stream):
         stream = external(stream, device=like.device)
+    elif stream.device != like.device:
+        raise ValueError("a stream of %s for tensors on %s" % (stream.device, like.device))
     with torch.cuda.stream(stream):
         out = run(*args)
     if not isinstance(stream, external):

@@ -51,3 +51,22 @@ def test_python_raises_what_the_status_tells(monkeypatch, reng_lib):
         gemm.gemm_fp8_blocks_status()
     gemm.gemm_fp8_blocks_status()
     assert not codes
+
+
+def test_a_stream_of_another_device_is_refused(monkeypatch):
+    import torch
+    from reng import _tensors
+
+    class Stream:
+        device = torch.device("cuda", 1)
+
+    class Tensor:
+        device = torch.device("cuda", 0)
+
+        def get_device(self):
+            return 0
+    monkeypatch.setattr(torch.cuda, "Stream", Stream)
+    with pytest.raises(ValueError, match="cuda:1.*cuda:0"):
+        _tensors.on_stream(Stream(), Tensor(), lambda: pytest.fail("ran"))
+    with pytest.raises(ValueError, match="not on a CUDA device"):
+        _tensors.on_stream(7, torch.zeros(2, 128), lambda: pytest.fail("ran"))
