@@ -162,7 +162,7 @@ def gemm_fp8_blocks(x, x_scales, w, w_scales, out, dtype, x_fmt, w_fmt):
     dev = index(x)
     ldx = matrix(x, "x", U8, dev)
     M, K = x.shape
-    N = w.shape[0]
+    N = w.shape[0] if w.dim() == 2 else _refuse(w, "w", U8, dev, None, None)
     kb = groups(K)
     ldw = matrix(w, "w", U8, dev, N, K)
     ldsx = matrix(x_scales, "x_scales", F32, dev, M, kb)

@@ -112,3 +112,22 @@ def test_a_side_stream_holds_its_inputs(what):
     got = outputs(call(*args, stream=side.cuda_stream))
     torch.cuda.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+# ---------------------------------------------------------------- refusals --
+def test_python_refuses_what_is_no_matrix(reng_lib):
+    from reng import fp8, gemm, norm
+    x, sx = fp8.quantize_blocks(torch.ones(4, 256, device="cuda"))
+    w, sw = fp8.quantize_blocks(torch.ones(200, 256, device="cuda"), 128)
+    b = torch.zeros(4, 256, dtype=torch.bfloat16, device="cuda")
+    for call in (lambda: gemm.gemm_fp8_blocks(x, sx, w[0, 0], sw), lambda: gemm.gemm_fp8_blocks(x, sx, w[0], sw),
+                 lambda: gemm.gemm_fp8_blocks(x[0], sx, w, sw), lambda: norm.block_norm(b[0]), lambda: norm.block_norm_fp8(b[0]),
+                 lambda: fp8.swiglu_quantize(b[0])):
+        with pytest.raises(ValueError):
+            call()
+    # what only the library sees: sizes of zero, numbers that are no finite f32
+    for call in (lambda: norm.block_norm(b, eps=-1.0), lambda: norm.block_norm(b, b, scale=float("inf")),
+                 lambda: norm.block_norm(b, b, scale=1e39), lambda: norm.block_norm(b, b, eps=-1e300),
+                 lambda: gemm.gemm_fp8_blocks(x, sx, w[:0], sw[:0]), lambda: fp8.quantize_blocks(b[:, :0])):
+        with pytest.raises(reng_lib.RengError):
+            call()
