@@ -385,7 +385,8 @@ typedef struct reng_block_norm_desc {
     const void *gate;       /* [rows, cols] multiplier of the branch, or [cols] with ld_gate 0; NULL: 1 */
     const float *post_gain; /* [cols] gain of the norm after the block; NULL: no such norm */
     const float *pre_gain;  /* [cols] gain of the norm before the next block; NULL: 1 */
-    void *y;                /* [rows, cols] new residual stream, residual_type; may be `residual` itself */
+    void *y;                /* [rows, cols] new residual stream, residual_type; may be `residual` itself,
+                             * at the same pitch */
     void *h;                /* [rows, cols] the next block's input (unused with RENG_NORM_NONE) */
     float *h_scales;        /* [rows, ceil(cols / 128)] with RENG_NORM_E4M3 / E5M2 */
     int64_t rows, cols;

@@ -552,6 +552,9 @@ extern "C" int reng_block_norm(const reng_block_norm_desc *d, void *stream) {
     if (d->rows == 0) return RENG_OK;
     RENG_CHECK_ARG(d->residual && (!d->branch || d->y) && (d->out == RENG_NORM_NONE || d->h) && (!fp8 || d->h_scales),
                    f + "NULL buffer");
+    // in place a row is written where it was read; at another pitch, where another row is still to be read
+    RENG_CHECK_ARG(!d->branch || d->y != d->residual || d->rows == 1 || d->ld_y == d->ld_residual,
+                   f + "y in place of residual at another row pitch");
     NormArgs a{};
     a.branch = d->branch;
     a.residual = d->residual;

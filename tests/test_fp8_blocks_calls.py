@@ -70,3 +70,12 @@ def test_a_stream_of_another_device_is_refused(monkeypatch):
         _tensors.on_stream(Stream(), Tensor(), lambda: pytest.fail("ran"))
     with pytest.raises(ValueError, match="not on a CUDA device"):
         _tensors.on_stream(7, torch.zeros(2, 128), lambda: pytest.fail("ran"))
+
+
+def test_a_norm_in_place_at_another_pitch_is_refused(reng_lib):
+    import ctypes as C
+    d = reng_lib.BlockNormDesc(branch=4096, residual=8192, y=8192, rows=4, cols=256, ld_branch=256, ld_residual=256, ld_y=264,
+                               out=reng_lib.RENG_NORM_NONE, scale=1.0, eps=1e-5)
+    L = reng_lib.lib()
+    assert L.reng_block_norm(C.byref(d), None) == reng_lib.RENG_E_INVAL
+    assert b"another row pitch" in L.reng_last_error()
