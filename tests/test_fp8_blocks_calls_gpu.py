@@ -131,3 +131,40 @@ def test_python_refuses_what_is_no_matrix(reng_lib):
                  lambda: gemm.gemm_fp8_blocks(x, sx, w[:0], sw[:0]), lambda: fp8.quantize_blocks(b[:, :0])):
         with pytest.raises(reng_lib.RengError):
             call()
+
+
+# --------------------------------------------------------------- the engine --
+@pytest.mark.parametrize("case,T", [("gqa", 2100), ("bias and qk_norm", 70), ("bias and qk_norm", 2100)])
+def test_engine_past_2048_positions_and_with_biases_before_the_norm(reng_lib, case, T):
+    """Decode attention's kernel for engines of 2048 positions and more, and q/k norms behind
+    biases, in the block-scaled mode: one layer against its 64-bit attention."""
+    import numpy as np
+    from reng.model import Engine
+    from reng.synth import prompt_ids
+    from test_decode_gpu import small_cfg
+    from test_fp8_blocks_engine_gpu import BLOCKS, attention_oracle, see_through
+    both = case == "bias and qk_norm"
+    cfg = small_cfg(bias=both, num_hidden_layers=1)
+    w = see_through(cfg, 7)
+    if both:
+        rng = np.random.default_rng(3)
+        for k in ("qn", "kn"):
+            w["layers"][0][k] = rng.uniform(0.2, 0.6, cfg.head_dim()).astype(np.float32)
+    ids = prompt_ids(T, cfg.vocab_size, seed=T)
+    want, bound = attention_oracle(cfg, w, ids, both)
+    e = Engine(cfg, w, batch=2, capacity=2304, fp8=BLOCKS)
+    H = cfg.hidden_size
+
+    def check(got, rows):
+        got = torch.from_numpy(np.ascontiguousarray(got[..., :H])).to(want.device).double().reshape(-1, H)
+        err = (got - want[rows]).abs()
+        assert bool((err <= bound[rows]).all()), "%d values off, worst %.3g of the bound" % (
+            int((err > bound[rows]).sum()), float((err / bound[rows]).max()))
+    check(e.prefill(1, ids, all_logits=True)[2], slice(None))
+    e.reset()
+    e.prefill(0, ids[:T // 3])
+    e.prefill(1, ids[:T - 1])
+    logits, _ = e.step_logits(np.array([ids[T // 3], ids[T - 1]], np.uint32))
+    check(logits[0], slice(T // 3, T // 3 + 1))
+    check(logits[1], slice(T - 1, T))
+    e.close()
