@@ -1003,7 +1003,9 @@ int gemm_fp8_blocks(const uint8_t* x, int64_t ldx, const float* sx, int64_t ldsx
     a.mbox = std::min(kRows, (M + 7) / 8 * 8);
     a.y_f32 = y_type == RENG_TYPE_F32;
     a.y_vec = ops_aligned(y, ldy * (a.y_f32 ? 4 : 2), 32);
-    a.y_tma = ops_aligned(y, ldy * (a.y_f32 ? 4 : 2), 16);
+    // a tensor copy's last columns are rounded up to 16 bytes, with zeros: not
+    // into the columns behind y's in a larger matrix
+    a.y_tma = ops_aligned(y, ldy * (a.y_f32 ? 4 : 2), 16) && (int64_t)N * (a.y_f32 ? 4 : 2) % 16 == 0;
     a.sx_vec = ops_aligned(sx, ldsx * 4, 16);
     a.err = err;
     const Plan p = plan(M, N, a.kb, sms);

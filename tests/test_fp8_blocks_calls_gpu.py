@@ -133,6 +133,28 @@ def test_python_refuses_what_is_no_matrix(reng_lib):
             call()
 
 
+# ---------------------------------------------- outputs in a larger matrix --
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("m,n,k", [(130, 1, 1), (282, 2, 3), (1356, 14, 130), (202, 1396, 40), (1323, 38, 32), (605, 5157, 256),
+                                   (300, 2047, 300), (257, 64, 128), (1001, 5123, 100), (40, 301, 200), (100, 40003, 64)])
+def test_a_product_writes_its_own_columns_alone(m, n, k, dtype):
+    """Rows on 16 bytes whose width is no multiple of 16 bytes, at every pitch to the next two: what lies
+    behind a row stays."""
+    from reng import gemm
+    from test_fp8_blocks_gpu import check_product, operands, pitched
+    ops = operands(m + n, m, n, k)
+    want = None
+    for pitch in range(n, n + 17):
+        y, store = pitched(m, n, pitch, dtype, 16, fill=-3.0)
+        gemm.gemm_fp8_blocks(*ops, out=y)
+        if want is None:
+            check_product(y, *ops)
+            want = y.clone()
+        assert torch.equal(y, want)
+        y.fill_(-3.0)
+        assert bool((store == -3.0).all()), pitch
+
+
 # --------------------------------------------------------------- the engine --
 @pytest.mark.parametrize("case,T", [("gqa", 2100), ("bias and qk_norm", 70), ("bias and qk_norm", 2100)])
 def test_engine_past_2048_positions_and_with_biases_before_the_norm(reng_lib, case, T):
