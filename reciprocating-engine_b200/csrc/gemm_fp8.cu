@@ -129,18 +129,6 @@ __device__ __forceinline__ void tmem_wait32(uint32_t (&r)[32]) {
                    "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]),
                    "+r"(r[29]), "+r"(r[30]), "+r"(r[31])::"memory");
 }
-// Two f32 in one register pair, and acc = s * v + acc on both.
-__device__ __forceinline__ unsigned long long pair2(uint32_t lo, uint32_t hi) {
-    unsigned long long r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "r"(lo), "r"(hi));
-    return r;
-}
-__device__ __forceinline__ void unpair2(unsigned long long v, float& lo, float& hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ void fma2(unsigned long long& acc, unsigned long long v, unsigned long long s) {
-    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(acc) : "l"(v), "l"(s));
-}
 // One MMA of 32 k: the operands' descriptors are K-major, 128-byte swizzle
 // (tc.cuh, umma_desc), given by their low words (address / 16, the only part
 // that changes).
@@ -328,7 +316,7 @@ struct AccState {
     bool bad;
 };
 template <bool PAIR, int NC, bool TWO>
-__device__ __forceinline__ void add_blocks(AccState& st, int k0, int k1, int edge, unsigned long long (&acc)[64]) {
+__device__ __forceinline__ void add_blocks(AccState& st, int k0, int k1, int edge, f2 (&acc)[64]) {
     uint32_t td = 0, ts = 0;  // early answers for the next block's sum and the next slot of scales
     float x = 0.f, w0 = 0.f, w1 = 0.f;  // the next block's scales
     wait(st.bar0 + 8u * (B_SFULL + st.slot), st.sph, st.bad);
@@ -379,16 +367,20 @@ __device__ __forceinline__ void add_blocks(AccState& st, int k0, int k1, int edg
             for (int h = 0; h < 2; h++) {
                 if (g + h >= NC) break;
                 const float s = TWO && 32 * (g + h) >= edge ? s1 : s0;
-                const unsigned long long ss = pair2(__float_as_uint(s), __float_as_uint(s));
+                const f2 ss = make_f2(s);
 #pragma unroll
-                for (int i = 0; i < 16; i++) fma2(acc[16 * (g + h) + i], pair2(v[h][2 * i], v[h][2 * i + 1]), ss);
+                for (int i = 0; i < 16; i++) {
+                    const f2 d = make_f2(__uint_as_float(v[h][2 * i]), __uint_as_float(v[h][2 * i + 1]));
+                    f2& to = acc[16 * (g + h) + i];
+                    to = fma_f2(d, ss, to);
+                }
             }
         }
     }
 }
 template <bool PAIR>
 __device__ __forceinline__ void add_tile(AccState& st, int nc, bool two, int k0, int k1, int edge,
-                                         unsigned long long (&acc)[64]) {
+                                         f2 (&acc)[64]) {
     if (nc == 0) add_blocks<PAIR, 0, false>(st, k0, k1, edge, acc);
     else if (nc == 4 && !two) add_blocks<PAIR, 4, false>(st, k0, k1, edge, acc);
     else if (nc == 4) add_blocks<PAIR, 4, true>(st, k0, k1, edge, acc);
@@ -416,7 +408,7 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // A thread's accumulators (row r of the tile, columns c0 .. c0 + cw - 1) into
 // the shared memory of the CTAs that own the columns.
 __device__ __forceinline__ void push_partials(const Fp8Gemm& a, uint32_t part, int rank, int r, int c0, int cw,
-                                              const unsigned long long (&acc)[64]) {
+                                              const f2 (&acc)[64]) {
     const int share = a.bn / a.ks, first = c0 / share;
     const uint32_t pitch = 4u * (uint32_t)(a.mbox + 1), mine = part + (uint32_t)(rank * share) * pitch + 4u * (uint32_t)r;
     int q = first, left = share - (c0 - first * share);
@@ -425,7 +417,7 @@ __device__ __forceinline__ void push_partials(const Fp8Gemm& a, uint32_t part, i
     for (int i = 0; i < 64; i++) {
         if (2 * i >= cw) break;
         float lo, hi;
-        unpair2(acc[i], lo, hi);
+        split_f2(acc[i], lo, hi);
         if (q == rank) {  // its own share
             sts_f(to, lo);
             sts_f(to + pitch, hi);
@@ -702,7 +694,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int n0 = at.n0 + c0;
             st.tmem = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + c0;
             const bool any = mw < a.M && n0 < a.N && cw > 0;  // the warp has outputs in this tile
-            unsigned long long acc[64];
+            f2 acc[64];
 #pragma unroll
             for (int c = 0; c < 64; c++) acc[c] = 0ull;
             // its columns touch at most two weight blocks; the second starts at column `edge`
@@ -720,7 +712,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                 for (int g = 0; g < 4; g++) {
                     if (32 * g >= cw || n0 + 32 * g >= a.N) break;
-                    const unsigned long long* q = acc + 16 * g;
+                    const f2* q = acc + 16 * g;
                     if (a.y_f32) {  // 128-byte rows, one box
                         const uint32_t buf = out0;
                         if (lane == 0) s2g_wait_read<0>();
@@ -728,8 +720,8 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int ch = 0; ch < 8; ch++) {
                             float f0, f1, f2, f3;
-                            unpair2(q[2 * ch], f0, f1);
-                            unpair2(q[2 * ch + 1], f2, f3);
+                            split_f2(q[2 * ch], f0, f1);
+                            split_f2(q[2 * ch + 1], f2, f3);
                             st_shared16(buf + lane * 128 + ((ch ^ (lane & 7)) << 4), __float_as_uint(f0), __float_as_uint(f1),
                                         __float_as_uint(f2), __float_as_uint(f3));
                         }
@@ -747,7 +739,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                             for (int i = 0; i < 4; i++) {
                                 float lo, hi;
-                                unpair2(q[4 * ch + i], lo, hi);
+                                split_f2(q[4 * ch + i], lo, hi);
                                 w[i] = bf16x2(lo, hi);
                             }
                             st_shared16(buf + lane * 64 + ((ch ^ ((lane >> 1) & 3)) << 4), w[0], w[1], w[2], w[3]);
@@ -765,14 +757,14 @@ __global__ void __launch_bounds__(kThreads, 1)
                     // warp's staging, consecutive lanes on consecutive columns
                     const int n = n0 + 16 * g;
                     if (16 * g >= cw || n >= a.N) break;
-                    const unsigned long long* q = acc + 8 * g;
+                    const f2* q = acc + 8 * g;
                     if (a.y_vec && n + 16 <= a.N) {
                         if (m < a.M) {
                             uint32_t w[16];
 #pragma unroll
                             for (int i = 0; i < 8; i++) {
                                 float lo, hi;
-                                unpair2(q[i], lo, hi);
+                                split_f2(q[i], lo, hi);
                                 if (a.y_f32) w[2 * i] = __float_as_uint(lo), w[2 * i + 1] = __float_as_uint(hi);
                                 else w[i] = bf16x2(lo, hi);
                             }
@@ -785,7 +777,7 @@ __global__ void __launch_bounds__(kThreads, 1)
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             float lo, hi;
-                            unpair2(q[i], lo, hi);
+                            split_f2(q[i], lo, hi);
                             sts_f(out0 + 4 * (lane * 17 + 2 * i), lo);
                             sts_f(out0 + 4 * (lane * 17 + 2 * i + 1), hi);
                         }
@@ -1004,7 +996,8 @@ int gemm_fp8_blocks(const uint8_t* x, int64_t ldx, const float* sx, int64_t ldsx
     a.y_f32 = y_type == RENG_TYPE_F32;
     a.y_vec = ops_aligned(y, ldy * (a.y_f32 ? 4 : 2), 32);
     // a tensor copy's last columns are rounded up to 16 bytes, with zeros: not
-    // into the columns behind y's in a larger matrix
+    // into the columns behind y's in a larger matrix (2048 x 4094 x 4096 by
+    // elements 33.9 us, 2048 x 4096 x 4096 by copies 32.6)
     a.y_tma = ops_aligned(y, ldy * (a.y_f32 ? 4 : 2), 16) && (int64_t)N * (a.y_f32 ? 4 : 2) % 16 == 0;
     a.sx_vec = ops_aligned(sx, ldsx * 4, 16);
     a.err = err;
