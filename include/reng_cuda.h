@@ -50,7 +50,10 @@ const char *reng_last_error(void);
 /* ABI version: (major << 16) | minor.  Minor 2 added reng_model_desc.qk_norm
  * and reng_layer_weights.qn / kn / no_rope (callers built against minor 1
  * pass structs that are too short); minor 3 added
- * reng_model_time_kernels_rows and removed reng_model_trace_step. */
+ * reng_model_time_kernels_rows and removed reng_model_trace_step.  A function
+ * or a constant that is only added does not move it: a library of minor 3 that
+ * lacks the block operators lacks their symbols, and refuses
+ * RENG_WEIGHTS_FP8_BLOCKS (RENG_E_INVAL, "unknown weight format"). */
 int reng_version(void);
 
 /* Number of CUDA devices (replaces reng-hal's Gaudi accel discovery,
@@ -346,8 +349,9 @@ int reng_fp8_swiglu_quantize(const void *gate, const void *up, int type, int64_t
  * y[m][n] = sum_b x_scales[m][b] * w_scales[n / 128][b] * sum_{k in block b} x[m][k] * w[n][k]
  *
  * x codes [M, K] with 1 x 128 scales, w codes [N, K] with 128 x 128 scales,
- * y [M, N] in y_type.  Products and sums in f32, scales applied to each
- * block's sum in f32, one rounding to y_type.  Codes must start on a 16-byte
+ * y [M, N] in y_type.  Products and sums in f32; a block's two scales are
+ * multiplied first, in f32 (their product is to stay a normal f32), and applied
+ * to its sum; one rounding to y_type.  Codes must start on a 16-byte
  * boundary and have a pitch that is a multiple of 16 (RENG_E_INVAL); M, N and
  * K are otherwise free up to 2^30.  The formats of x and w are independent.
  * E4M3 codes are read with the tensor core's table: the codes this library's

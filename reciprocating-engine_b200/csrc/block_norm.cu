@@ -334,8 +334,9 @@ __device__ __forceinline__ void copy_own(uint8_t* dst, const void* row, const Ti
 // takes stay in registers, so HBM is busy while teams wait for their sums.
 // Held as loads in registers instead, the next row left 15 warps an SM and
 // rows of any alignment spilled: 1023 x 5120, f32 branch, gate and both norms
-// 22.5 us against 15.1 (4.2 TB/s); 8192 x 4096 to FP8 65 against 56 (bound by
-// instruction issue, the codes above all); 6599 x 578 to FP8 43 against 16.
+// 22.5 us against 14.1 (4.5 TB/s); 8192 x 4096 to FP8 65 against 56 (two thirds
+// of the issue slots, the codes above all, and waits on shared memory of the 24
+// warps that the registers leave); 6599 x 578 to FP8 43 against 17.
 // A third slot costs wide rows their second team (5120 columns: 18.3 us).
 template <int TB, int TR, int G>
 __global__ void __launch_bounds__(32 * kMaxWarps, 1) k_block_norm(const NormArgs a, const Plan p) {

@@ -25,13 +25,16 @@
 //   * Many rows (PAIR): two CTAs of a cluster multiply one 256-row tile with
 //     tcgen05 cta_group::2; each loads its own 128 token rows and half of the
 //     weight rows, so the bytes an SM takes from L2 per block drop from 48 to
-//     32 KB at bn = 256.  8192 x 28672 x 4096 takes 800 us (2.4 PFLOP/s): the
-//     power limit, the tensor cores busy for 512 of a block's 684 cycles.
+//     32 KB at bn = 256.  A block takes some 670 cycles, 512 of them the
+//     MMAs', and a tile 3100 more (8192 x 28672 x 4096 1.208 M cycles, 771 a
+//     block in all; 8192 x 4096 x 14336 0.548 M, 699).  The clock is the power
+//     limit's: 803 us at 1.50 GHz in a first launch (2.4 PFLOP/s), 937 at 1.29
+//     after a thousand, the cycles the same.
 //     (The two halves of the columns as MMAs of their own read the token rows
 //     twice from shared memory: 8192 x 4096 x 14336 440 us against 390.)
 //   * The last round of tiles over the SMs is rarely full: it takes narrower
 //     tiles than the rounds before it (1001 x 5120 x 27648: 166 us in tiles of
-//     192 columns, 154 in 18 of 256 and 8 of 64; 5789 x 909 x 4011 64 and 50).
+//     192 columns, 150 in 18 of 256 and 8 of 64; 5789 x 909 x 4011 64 and 50).
 //   * Few tiles (decode): K is split over the CTAs of a cluster.  Each CTA owns
 //     a share of the columns; all of them write their f32 partials of it into
 //     its shared memory (stores to a peer do not wait, loads from one take a

@@ -8,9 +8,9 @@
 
 namespace reng {
 
-// Latency-bound: 8 KB in and out a row against a launch of 2-3 us (the q/k/v
-// kind, product and this, takes 13.2 us at one row of 4096 -> 6144 and 44.4 us
-// at 1024).  One CTA per row; a thread takes two neighbouring dims of both halves of a
+// Latency-bound: 2 (q_dim + 2 kv_dim) bytes in and as many out a row, 12 KB each
+// at 4096 -> 6144, against a launch of 2-3 us (the q/k/v kind, product and this,
+// takes 11.3 us at one such row and 45 us at 1024).  One CTA per row; a thread takes two neighbouring dims of both halves of a
 // head (or two of v), 4 bytes an access.  The rotation is
 //   y[d] = x[d] cos[d] - x[d + hd/2] sin[d],  y[d + hd/2] = x[d + hd/2] cos[d + hd/2] + x[d] sin[d + hd/2].
 __global__ void __launch_bounds__(256) k_rope_kv(RopeKvArgs a) {
