@@ -133,6 +133,29 @@ def test_python_refuses_what_is_no_matrix(reng_lib):
             call()
 
 
+# -------------------------------------------------------------- long rows --
+# A thread adds 16 squares in f32 (8 and 1 in sequence) and its tiles in 64 bits, the CTA 5 + 16 more:
+# 32 roundings of the sum at most, 16 of its root, and 8 as in test_fp8_blocks_gpu.py: below its 48.
+@pytest.mark.parametrize("cols", [40000, 1 << 20, (1 << 24) + 8, (1 << 24) + 3])
+@pytest.mark.parametrize("post", [False, True])
+def test_the_norm_of_a_long_row(cols, post):
+    """Equal values, whose running sum in f32 would be off by one way of rounding, and normal ones."""
+    from reng import norm
+    from test_fp8_blocks_gpu import NORM_REL
+    for x in (torch.full((2, cols), 1.1, device="cuda"), torch.randn(2, cols, device="cuda")):
+        gain = torch.full((cols,), 0.75, device="cuda") if post else None
+        y, h = norm.block_norm(torch.zeros_like(x), x, post_gain=gain, scale=1.0, eps=1e-5, dtype=torch.float32)
+
+        def root(t):  # row by row: 64-bit copies of a whole matrix are large
+            return torch.stack([(r.double().square().mean() + 1e-5).sqrt() for r in t])
+        want = x.double()
+        if post:
+            want = want / root(x)[:, None] * 0.75
+        assert bool(((y.double() - want).abs() <= NORM_REL * want.abs()).all())
+        want = y.double() / root(y)[:, None]
+        assert bool(((h.double() - want).abs() <= NORM_REL * want.abs()).all())
+
+
 # ---------------------------------------------- outputs in a larger matrix --
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("m,n,k", [(130, 1, 1), (282, 2, 3), (1356, 14, 130), (202, 1396, 40), (1323, 38, 32), (605, 5157, 256),
