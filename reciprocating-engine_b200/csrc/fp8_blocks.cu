@@ -65,7 +65,7 @@ __device__ __forceinline__ f2 swiglu_far(f2 g, f2 u) {
 
 // v[i] = silu(v[i]) u[i].  The quotient is rcp's, corrected by its residual.
 // About 6 roundings in all.  Where 1 + exp(-g) nears the end of the f32 range
-// (g from about -86.9 down, and infinities and NaN), a pair that some lane has
+// (g from -86.5 down, and infinities and NaN), a pair that some lane has
 // there is formed again by swiglu_far; activations have such gates in single
 // columns (a test for each pair, then: SwiGLU of 8192 x 14336 bf16 with a gate
 // of 87 in a quarter of its warp tiles 119 us, all pairs again 127, and 114
@@ -84,7 +84,7 @@ __device__ __forceinline__ void swiglu(f2 (&v)[8], const f2 (&u)[8]) {
         const f2 r = make_f2(d0, d1), y = mul_f2(g, r), ny = mul_f2(y, make_f2(-1.0f));
         h[i] = mul_f2(fma_f2(fma_f2(ny, d, g), r, y), u[i]);
     }
-    if (__any_sync(0xffffffffu, !(top < 5.5e37f))) {
+    if (__any_sync(0xffffffffu, !(top < 3.6e37f))) {  // under exp(86.5): a value's form does not depend on its neighbours'
 #pragma unroll
         for (int i = 0; i < 8; i++) {
             float g0, g1, f0, f1, h0, h1;

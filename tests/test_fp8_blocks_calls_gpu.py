@@ -48,6 +48,17 @@ def test_swiglu_of_far_gates(dtype, cols, fmt):
     assert bool(((got - v).abs() <= bound)[alive].all())
 
 
+def test_swiglu_of_a_gate_does_not_depend_on_its_neighbours():
+    """Gates about the border of the far form, by themselves and between rows beyond it."""
+    from reng import fp8
+    gate = torch.linspace(-88, -85.5, 20000, device="cuda").reshape(-1, 1)
+    both = torch.cat([gate, torch.full_like(gate, 1e38)], 1)
+    rows = torch.cat([both, torch.tensor([[-150.0, 1.0]], device="cuda").expand(len(gate), 2)], 1).reshape(-1, 2)
+    alone = torch.cat([fp8.swiglu_quantize(b)[1] for b in both.split(1)])
+    assert torch.equal(fp8.swiglu_quantize(rows)[1][::2], alone)
+    assert torch.equal(fp8.swiglu_quantize(both)[1], alone)
+
+
 def test_swiglu_of_infinite_gates():
     from reng import fp8
     inf = float("inf")
