@@ -125,7 +125,8 @@ __device__ __forceinline__ void encode_tile(const Raw16<TYPE, G>& x, const Raw16
 // 1 x 128 groups: one warp tile of 4 consecutive groups (of any rows) each,
 // codes and scales straight from registers.  4 CTAs an SM: with the loads'
 // latency and the exponentials 3 leave issue slots free, and 5 spill (SwiGLU of
-// 8192 x 14336 bf16: 122, 117 and 132 us).
+// 8192 x 14336 bf16 on 3, 4 and 5: 122, 117 and 132 us,
+// without the far form).
 template <int TYPE, int FMT, int G, bool SWIGLU>
 __global__ void __launch_bounds__(256, 4) k_fp8_groups(GroupArgs a) {
     const uint32_t t0 = (blockIdx.x * 8 + (threadIdx.x >> 5)) * kTileGroups;
@@ -136,7 +137,7 @@ __global__ void __launch_bounds__(256, 4) k_fp8_groups(GroupArgs a) {
     uint32_t w[4];
     if constexpr (G == 4) {
         // by elements, 4 whole groups of one row (most tiles): one base address
-        // and no test (SwiGLU of 4346 x 9669 bf16: 72 us tile by tile, 62 so)
+        // and no test (SwiGLU of 4346 x 9669 bf16: 10 us of 74)
         const uint32_t row = a.per_row.div(t0), grp = t0 - row * a.per_row.d;
         if (t0 < a.blocks && grp + kTileGroups <= (uint32_t)a.cols / kFp8Group) {
             const int c = (int)(grp * kFp8Group);
